@@ -1,0 +1,205 @@
+// What the decode and the prefill attention over the block-scaled paged cache share: the cache's view, the page math on
+// warp-level matrix instructions, and the checks of their C entries.
+//
+// With x_j = scale * log2(e) * ks_j * (q . kcode_j) the output of a row is sum_j 2^x_j vs_j vcode_j / sum_j 2^x_j.  The
+// scales never touch the codes: ks_j multiplies a score, and vs_j is a power of two that goes into the exponent,
+//   M = max_j (x_j + log2 vs_j),  P_j = 2^(x_j + log2 vs_j - M) <= 1,  out = sum_j P_j vcode_j / l,  l = sum_j P_j / vs_j,
+// so that P is always fit for 16 bits whatever the blocks' magnitudes are, and a block with small values does not
+// disturb one with large ones.  Scales lie in [2^-60, 2^40] (what the store writes), which keeps l inside float32.
+//
+// Codes are converted to f16 (exact) in registers.  A query row is brought to a power of two of its own before it goes to
+// f16 (largest element in [2^14, 2^15)), so that bf16's range does not matter: elements that lose bits there are below
+// 2^-28 of the row's largest.  P is rounded to f16, 2^-12 of a weight at most; scores, M, l and the output are float32.
+#pragma once
+
+#include "common.cuh"
+
+namespace fdms {
+
+constexpr int kCachePage = 16;                  // rows per step of a warp; a block is 1, 2, 4 or 8 of them
+constexpr float kPagedLog2e = 1.4426950408889634f;
+constexpr float kPagedLn2 = 0.6931471805599453f;
+
+struct PagedCache {
+    const uint8_t* k;
+    const uint8_t* v;
+    int64_t k_sb, k_sh, k_sr, v_sb, v_sh, v_sr;     // block, head and row stride in bytes
+    const float* k_scale;                           // [blocks, heads]
+    const float* v_scale;
+    const int32_t* tables;
+    int64_t table_stride;
+    const int32_t* kv_lens;
+    int32_t* status;
+    int32_t num_blocks, max_blocks, heads, shift;   // shift: log2(block size)
+};
+
+__device__ __forceinline__ float paged_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float paged_lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Four e4m3 bytes as two f16x2: bytes 0,1 and bytes 2,3.
+__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t*)&h;
+}
+
+// Rows of a sequence that the cache really holds room for; an impossible length raises the status bit.
+__device__ __forceinline__ int paged_len(const PagedCache& c, int b) {
+    int len = c.kv_lens[b];
+    const int64_t room = (int64_t)c.max_blocks << c.shift;
+    if (len < 0 || len > room) {
+        if (c.status) atomicOr(c.status, FDMS_DEV_BAD_INDEX);
+        len = len < 0 ? 0 : (int)room;
+    }
+    return len;
+}
+
+// Power of two that brings a row with largest magnitude `top` to [2^14, 2^15), and its inverse.
+__device__ __forceinline__ void row_power(float top, float& up, float& down) {
+    const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;      // -127 for zero and subnormals, 128 for inf
+    const int k = min(max(14 - e, -100), 100);
+    up = __uint_as_float((uint32_t)(127 + k) << 23);
+    down = __uint_as_float((uint32_t)(127 - k) << 23);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
+    if (BF16) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    } else {
+        const __half2 h = *(const __half2*)&w;
+        a = __low2float(h);
+        b = __high2float(h);
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    if (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *(const uint32_t*)&h;
+    }
+    return f16x2_of(a, b);
+}
+
+// D(16x8, f32) += A(16x16, f16) B(16x8, f16), all of the fragment's rows.
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with rows 8..15 of A zero: only c0, c1 (row lane / 4) carry data.
+__device__ __forceinline__ void mma_816(float& c0, float& c1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+    float d2, d3;
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%10,%10};"
+        : "+f"(c0), "+f"(c1), "=f"(d2), "=f"(d3) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// One 16-row page as matrix operands.  Lane (g, t) = (lane / 4, lane % 4).
+//   Scores: B holds K^T.  Column c of the two 8-column tiles is key 4 (c / 2) + c % 2 and the same + 2, so that a lane's
+//   four scores are keys 4t .. 4t + 3, which is what the second product wants from it.  The k index is permuted: in chunk
+//   n (64 bytes of a row) lane t brings bytes 64 n + 16 t + [0, 16), four of them for each of four steps; a query fragment
+//   is loaded in the same order.
+//   Output: A holds P, its k index the keys in the order above; B holds V, column g of tile j being channel (D / 8) g + j,
+//   so that a lane loads D / 8 consecutive bytes of keys 4t .. 4t + 3 and ends up with consecutive channels.
+template <int D>
+struct PageRegs {
+    uint4 k[2][D / 64];         // keys a, a + 2; chunks
+    uint4 v[D == 128 ? 4 : 2];  // keys 4t .. 4t + 3, D / 8 bytes each (D = 64: two keys per vector)
+};
+
+template <int D>
+__device__ __forceinline__ void load_k(PageRegs<D>& p, const uint8_t* k, int64_t sr, int lane) {
+    const int g = lane >> 2, t = lane & 3, key = 4 * (g >> 1) + (g & 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) p.k[i][n] = __ldg((const uint4*)(k + (key + 2 * i) * sr + 64 * n + 16 * t));
+}
+template <int D>
+__device__ __forceinline__ void load_v(PageRegs<D>& p, const uint8_t* v, int64_t sr, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    if (D == 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.v[i] = __ldg((const uint4*)(v + (4 * t + i) * sr + 16 * g));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint2 a = __ldg((const uint2*)(v + (4 * t + 2 * i) * sr + 8 * g));
+            const uint2 b = __ldg((const uint2*)(v + (4 * t + 2 * i + 1) * sr + 8 * g));
+            p.v[i] = make_uint4(a.x, a.y, b.x, b.y);
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ void zero_page(PageRegs<D>& p) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) p.k[i][n] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < (D == 128 ? 4 : 2); ++i) p.v[i] = make_uint4(0, 0, 0, 0);
+}
+// Word w (channels 4w .. 4w + 3 of the lane's) of key 4t + i.
+template <int D>
+__device__ __forceinline__ uint32_t v_word(const PageRegs<D>& p, int i, int w) {
+    const uint4& x = D == 128 ? p.v[i] : p.v[i >> 1];
+    const int n = D == 128 ? w : (i & 1) * 2 + w;
+    return n == 0 ? x.x : n == 1 ? x.y : n == 2 ? x.z : x.w;
+}
+// Rows at and beyond `rows` hold whatever the memory held: zero, so that P = 0 leaves no trace of them.
+template <int D>
+__device__ __forceinline__ void mask_v(PageRegs<D>& p, int rows, int lane) {
+    const int t = lane & 3;
+    if (D == 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * t + i >= rows) p.v[i] = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (4 * t + 2 * i >= rows) p.v[i].x = p.v[i].y = 0;
+            if (4 * t + 2 * i + 1 >= rows) p.v[i].z = p.v[i].w = 0;
+        }
+    }
+}
+
+// Checks that both attention entries make, and the cache's view.
+inline int32_t paged_check(
+    const char* name, PagedCache& c, int32_t q_dtype, const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_sb, int64_t k_sh, int64_t k_sr,
+    int64_t v_sb, int64_t v_sh, int64_t v_sr, const float* k_scale, const float* v_scale, int64_t num_blocks, int32_t block_size,
+    const int32_t* tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens, int32_t num_seqs, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t* status) {
+    FDMS_REQUIRE(q_dtype == FDMS_BF16 || q_dtype == FDMS_F16, FDMS_E_DTYPE, "%s: bf16 or f16 queries only", name);
+    FDMS_REQUIRE(head_dim == 64 || head_dim == 128, FDMS_E_ARG, "%s: head_dim must be 64 or 128, got %d", name, head_dim);
+    const int shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
+    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "%s: block_size must be 16, 32, 64 or 128, got %d", name, block_size);
+    FDMS_REQUIRE(num_seqs >= 0 && num_blocks >= 0 && max_blocks >= 0 && num_kv_heads > 0 && num_q_heads > 0, FDMS_E_ARG, "%s: negative size", name);
+    FDMS_REQUIRE(num_q_heads % num_kv_heads == 0 && num_q_heads / num_kv_heads <= 64, FDMS_E_ARG,
+                 "%s: q_heads=%d must be kv_heads=%d times 1 to 64", name, num_q_heads, num_kv_heads);
+    FDMS_REQUIRE(num_blocks <= (0x7fffffffll >> shift) && max_blocks <= (0x7fffffff >> shift), FDMS_E_CAPACITY,
+                 "%s: slot numbers must fit in 31 bits", name);
+    if (num_seqs > 0) {
+        FDMS_REQUIRE(((k_cache && v_cache && k_scale && v_scale) || num_blocks == 0) && (tables || max_blocks == 0) && kv_lens, FDMS_E_ARG,
+                     "%s: null pointer", name);
+        FDMS_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)(k_sb | k_sh | k_sr | v_sb | v_sh | v_sr)) & 15) == 0, FDMS_E_ARG,
+                     "%s: cache pointers and strides must be 16-byte aligned", name);
+    }
+    c = {k_cache, v_cache, k_sb, k_sh, k_sr, v_sb, v_sh, v_sr, k_scale, v_scale, tables, bt_stride, kv_lens, status,
+         (int32_t)num_blocks, max_blocks, num_kv_heads, shift};
+    return FDMS_OK;
+}
+
+}  // namespace fdms

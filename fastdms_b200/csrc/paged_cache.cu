@@ -1,0 +1,558 @@
+// Block-scaled paged KV cache: block tables and slot maps of a step, release of blocks, and the quantising store.
+//
+// The cache holds K and V in e4m3, [blocks, kv_heads, block_size, head_dim] (block_size 16, 32, 64 or 128), with one
+// float32 scale per (block, KV head): value = code * scale.  Scales are powers of two, 2^k with k in [-60, 40], so
+// that dividing by one is exact and a code is ONE rounding of the value; a block whose later rows are louder than its
+// earlier ones moves the earlier codes to the larger scale, which is an exponent shift (exact down to e4m3's
+// subnormals).
+#include "common.cuh"
+
+namespace fdms {
+
+// ---------------------------------------------------------------------------------------------------------------
+// Tables.  held = ceil(kv / bs), need = ceil((kv + new) / bs) - held; request i takes the blocks
+// free[count - 1 - (sum of need before i) - j], j < need, if the stack reaches that far (requests are served in
+// order).  A token whose position is a multiple of bs is the first of a newly opened block, and every opened block has
+// exactly one such token: it writes the table entry, so that tokens are the only unit of work after the scan.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kScanThreads = 1024;
+constexpr int kFillThreads = 256;
+constexpr int kFillTokens = 4;                 // consecutive tokens per thread: one 16-byte store of slots
+constexpr int kFusedRequests = 1024;           // the one-launch form keeps its requests in shared memory
+
+struct MetaArgs {
+    const int32_t* new_lens;
+    const int32_t* kv_lens;
+    int32_t* kv_lens_out;
+    int32_t* tables;
+    int64_t table_stride;
+    const int32_t* free_blocks;
+    int64_t free_capacity;
+    const int32_t* free_count;
+    int32_t* free_count_out;
+    int32_t* cu_seqlens;
+    int32_t* slots;
+    int64_t* positions;
+    int32_t* status;
+    int64_t total;
+    int32_t n, max_blocks, shift;
+};
+
+// What a token needs to know of its request: rows stored before the step, and the stack index of its first block
+// (-1: the request is not served).
+struct Served {
+    int32_t kv;
+    int32_t top;
+};
+
+// Exclusive prefix sums of (blocks, tokens) over the CTA; returns the totals.
+__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& ta, int64_t& tb, int64_t* s_a, int64_t* s_b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t ia = a, ib = b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t xa = __shfl_up_sync(0xffffffffu, ia, o), xb = __shfl_up_sync(0xffffffffu, ib, o);
+        if (lane >= o) { ia += xa; ib += xb; }
+    }
+    __syncthreads();                            // the previous use of s_a / s_b is over
+    if (lane == 31) { s_a[warp] = ia; s_b[warp] = ib; }
+    __syncthreads();
+    if (warp == 0) {
+        int64_t wa = s_a[lane], wb = s_b[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t xa = __shfl_up_sync(0xffffffffu, wa, o), xb = __shfl_up_sync(0xffffffffu, wb, o);
+            if (lane >= o) { wa += xa; wb += xb; }
+        }
+        s_a[lane] = wa;
+        s_b[lane] = wb;
+    }
+    __syncthreads();
+    const int64_t ea = warp ? s_a[warp - 1] : 0, eb = warp ? s_b[warp - 1] : 0;
+    ta = s_a[31];
+    tb = s_b[31];
+    a = ea + ia - a;
+    b = eb + ib - b;
+}
+
+// Slots, positions and table entries of tokens [t0, t0 + kFillTokens).  `cu` (n + 1 prefix sums) and `req` may be in
+// shared or in global memory.
+__device__ __forceinline__ void fill_tokens(const MetaArgs& a, const int32_t* cu, const Served* req, int64_t t0) {
+    if (t0 >= a.total) return;
+    int lo = 0, hi = a.n;                       // first request whose end is beyond t0
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid + 1] > t0) hi = mid; else lo = mid + 1;
+    }
+    int32_t slot[kFillTokens];
+    int64_t pos[kFillTokens];
+    int r = lo;
+    const int mask = (1 << a.shift) - 1;
+#pragma unroll
+    for (int i = 0; i < kFillTokens; ++i) {
+        const int64_t t = t0 + i;
+        slot[i] = -1;
+        pos[i] = 0;
+        while (r < a.n && cu[r + 1] <= t) ++r;
+        if (r >= a.n || t >= a.total) continue;
+        const Served s = req[r];
+        pos[i] = (int64_t)s.kv + (t - cu[r]);
+        if (s.top < 0) continue;
+        const int32_t p = (int32_t)pos[i];      // a served request fits into its row of the table
+        const int held = (s.kv + mask) >> a.shift, col = p >> a.shift;
+        int32_t block;
+        if (col < held) {
+            block = a.tables[(int64_t)r * a.table_stride + col];
+        } else {
+            block = a.free_blocks[s.top - (col - held)];
+            if ((p & mask) == 0) a.tables[(int64_t)r * a.table_stride + col] = block;
+        }
+        slot[i] = block < 0 ? -1 : (block << a.shift) + (p & mask);
+    }
+    if (t0 + kFillTokens <= a.total) {          // slots and positions are 16-byte aligned (checked by the caller)
+        *(int4*)(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        *(longlong2*)(a.positions + t0) = make_longlong2(pos[0], pos[1]);
+        *(longlong2*)(a.positions + t0 + 2) = make_longlong2(pos[2], pos[3]);
+    } else {
+        for (int i = 0; i < kFillTokens && t0 + i < a.total; ++i) {
+            a.slots[t0 + i] = slot[i];
+            a.positions[t0 + i] = pos[i];
+        }
+    }
+}
+
+// One CTA: the scan over the requests, and with FUSED the tokens too.
+template <bool FUSED>
+__global__ void __launch_bounds__(kScanThreads) paged_scan_kernel(MetaArgs a, Served* req_out) {
+    __shared__ int64_t s_a[32], s_b[32];
+    __shared__ int32_t s_cu[FUSED ? kFusedRequests + 1 : 1];
+    __shared__ Served s_req[FUSED ? kFusedRequests : 1];
+    if (!FUSED) pdl_trigger();
+    const int64_t room = (int64_t)a.max_blocks << a.shift;
+    const int mask = (1 << a.shift) - 1;
+    int32_t count = *a.free_count;
+    bool bad = count < 0 || count > a.free_capacity;
+    if (bad) count = 0;
+    int64_t blocks_before = 0, tokens_before = 0, taken = 0;
+    int32_t* cu = FUSED ? s_cu : a.cu_seqlens;
+    Served* req = FUSED ? s_req : req_out;
+    for (int base = 0; base < a.n; base += kScanThreads) {
+        const int i = base + threadIdx.x;
+        int64_t kv = 0, add = 0, need = 0;
+        int32_t before = 0;
+        bool fits = false;
+        if (i < a.n) {
+            kv = before = a.kv_lens[i];
+            add = a.new_lens[i];
+            fits = kv >= 0 && add >= 0 && kv + add <= room;
+            if (add < 0) add = 0;
+            if (kv < 0) kv = 0;
+            if (fits) need = ((kv + add + mask) >> a.shift) - ((kv + mask) >> a.shift);
+        }
+        int64_t b0 = need, t0 = add, tb, tt;
+        block_scan2(b0, t0, tb, tt, s_a, s_b);
+        b0 += blocks_before;
+        t0 += tokens_before;
+        if (i < a.n) {
+            const bool served = fits && t0 + add <= a.total && (need == 0 || b0 + need <= count);
+            bad = bad || !fits || t0 + add > a.total;     // running out of blocks is an answer, not an error
+            req[i] = {(int32_t)kv, served ? (need ? (int32_t)(count - 1 - b0) : 0) : -1};
+            cu[i + 1] = (int32_t)min(t0 + add, a.total);
+            if (FUSED) a.cu_seqlens[i + 1] = cu[i + 1];
+            a.kv_lens_out[i] = served ? (int32_t)(kv + add) : before;
+            if (served && need) taken = max(taken, b0 + need);
+        }
+        blocks_before += tb;
+        tokens_before += tt;
+    }
+    if (threadIdx.x == 0) {
+        cu[0] = 0;
+        if (FUSED) a.cu_seqlens[0] = 0;
+    }
+    // the served requests that take blocks are the first ones that do, so the largest end is what the stack loses
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) taken = max(taken, __shfl_xor_sync(0xffffffffu, taken, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_a[threadIdx.x >> 5] = taken;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        taken = s_a[threadIdx.x];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) taken = max(taken, __shfl_xor_sync(0xffffffffu, taken, o));
+        if (threadIdx.x == 0) *a.free_count_out = count - (int32_t)taken;
+    }
+    if (bad && a.status) atomicOr(a.status, FDMS_DEV_BAD_INDEX);
+    if (FUSED)
+        for (int64_t t = (int64_t)threadIdx.x * kFillTokens; t < a.total; t += kScanThreads * kFillTokens)
+            fill_tokens(a, s_cu, s_req, t);
+}
+
+__global__ void __launch_bounds__(kFillThreads) paged_fill_kernel(MetaArgs a, const Served* req) {
+    pdl_wait();
+    fill_tokens(a, a.cu_seqlens, req, ((int64_t)blockIdx.x * kFillThreads + threadIdx.x) * kFillTokens);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Release: the blocks of the listed rows go back onto the stack in the order of the list, a row's last block lowest,
+// so that admitting a request and releasing it again leaves the stack as it was.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kReleaseThreads = 1024;
+constexpr int kReleaseRows = 4096;
+
+__global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
+    const int32_t* rows, int n, int32_t* kv_lens, int num_rows, int32_t* tables, int64_t table_stride, int max_blocks,
+    int shift, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count, int32_t* status) {
+    __shared__ int32_t s_row[kReleaseRows];     // row of each entry, -1 where it is out of range or listed before
+    __shared__ int32_t s_held[kReleaseRows];    // usable blocks of the entry, then their place on the stack
+    __shared__ int32_t s_end;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kReleaseThreads / 32;
+    bool bad = false;
+    for (int i = threadIdx.x; i < n; i += kReleaseThreads) {
+        const int r = rows ? rows[i] : i;
+        s_row[i] = r >= 0 && r < num_rows ? r : -1;
+        bad = bad || s_row[i] < 0;
+    }
+    __syncthreads();
+    for (int i = warp; i < n; i += warps) {     // a row listed twice is released once
+        const int r = s_row[i];
+        bool twice = false;
+        if (r >= 0 && rows)
+            for (int j = lane; j < i; j += 32) twice = twice || rows[j] == r;
+        twice = __any_sync(0xffffffffu, twice);
+        bad = bad || twice;
+        int held = 0;
+        if (r >= 0 && !twice) {
+            const int64_t len = max(kv_lens[r], 0);
+            const int cols = (int)min((len + (1 << shift) - 1) >> shift, (int64_t)max_blocks);
+            for (int c = lane; c < cols; c += 32) {
+                const int b = tables[(int64_t)r * table_stride + c];
+                if (b >= 0 && b < free_capacity) ++held; else bad = true;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) held += __shfl_xor_sync(0xffffffffu, held, o);
+        }
+        if (lane == 0) s_held[i] = twice ? -1 : held;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int64_t at = min((int64_t)max(*free_count, 0), free_capacity);
+        for (int i = 0; i < n; ++i) {
+            const int held = s_held[i];
+            if (held < 0) continue;
+            s_held[i] = (int32_t)at;
+            at += held;
+        }
+        if (at > free_capacity) { bad = true; at = free_capacity; }
+        s_end = (int32_t)at;
+    }
+    __syncthreads();
+    for (int i = warp; i < n; i += warps) {
+        const int r = s_row[i];
+        if (r < 0 || s_held[i] < 0) continue;
+        int64_t at = s_held[i];
+        const int64_t len = max(kv_lens[r], 0);
+        const int cols = (int)min((len + (1 << shift) - 1) >> shift, (int64_t)max_blocks);
+        for (int base = ((cols - 1) >> 5) << 5; base >= 0 && cols > 0; base -= 32) {        // last block first
+            const int c = base + 31 - lane;
+            int b = -1;
+            if (c < cols) {
+                b = tables[(int64_t)r * table_stride + c];
+                tables[(int64_t)r * table_stride + c] = -1;
+            }
+            const bool use = b >= 0 && b < free_capacity;
+            const unsigned m = __ballot_sync(0xffffffffu, use);
+            const int64_t to = at + __popc(m & ((1u << lane) - 1));
+            if (use && to < free_capacity) free_blocks[to] = b;
+            at += __popc(m);
+        }
+        __syncwarp();
+        if (lane == 0) kv_lens[r] = 0;
+    }
+    if (threadIdx.x == 0) *free_count = s_end;
+    if (bad && status) atomicOr(status, FDMS_DEV_BAD_INDEX);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Store.  A token begins a run when its slot opens a block or does not follow the token before it; a run ends with its
+// block, so that a (run, head) of K or of V is one piece of work with a scale of its own: amax over the run's rows,
+// 2^k the least with amax <= 448 * 2^k, the maximum with the block's scale where it holds earlier rows.
+// One warp per 16 rows of the block keeps its rows in registers between the two passes (amax, rounding), so that every
+// row is read once; larger blocks exchange their maxima through shared memory.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kStoreWarps = 8;
+constexpr int kScaleExpMin = -60, kScaleExpMax = 40;
+
+struct StoreArgs {
+    const uint16_t* src[2];                     // K, V
+    int64_t src_st[2], src_sh[2];               // token and head stride in elements
+    uint8_t* cache[2];
+    int64_t sb[2], sh[2], sr[2];                // block, head and row stride in bytes
+    float* scale[2];                            // [blocks, heads]
+    const int32_t* slots;
+    int32_t* status;
+    int64_t tokens;
+    int64_t num_slots;
+    int32_t heads, shift, group;                // group: tokens per CTA
+};
+
+// Exponent k of the scale for a largest magnitude.
+__device__ __forceinline__ int scale_exponent(float amax) {
+    if (!(amax > 0.0f)) return kScaleExpMin;
+    const uint32_t u = __float_as_uint(amax);
+    // amax = 1.f * 2^e <= 448 * 2^k = 1.75 * 2^(k + 8); subnormal magnitudes read as e = -127 and land on the least k
+    const int e = (int)(u >> 23) - 127;
+    const int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(k, kScaleExpMin), kScaleExpMax);
+}
+
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
+
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
+    if (BF16) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    } else {
+        const __half2 h = *(const __half2*)&w;
+        a = __low2float(h);
+        b = __high2float(h);
+    }
+}
+
+// D: head_dim.  A lane holds 8 elements of every (32 / (D / 8))-th row of the warp's 16.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kStoreWarps * 32) paged_store_kernel(StoreArgs a) {
+    constexpr int kLanes = D / 8;               // lanes per row
+    constexpr int kRows = 32 / kLanes;          // rows per step
+    constexpr int kSteps = 16 / kRows;
+    __shared__ float s_max[kStoreWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int W = (1 << a.shift) >> 4;          // warps per piece of work
+    const int per_cta = kStoreWarps / W;
+    const int item = blockIdx.y * per_cta + warp / W, part = warp % W;
+    const bool have = item < 2 * a.heads;
+    const int which = have && item >= a.heads ? 1 : 0, head = have ? item - which * a.heads : 0;
+    const int bs = 1 << a.shift;
+
+    // runs that begin in this CTA's tokens
+    const int64_t first = (int64_t)blockIdx.x * a.group;
+    int32_t my_slot = -1;
+    bool begins = false;
+    if (lane < a.group && first + lane < a.tokens) {
+        const int64_t t = first + lane;
+        my_slot = a.slots[t];
+        const int32_t prev = t > 0 ? a.slots[t - 1] : -1;
+        if (my_slot >= 0) {
+            begins = (my_slot & (bs - 1)) == 0 || prev != my_slot - 1;
+            // a slot map lists a block's tokens in order and together
+            if (my_slot >= a.num_slots || (begins && prev >= 0 && (prev >> a.shift) == (my_slot >> a.shift))) {
+                begins = false;
+                if (a.status) atomicOr(a.status, FDMS_DEV_BAD_INDEX);
+            }
+        }
+    }
+    unsigned todo = __ballot_sync(0xffffffffu, begins);
+    const int col = (lane % kLanes) * 8, row0 = lane / kLanes;
+    while (todo) {
+        const int src_lane = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int64_t t0 = first + src_lane;
+        const int32_t slot = __shfl_sync(0xffffffffu, my_slot, src_lane);
+        const int block = slot >> a.shift, off = slot & (bs - 1);
+        int count = 1;                          // rows of the run: slots that follow one another, inside the block
+        for (int base = 1; base < bs - off; base += 32) {
+            const int i = base + lane;
+            const bool on = i < bs - off && t0 + i < a.tokens && a.slots[t0 + i] == slot + i;
+            const unsigned m = __ballot_sync(0xffffffffu, on);
+            const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+            count += run;
+            if (run < 32) break;
+        }
+        uint4 x[kSteps];
+        float top = 0.0f;
+        const uint16_t* src = a.src[which] + (int64_t)head * a.src_sh[which] + col;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const int r = part * 16 + j * kRows + row0 - off;       // row of the run
+            x[j] = make_uint4(0, 0, 0, 0);
+            if (have && r >= 0 && r < count) x[j] = __ldcs((const uint4*)(src + (t0 + r) * a.src_st[which]));
+        }
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float f, g;
+                unpack2<BF16>(w[i], f, g);
+                top = fmaxf(top, fmaxf(fabsf(f), fabsf(g)));        // a NaN does not count
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float* scale = a.scale[which] + (int64_t)block * a.heads + head;
+        const float old = have && off > 0 ? *scale : 0.0f;
+        if (W > 1) {
+            if (lane == 0) s_max[warp] = top;
+            __syncthreads();
+            for (int i = 0; i < W; ++i) top = fmaxf(top, s_max[warp - part + i]);
+            __syncthreads();
+        }
+        if (!have) continue;
+        const float fresh = pow2(scale_exponent(top));
+        const float now = fmaxf(old, fresh);
+        const float inv = __frcp_rn(now);       // exact for a power of two
+        uint8_t* dst = a.cache[which] + (int64_t)block * a.sb[which] + (int64_t)head * a.sh[which] + col;
+        const bool moves = old > 0.0f && old < now;
+        const float ratio = old * inv;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const int br = part * 16 + j * kRows + row0, r = br - off;
+            uint2* p = (uint2*)(dst + (int64_t)br * a.sr[which]);
+            if (r >= 0 && r < count) {
+                const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) unpack2<BF16>(w[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] *= inv;
+                *p = make_uint2(pack_e4m3x4(f[0], f[1], f[2], f[3]), pack_e4m3x4(f[4], f[5], f[6], f[7]));
+            } else if (r < 0 && moves) {        // an earlier row of the block moves to the larger scale
+                const uint2 c = *p;
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f[i] = e4m3_to_float((uint8_t)(c.x >> (8 * i))) * ratio;
+                    f[4 + i] = e4m3_to_float((uint8_t)(c.y >> (8 * i))) * ratio;
+                }
+                *p = make_uint2(pack_e4m3x4(f[0], f[1], f[2], f[3]), pack_e4m3x4(f[4], f[5], f[6], f[7]));
+            }
+        }
+        __syncwarp();                           // every lane has read the old scale
+        if (lane == 0 && part == 0) *scale = now;
+    }
+}
+
+}  // namespace fdms
+
+using namespace fdms;
+
+static int32_t block_shift(int32_t block_size) {
+    return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
+}
+
+extern "C" int64_t fdms_paged_metadata_workspace_bytes(int32_t num_seqs) {
+    return num_seqs < 0 ? -1 : (int64_t)num_seqs * (int64_t)sizeof(Served) + 16;
+}
+
+extern "C" int32_t fdms_paged_metadata(
+    const int32_t* new_lens, const int32_t* kv_lens, int32_t* kv_lens_out, int32_t* block_tables, int64_t bt_stride,
+    int32_t max_blocks, int32_t block_size, const int32_t* free_blocks, int64_t free_capacity, const int32_t* free_count,
+    int32_t* free_count_out, int32_t* cu_seqlens, int32_t* slot_mapping, int64_t* positions, int64_t total_tokens,
+    int32_t num_seqs, void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream) {
+    clear_error();
+    FDMS_REQUIRE(free_count && free_count_out && cu_seqlens && (free_blocks || free_capacity == 0) &&
+                     ((new_lens && kv_lens && kv_lens_out && (block_tables || max_blocks == 0)) || num_seqs == 0),
+                 FDMS_E_ARG, "fdms_paged_metadata: null pointer");
+    const int32_t shift = block_shift(block_size);
+    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_metadata: block_size must be 16, 32, 64 or 128, got %d", block_size);
+    FDMS_REQUIRE(num_seqs >= 0 && max_blocks >= 0 && total_tokens >= 0 && free_capacity >= 0 && bt_stride >= max_blocks, FDMS_E_ARG,
+                 "fdms_paged_metadata: negative size, or rows of the block table overlap");
+    FDMS_REQUIRE(total_tokens == 0 || (slot_mapping && positions), FDMS_E_ARG, "fdms_paged_metadata: null pointer");
+    FDMS_REQUIRE(((uintptr_t)slot_mapping & 15) == 0 && ((uintptr_t)positions & 15) == 0, FDMS_E_ARG,
+                 "fdms_paged_metadata: slot_mapping and positions must be 16-byte aligned");
+    FDMS_REQUIRE(total_tokens < (1ll << 31) - 1 && free_capacity <= (0x7fffffffll >> shift) && max_blocks <= (0x7fffffff >> shift), FDMS_E_CAPACITY,
+                 "fdms_paged_metadata: token and slot numbers must fit in 31 bits");
+    const MetaArgs a = {new_lens, kv_lens, kv_lens_out, block_tables, bt_stride, free_blocks, free_capacity, free_count, free_count_out,
+                        cu_seqlens, slot_mapping, positions, dev_status, total_tokens, num_seqs, max_blocks, shift};
+    // One CTA does all of a decode step in one launch.  Beyond kFusedTokens its writes are what takes time, and a second
+    // launch spreads them over the GPU.
+    constexpr int64_t kFusedTokens = 4 * kScanThreads * kFillTokens;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (num_seqs <= kFusedRequests && total_tokens <= kFusedTokens) {
+        paged_scan_kernel<true><<<1, kScanThreads, 0, st>>>(a, nullptr);
+        FDMS_CHECK_LAUNCH("paged_scan_kernel");
+        return FDMS_OK;
+    }
+    FDMS_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= fdms_paged_metadata_workspace_bytes(num_seqs),
+                 FDMS_E_WORKSPACE, "fdms_paged_metadata: workspace missing, unaligned or smaller than %lld bytes",
+                 (long long)fdms_paged_metadata_workspace_bytes(num_seqs));
+    paged_scan_kernel<false><<<1, kScanThreads, 0, st>>>(a, (Served*)workspace);
+    FDMS_CHECK_LAUNCH("paged_scan_kernel");
+    if (total_tokens == 0) return FDMS_OK;
+    const int64_t per = kFillThreads * kFillTokens;
+    FDMS_CUDA_OK(launch_chained(paged_fill_kernel, dim3((unsigned)((total_tokens + per - 1) / per)), dim3(kFillThreads), st, true, a,
+                                (const Served*)workspace));
+    FDMS_CHECK_LAUNCH("paged_fill_kernel");
+    return FDMS_OK;
+}
+
+extern "C" int32_t fdms_paged_release(
+    const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
+    int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
+    int32_t* dev_status, void* stream) {
+    clear_error();
+    FDMS_REQUIRE(free_count && (free_blocks || free_capacity == 0) && ((kv_lens && (block_tables || max_blocks == 0)) || num_rows == 0), FDMS_E_ARG,
+                 "fdms_paged_release: null pointer");
+    const int32_t shift = block_shift(block_size);
+    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_release: block_size must be 16, 32, 64 or 128, got %d", block_size);
+    FDMS_REQUIRE(num_listed >= 0 && num_rows >= 0 && max_blocks >= 0 && free_capacity >= 0 && bt_stride >= max_blocks, FDMS_E_ARG,
+                 "fdms_paged_release: negative size, or rows of the block table overlap");
+    FDMS_REQUIRE(rows || num_listed <= num_rows, FDMS_E_ARG, "fdms_paged_release: more rows than the block table has");
+    FDMS_REQUIRE(num_listed <= kReleaseRows && free_capacity <= (0x7fffffffll >> shift), FDMS_E_CAPACITY,
+                 "fdms_paged_release: at most %d rows a call, and slot numbers must fit in 31 bits", kReleaseRows);
+    if (num_listed == 0) return FDMS_OK;
+    paged_release_kernel<<<1, kReleaseThreads, 0, (cudaStream_t)stream>>>(rows, num_listed, kv_lens, num_rows, block_tables, bt_stride,
+                                                                         max_blocks, shift, free_blocks, free_capacity, free_count, dev_status);
+    FDMS_CHECK_LAUNCH("paged_release_kernel");
+    return FDMS_OK;
+}
+
+extern "C" int32_t fdms_paged_store(
+    const void* k, const void* v, int32_t act_dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+    uint8_t* k_cache, uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
+    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, float* k_scale, float* v_scale,
+    const int32_t* slot_mapping, int64_t tokens, int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+    int32_t* dev_status, void* stream) {
+    clear_error();
+    FDMS_REQUIRE(act_dtype == FDMS_BF16 || act_dtype == FDMS_F16, FDMS_E_DTYPE, "fdms_paged_store: bf16 or f16 activations only");
+    const int32_t shift = block_shift(block_size);
+    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_store: block_size must be 16, 32, 64 or 128, got %d", block_size);
+    FDMS_REQUIRE(head_dim == 64 || head_dim == 128, FDMS_E_ARG, "fdms_paged_store: head_dim must be 64 or 128, got %d", head_dim);
+    FDMS_REQUIRE(tokens >= 0 && num_blocks >= 0 && num_kv_heads > 0, FDMS_E_ARG, "fdms_paged_store: negative size");
+    if (tokens == 0) return FDMS_OK;
+    FDMS_REQUIRE(k && v && k_cache && v_cache && k_scale && v_scale && slot_mapping, FDMS_E_ARG, "fdms_paged_store: null pointer");
+    FDMS_REQUIRE(num_blocks <= (0x7fffffffll >> shift) && num_kv_heads <= 4096, FDMS_E_CAPACITY,
+                 "fdms_paged_store: slot numbers must fit in 31 bits, and at most 4096 KV heads");
+    const uintptr_t act = (uintptr_t)k | (uintptr_t)v | (uintptr_t)(2 * (k_stride_t | k_stride_h | v_stride_t | v_stride_h));
+    const uintptr_t cached = (uintptr_t)k_cache | (uintptr_t)v_cache |
+                             (uintptr_t)(k_stride_b | k_stride_hd | k_stride_r | v_stride_b | v_stride_hd | v_stride_r);
+    FDMS_REQUIRE((act & 15) == 0 && (cached & 15) == 0, FDMS_E_ARG, "fdms_paged_store: pointers and strides must be 16-byte aligned");
+    const int W = block_size / 16, per_cta = kStoreWarps / W;
+    // Tokens per CTA: few runs begin in a prompt's tokens, one at every token of a decode batch.  1024 CTAs keep the GPU
+    // busy either way; more than a block's worth of tokens per CTA would only make them unequal.
+    int group = 1;
+    while (group < 16 && tokens > (int64_t)group * 1024) group *= 2;
+    StoreArgs a = {{(const uint16_t*)k, (const uint16_t*)v}, {k_stride_t, v_stride_t}, {k_stride_h, v_stride_h}, {k_cache, v_cache},
+                   {k_stride_b, v_stride_b}, {k_stride_hd, v_stride_hd}, {k_stride_r, v_stride_r}, {k_scale, v_scale}, slot_mapping,
+                   dev_status, tokens, num_blocks << shift, num_kv_heads, shift, group};
+    const int64_t ctas = (tokens + group - 1) / group;
+    FDMS_REQUIRE(ctas < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_store: too many tokens");
+    const dim3 grid((unsigned)ctas, (unsigned)((2 * num_kv_heads + per_cta - 1) / per_cta));
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool bf = act_dtype == FDMS_BF16;
+    if (head_dim == 64) {
+        if (bf) paged_store_kernel<64, true><<<grid, kStoreWarps * 32, 0, st>>>(a);
+        else paged_store_kernel<64, false><<<grid, kStoreWarps * 32, 0, st>>>(a);
+    } else {
+        if (bf) paged_store_kernel<128, true><<<grid, kStoreWarps * 32, 0, st>>>(a);
+        else paged_store_kernel<128, false><<<grid, kStoreWarps * 32, 0, st>>>(a);
+    }
+    FDMS_CHECK_LAUNCH("paged_store_kernel");
+    return FDMS_OK;
+}

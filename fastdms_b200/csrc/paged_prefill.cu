@@ -1,0 +1,277 @@
+// Prefill attention over the block-scaled paged cache: the tokens of a step, packed sequence by sequence, against their
+// sequence's cached rows.  Token i of a sequence with n tokens in the step and kv rows in the cache sees rows
+// 0 .. kv - n + i; a token that sees no row gets zeros and a log-sum-exp of -inf.
+#include "paged_attn.cuh"
+
+namespace fdms {
+
+constexpr int kPreWarps = 4;
+constexpr int kPreRows = kPreWarps * 16;        // (token, q head) rows of a CTA, heads of a token together
+
+struct PrefillArgs {
+    PagedCache c;
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;                                 // optional [q_heads, tokens]
+    const int32_t* cu;                          // [seqs + 1]
+    int64_t q_st, q_sh, o_st, o_sh, lse_sh, lse_st;
+    int64_t tokens;
+    int32_t seqs, group;
+    float scale;
+};
+
+// Sequence and first token (within the sequence) of tile x, tiles of `per` tokens; false beyond the last tile.  Every warp
+// finds it for itself: 32 sequences at a time.
+__device__ __forceinline__ bool find_tile(const PrefillArgs& a, int64_t x, int per, int& seq, int64_t& first, int64_t& begin, int64_t& count) {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < a.seqs; base += 32) {
+        const int s = base + lane;
+        int64_t b = 0, e = 0;
+        if (s < a.seqs) {
+            b = min(max((int64_t)a.cu[s], (int64_t)0), a.tokens);
+            e = min(max((int64_t)a.cu[s + 1], b), a.tokens);
+        }
+        const int64_t tiles = (e - b + per - 1) / per;
+        int64_t sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, sum > x);
+        if (m) {
+            const int l = __ffs(m) - 1;
+            seq = base + l;
+            first = (x - __shfl_sync(0xffffffffu, sum - tiles, l)) * per;
+            begin = __shfl_sync(0xffffffffu, b, l);
+            count = __shfl_sync(0xffffffffu, e - b, l);
+            return true;
+        }
+        x -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kPreWarps * 32) paged_prefill_kernel(PrefillArgs a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int per = kPreRows / a.group;         // tokens per tile
+    int seq;
+    int64_t first, begin, count;
+    // the last tiles of a sequence see the most rows: they start first
+    if (!find_tile(a, (int64_t)gridDim.x - 1 - blockIdx.x, per, seq, first, begin, count)) return;
+    const int head = blockIdx.y;
+    const int kv = paged_len(a.c, seq);
+    // this lane's rows
+    int64_t tok[2], last[2];                    // token of the step, last cached row it sees
+    int hq[2];
+    bool live[2];
+    float up[2], factor[2];
+    uint32_t qa[D / 16][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = warp * 16 + g + 8 * i;
+        const int64_t j = first + r / a.group;
+        live[i] = r < per * a.group && j < count;
+        tok[i] = begin + (live[i] ? j : first);
+        hq[i] = head * a.group + (live[i] ? r % a.group : 0);
+        last[i] = live[i] ? (int64_t)kv - count + j : -1;
+        const uint16_t* q = a.q + tok[i] * a.q_st + (int64_t)hq[i] * a.q_sh;
+        uint4 w[D / 64][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                w[n][k] = *(const uint4*)(q + 64 * n + 16 * t + 8 * k);
+                const uint32_t x[4] = {w[n][k].x, w[n][k].y, w[n][k].z, w[n][k].w};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    float e, f;
+                    unpack_pair<BF16>(x[v], e, f);
+                    top = fmaxf(top, fmaxf(fabsf(e), fabsf(f)));
+                }
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        row_power(top, up[i], factor[i]);
+        factor[i] *= a.scale * kPagedLog2e;
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t x[4] = {w[n][k].x, w[n][k].y, w[n][k].z, w[n][k].w};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    float e, f;
+                    unpack_pair<BF16>(x[v], e, f);
+                    qa[4 * n + 2 * k + (v >> 1)][2 * (v & 1) + i] = f16x2_of(e * up[i], f * up[i]);
+                }
+            }
+    }
+    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    int64_t most = max(last[0], last[1]);
+    int64_t least = min(live[0] ? last[0] : (int64_t)kv, live[1] ? last[1] : (int64_t)kv);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, s));
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, s));
+    }
+    const int pages = (int)((most + kCachePage) / kCachePage);
+    const int ppb = a.c.shift - 4;
+    for (int p = 0; p < pages; ++p) {
+        const int blk = a.c.tables[seq * a.c.table_stride + (p >> ppb)];
+        if (blk < 0 || blk >= a.c.num_blocks) {
+            if (lane == 0 && a.c.status) atomicOr(a.c.status, FDMS_DEV_BAD_INDEX);
+            continue;
+        }
+        const int row = (p & ((1 << ppb) - 1)) * kCachePage;
+        PageRegs<D> pg;
+        const uint8_t* vp = a.c.v + (int64_t)blk * a.c.v_sb + head * a.c.v_sh + row * a.c.v_sr;
+        load_k<D>(pg, a.c.k + (int64_t)blk * a.c.k_sb + head * a.c.k_sh + row * a.c.k_sr, a.c.k_sr, lane);
+        load_v<D>(pg, vp, a.c.v_sr, lane);
+        const float ks = a.c.k_scale[(int64_t)blk * a.c.heads + head], vs = a.c.v_scale[(int64_t)blk * a.c.heads + head];
+        const float lvs = paged_lg2(vs), ivs = __frcp_rn(vs);
+        float s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};       // keys 4t, 4t + 1 and 4t + 2, 4t + 3 of rows g and g + 8
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t(&q4)[4] = qa[4 * c + j];
+                uint32_t b0, b1;
+                e4m3x4_f16(j == 0 ? pg.k[0][c].x : j == 1 ? pg.k[0][c].y : j == 2 ? pg.k[0][c].z : pg.k[0][c].w, b0, b1);
+                mma_16816(s0, q4[0], q4[1], q4[2], q4[3], b0, b1);
+                e4m3x4_f16(j == 0 ? pg.k[1][c].x : j == 1 ? pg.k[1][c].y : j == 2 ? pg.k[1][c].z : pg.k[1][c].w, b0, b1);
+                mma_16816(s1, q4[0], q4[1], q4[2], q4[3], b0, b1);
+            }
+        uint32_t pa[4];
+        const int key = p * kCachePage + 4 * t;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float s[4] = {s0[2 * i], s0[2 * i + 1], s1[2 * i], s1[2 * i + 1]}, top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[j] = key + j <= last[i] ? fmaf(s[j], ks * factor[i], lvs) : -INFINITY;
+                top = fmaxf(top, s[j]);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (__any_sync(0xffffffffu, top > m[i] + 8.0f)) {
+                const float next = fmaxf(m[i], top);
+                const float r = next == -INFINITY ? 1.0f : paged_ex2(m[i] - next);
+                m[i] = next;
+                l[i] *= r;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) { o[j][2 * i] *= r; o[j][2 * i + 1] *= r; }
+            }
+            const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] = paged_ex2(s[j] - ref);
+            l[i] = fmaf((s[0] + s[1]) + (s[2] + s[3]), ivs, l[i]);
+            pa[i] = f16x2_of(s[0], s[1]);
+            pa[2 + i] = f16x2_of(s[2], s[3]);
+        }
+        if ((p + 1) * kCachePage > least + 1) {
+            // Some row does not see all of the page.  What it does not see may be anything, a NaN code among it: such
+            // codes count as zero in the product and are put into the rows that do see them.
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w) {
+                    const uint32_t x = v_word<D>(pg, i, w) & 0x7f7f7f7fu;
+                    odd = odd || ((x + 0x01010101u) & 0x80808080u) != 0;
+                }
+            if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+                for (int i = 0; i < (D == 128 ? 4 : 2); ++i) {
+                    uint32_t* x = (uint32_t*)&pg.v[i];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t nan = ((x[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;      // top bit of each NaN byte
+                        x[w] &= ~((nan >> 7) * 0xffu);
+                    }
+                }
+                for (int k = 0; k < kCachePage; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (p * kCachePage + k <= last[i])
+#pragma unroll
+                            for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                                for (int n = 0; n < 2; ++n)
+                                    if ((vp[k * a.c.v_sr + (D / 8) * (2 * t + n) + j] & 0x7f) == 0x7f) o[j][2 * i + n] = NAN;
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+            const uint32_t k0 = v_word<D>(pg, 0, w), k1 = v_word<D>(pg, 1, w), k2 = v_word<D>(pg, 2, w), k3 = v_word<D>(pg, 3, w);
+            uint32_t b0[4], b1[4];
+            e4m3x4_f16(__byte_perm(k0, k1, 0x5140), b0[0], b0[1]);
+            e4m3x4_f16(__byte_perm(k0, k1, 0x7362), b0[2], b0[3]);
+            e4m3x4_f16(__byte_perm(k2, k3, 0x5140), b1[0], b1[1]);
+            e4m3x4_f16(__byte_perm(k2, k3, 0x7362), b1[2], b1[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_16816(o[4 * w + j], pa[0], pa[1], pa[2], pa[3], b0[j], b1[j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (!live[i]) continue;
+        const float inv = l[i] > 0.0f || l[i] != l[i] ? __frcp_rn(l[i]) : 0.0f;
+        uint16_t* out = a.out + tok[i] * a.o_st + (int64_t)hq[i] * a.o_sh;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int j = 0; j < D / 8; j += 2)
+                *(uint32_t*)(out + (D / 8) * (2 * t + n) + j) = pack_pair<BF16>(o[j][2 * i + n] * inv, o[j + 1][2 * i + n] * inv);
+        if (a.lse && t == 0) a.lse[(int64_t)hq[i] * a.lse_sh + tok[i] * a.lse_st] = kPagedLn2 * (m[i] + paged_lg2(l[i]));
+    }
+}
+
+}  // namespace fdms
+
+using namespace fdms;
+
+extern "C" int32_t fdms_paged_attn_prefill(
+    const void* q, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h,
+    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
+    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
+    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
+    const int32_t* cu_seqlens_q, int64_t tokens, void* out, int64_t out_stride_t, int64_t out_stride_h,
+    float* lse_out, int64_t lse_stride_h, int64_t lse_stride_t,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale, int32_t* dev_status, void* stream) {
+    clear_error();
+    PagedCache c;
+    const int32_t rc = paged_check("fdms_paged_attn_prefill", c, q_dtype, k_cache, v_cache, k_stride_b, k_stride_hd, k_stride_r, v_stride_b,
+                                   v_stride_hd, v_stride_r, k_scale, v_scale, num_blocks, block_size, block_tables, bt_stride, max_blocks, kv_lens,
+                                   num_seqs, num_q_heads, num_kv_heads, head_dim, dev_status);
+    if (rc != FDMS_OK) return rc;
+    FDMS_REQUIRE(tokens >= 0, FDMS_E_ARG, "fdms_paged_attn_prefill: negative size");
+    if (num_seqs == 0 || tokens == 0) return FDMS_OK;
+    FDMS_REQUIRE(q && out && cu_seqlens_q, FDMS_E_ARG, "fdms_paged_attn_prefill: null pointer");
+    FDMS_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)(2 * (q_stride_t | q_stride_h | out_stride_t | out_stride_h))) & 15) == 0, FDMS_E_ARG,
+                 "fdms_paged_attn_prefill: q and out pointers and strides must be 16-byte aligned");
+    FDMS_REQUIRE(num_kv_heads <= 65535, FDMS_E_CAPACITY, "fdms_paged_attn_prefill: at most 65535 KV heads");
+    const int group = num_q_heads / num_kv_heads;
+    PrefillArgs a = {c, (const uint16_t*)q, (uint16_t*)out, lse_out, cu_seqlens_q, q_stride_t, q_stride_h, out_stride_t, out_stride_h,
+                     lse_stride_h, lse_stride_t, tokens, num_seqs, group, scale};
+    const int64_t tiles = tokens / (kPreRows / group) + num_seqs;
+    FDMS_REQUIRE(tokens < (1ll << 31) && tiles < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_prefill: too many tokens");
+    const dim3 grid((unsigned)tiles, (unsigned)num_kv_heads);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool bf = q_dtype == FDMS_BF16;
+    if (head_dim == 64) {
+        if (bf) paged_prefill_kernel<64, true><<<grid, kPreWarps * 32, 0, st>>>(a);
+        else paged_prefill_kernel<64, false><<<grid, kPreWarps * 32, 0, st>>>(a);
+    } else {
+        if (bf) paged_prefill_kernel<128, true><<<grid, kPreWarps * 32, 0, st>>>(a);
+        else paged_prefill_kernel<128, false><<<grid, kPreWarps * 32, 0, st>>>(a);
+    }
+    FDMS_CHECK_LAUNCH("paged_prefill_kernel");
+    return FDMS_OK;
+}

@@ -487,6 +487,73 @@ int32_t fdms_linear_decode_allreduce(
     void* y, int64_t y_row_stride, int32_t dtype, int32_t rows, int32_t out_features, int32_t in_features,
     void* const* peer_regions, int32_t rank, int32_t world, int32_t* dev_status, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * (f) dense paged KV cache in 8 bits with a scale for each block of tokens and KV head, for models that are
+ * served without eviction (the reference's dense branch keeps its cache in the model's type and quantises with one
+ * scale, fastdms/layers/attention.py:85-123).
+ * K and V of a layer: e4m3 [num_blocks, kv_heads, block_size, head_dim], block, head and row stride in bytes
+ * (multiples of 16; rows contiguous), block_size 16, 32, 64 or 128, head_dim 64 or 128; scales float32
+ * [num_blocks, kv_heads], powers of two in [2^-60, 2^40]: value = code * scale.  Row r of a sequence is row
+ * r % block_size of block block_tables[s * bt_stride + r / block_size].  Slots and lengths are int32, so a pool holds
+ * fewer than 2^31 rows.
+ *
+ * fdms_paged_metadata: sequence i holds kv_lens[i] rows and gets new_lens[i] more.  The blocks it needs are popped from
+ *   free_blocks[0 .. free_count) (the top is the end) into its row of the table, in the order of the sequences; where the
+ *   stack runs out a sequence and the later ones that need blocks are not served: slots -1, length and table as before.
+ *   cu_seqlens [num_seqs + 1] = prefix sums of new_lens; slot_mapping and positions [total_tokens], 16-byte aligned
+ *   (tokens behind the last: -1 and 0).  kv_lens_out / free_count_out may be kv_lens / free_count.  A negative length, one
+ *   beyond max_blocks * block_size, or more tokens than total_tokens is not served and raises FDMS_DEV_BAD_INDEX.
+ *   workspace: fdms_paged_metadata_workspace_bytes(num_seqs) bytes, 8-byte aligned, any contents.
+ * fdms_paged_release: the blocks of rows[0 .. num_listed) (NULL: rows 0 .. num_listed) return to the stack; their
+ *   table entries become -1 and their lengths 0.  At most 4096 rows; a row listed twice is released once.
+ * fdms_paged_store: k, v [tokens, kv_heads, head_dim] (bf16 / f16, strides in elements, 16-byte aligned) into the rows of
+ *   slot_mapping (negative: skipped).  Per block and head: the scale is the least 2^k with |x| <= 448 * 2^k over the rows
+ *   written, not below the scale of a block that holds earlier rows, whose codes then move to the new scale.  A sequence's
+ *   tokens are consecutive; no block is written by two sequences.
+ * fdms_paged_attn_decode: out[b, hq] = softmax(scale * q[b, hq] K^T) V over the first kv_lens[b] rows, q [batch, q_heads,
+ *   head_dim]; no rows: zeros.  lse_out (optional): natural-log log-sum-exp, -inf without rows.  batch <= 2048.
+ *   workspace: fdms_paged_attn_decode_workspace_bytes(...) bytes of the current device, 16-byte aligned, any contents; calls
+ *   that share one must not overlap on the GPU.
+ * fdms_paged_attn_prefill: q [tokens, q_heads, head_dim], sequence s's tokens at cu_seqlens_q[s] .. cu_seqlens_q[s + 1];
+ *   with n of them, token i sees rows 0 .. kv_lens[s] - n + i (none: zeros, lse -inf).  Tokens behind the last sequence
+ *   are left untouched.
+ * Both attentions: q_heads = kv_heads times 1 to 64, bf16 / f16; a needed table entry outside [0, num_blocks) is left out
+ * and raises FDMS_DEV_BAD_INDEX, as does a length beyond the table.
+ * --------------------------------------------------------------------------------------------- */
+int64_t fdms_paged_metadata_workspace_bytes(int32_t num_seqs);
+int32_t fdms_paged_metadata(
+    const int32_t* new_lens, const int32_t* kv_lens, int32_t* kv_lens_out, int32_t* block_tables, int64_t bt_stride,
+    int32_t max_blocks, int32_t block_size, const int32_t* free_blocks, int64_t free_capacity, const int32_t* free_count,
+    int32_t* free_count_out, int32_t* cu_seqlens, int32_t* slot_mapping, int64_t* positions, int64_t total_tokens,
+    int32_t num_seqs, void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream);
+int32_t fdms_paged_release(
+    const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
+    int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
+    int32_t* dev_status, void* stream);
+int32_t fdms_paged_store(
+    const void* k, const void* v, int32_t act_dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+    uint8_t* k_cache, uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
+    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, float* k_scale, float* v_scale,
+    const int32_t* slot_mapping, int64_t tokens, int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+    int32_t* dev_status, void* stream);
+int64_t fdms_paged_attn_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
+int32_t fdms_paged_attn_decode(
+    const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
+    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
+    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
+    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
+    void* out, int64_t out_stride_b, int64_t out_stride_h, float* lse_out, int64_t lse_stride_b, int64_t lse_stride_h,
+    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream);
+int32_t fdms_paged_attn_prefill(
+    const void* q, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h,
+    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
+    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
+    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
+    const int32_t* cu_seqlens_q, int64_t tokens, void* out, int64_t out_stride_t, int64_t out_stride_h,
+    float* lse_out, int64_t lse_stride_h, int64_t lse_stride_t,
+    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale, int32_t* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
