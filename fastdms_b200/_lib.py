@@ -79,16 +79,13 @@ _SIGNATURES = {
     "fdms_linear_decode_fp8": (I32, [P, I64, P, I64, P, P, P, I64, I32, I32, I32, I32, P]),
     "fdms_linear_allreduce_region_bytes": (I64, [I32]),
     "fdms_linear_decode_allreduce": (I32, [P, I64, P, I64, P, P, I64, I32, I32, I32, I32, P, I32, I32, P, P]),
-    "fdms_paged_metadata_workspace_bytes": (I64, [I32]),
-    "fdms_paged_metadata": (I32, [P, P, P, P, I64, I32, I32, P, I64, P, P, P, P, P, I64, I32, P, I64, P, P]),
+    "fdms_paged_metadata_workspace_bytes": (I64, [I64, I64]),
+    "fdms_paged_metadata": (I32, [c_char_p, P]),
     "fdms_paged_release": (I32, [P, I32, P, I32, P, I64, I32, I32, P, I64, P, P, P]),
-    "fdms_paged_store": (I32, [P, P, I32, I64, I64, I64, I64, P, P, I64, I64, I64, I64, I64, I64, P, P, P, I64, I64,
-                               I32, I32, I32, P, P]),
+    "fdms_paged_store": (I32, [c_char_p, P]),
     "fdms_paged_attn_decode_workspace_bytes": (I64, [I32, I32, I32, I32]),
-    "fdms_paged_attn_decode": (I32, [P, I32, I64, I64, P, P, I64, I64, I64, I64, I64, I64, P, P, I64, I32, P, I64, I32, P,
-                                     P, I64, I64, P, I64, I64, I32, I32, I32, I32, F, P, I64, P, P]),
-    "fdms_paged_attn_prefill": (I32, [P, I32, I64, I64, P, P, I64, I64, I64, I64, I64, I64, P, P, I64, I32, P, I64, I32, P,
-                                      P, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, F, P, P]),
+    "fdms_paged_attn_decode": (I32, [c_char_p, P]),
+    "fdms_paged_attn_prefill": (I32, [c_char_p, P]),
 }
 
 _lib = None

@@ -176,29 +176,44 @@ __device__ __forceinline__ void mask_v(PageRegs<D>& p, int rows, int lane) {
     }
 }
 
+// Checks of a cache that every entry makes; `idle`: the call has nothing to do, so its pointers may be null.
+inline int32_t paged_cache_check(const char* name, const fdms_paged_cache& c, int64_t dtype, bool idle, int32_t& shift) {
+    FDMS_REQUIRE(dtype == FDMS_BF16 || dtype == FDMS_F16, FDMS_E_DTYPE, "%s: bf16 or f16 activations only", name);
+    FDMS_REQUIRE(c.head_dim == 64 || c.head_dim == 128, FDMS_E_ARG, "%s: head_dim must be 64 or 128, got %lld", name, (long long)c.head_dim);
+    shift = c.block_size == 16 ? 4 : c.block_size == 32 ? 5 : c.block_size == 64 ? 6 : c.block_size == 128 ? 7 : -1;
+    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "%s: block_size must be 16, 32, 64 or 128, got %lld", name, (long long)c.block_size);
+    FDMS_REQUIRE(c.num_blocks >= 0 && c.kv_heads > 0, FDMS_E_ARG, "%s: negative size, or no KV heads", name);
+    FDMS_REQUIRE(c.num_blocks <= (0x7fffffff >> shift) && c.kv_heads <= 4096, FDMS_E_CAPACITY,
+                 "%s: slot numbers must fit in 31 bits, and at most 4096 KV heads", name);
+    if (idle || c.num_blocks == 0) return FDMS_OK;
+    FDMS_REQUIRE(c.k && c.v && c.k_scale && c.v_scale, FDMS_E_ARG, "%s: null pointer", name);
+    const int64_t strides = c.k_stride[0] | c.k_stride[1] | c.k_stride[2] | c.v_stride[0] | c.v_stride[1] | c.v_stride[2];
+    FDMS_REQUIRE((((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)strides) & 15) == 0 && c.k_stride[3] == 1 && c.v_stride[3] == 1, FDMS_E_ARG,
+                 "%s: the cache must be contiguous in its last dimension and aligned to 16 bytes in the others", name);
+    return FDMS_OK;
+}
+
 // Checks that both attention entries make, and the cache's view.
-inline int32_t paged_check(
-    const char* name, PagedCache& c, int32_t q_dtype, const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_sb, int64_t k_sh, int64_t k_sr,
-    int64_t v_sb, int64_t v_sh, int64_t v_sr, const float* k_scale, const float* v_scale, int64_t num_blocks, int32_t block_size,
-    const int32_t* tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens, int32_t num_seqs, int32_t num_q_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t* status) {
-    FDMS_REQUIRE(q_dtype == FDMS_BF16 || q_dtype == FDMS_F16, FDMS_E_DTYPE, "%s: bf16 or f16 queries only", name);
-    FDMS_REQUIRE(head_dim == 64 || head_dim == 128, FDMS_E_ARG, "%s: head_dim must be 64 or 128, got %d", name, head_dim);
-    const int shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
-    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "%s: block_size must be 16, 32, 64 or 128, got %d", name, block_size);
-    FDMS_REQUIRE(num_seqs >= 0 && num_blocks >= 0 && max_blocks >= 0 && num_kv_heads > 0 && num_q_heads > 0, FDMS_E_ARG, "%s: negative size", name);
-    FDMS_REQUIRE(num_q_heads % num_kv_heads == 0 && num_q_heads / num_kv_heads <= 64, FDMS_E_ARG,
-                 "%s: q_heads=%d must be kv_heads=%d times 1 to 64", name, num_q_heads, num_kv_heads);
-    FDMS_REQUIRE(num_blocks <= (0x7fffffffll >> shift) && max_blocks <= (0x7fffffff >> shift), FDMS_E_CAPACITY,
-                 "%s: slot numbers must fit in 31 bits", name);
-    if (num_seqs > 0) {
-        FDMS_REQUIRE(((k_cache && v_cache && k_scale && v_scale) || num_blocks == 0) && (tables || max_blocks == 0) && kv_lens, FDMS_E_ARG,
-                     "%s: null pointer", name);
-        FDMS_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)(k_sb | k_sh | k_sr | v_sb | v_sh | v_sr)) & 15) == 0, FDMS_E_ARG,
-                     "%s: cache pointers and strides must be 16-byte aligned", name);
+inline int32_t paged_attn_check(const char* name, const fdms_paged_attn_args* args, PagedCache& view, bool idle) {
+    FDMS_REQUIRE(args, FDMS_E_ARG, "%s: null pointer", name);
+    const fdms_paged_attn_args& p = *args;
+    const fdms_paged_cache& c = p.cache;
+    int32_t shift = 0;
+    const int32_t rc = paged_cache_check(name, c, p.dtype, idle, shift);
+    if (rc != FDMS_OK) return rc;
+    FDMS_REQUIRE(p.tokens >= 0 && p.num_seqs >= 0 && p.max_blocks >= 0 && p.num_q_heads > 0, FDMS_E_ARG, "%s: negative size", name);
+    FDMS_REQUIRE(p.num_q_heads % c.kv_heads == 0 && p.num_q_heads / c.kv_heads <= 64, FDMS_E_ARG, "%s: q_heads=%lld must be kv_heads=%lld times 1 to 64",
+                 name, (long long)p.num_q_heads, (long long)c.kv_heads);
+    FDMS_REQUIRE(p.max_blocks <= (0x7fffffff >> shift) && p.tokens < 0x7fffffff && p.num_seqs < 0x7fffffff, FDMS_E_CAPACITY,
+                 "%s: token and slot numbers must fit in 31 bits", name);
+    if (!idle) {
+        FDMS_REQUIRE(p.q && p.out && p.kv_lens && (p.block_tables || p.max_blocks == 0), FDMS_E_ARG, "%s: null pointer", name);
+        const int64_t strides = p.q_stride[0] | p.q_stride[1] | p.out_stride[0] | p.out_stride[1];
+        FDMS_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)(2 * strides)) & 15) == 0 && p.q_stride[2] == 1 && p.out_stride[2] == 1, FDMS_E_ARG,
+                     "%s: q and out must be contiguous in their last dimension and aligned to 16 bytes in the others", name);
     }
-    c = {k_cache, v_cache, k_sb, k_sh, k_sr, v_sb, v_sh, v_sr, k_scale, v_scale, tables, bt_stride, kv_lens, status,
-         (int32_t)num_blocks, max_blocks, num_kv_heads, shift};
+    view = {c.k, c.v, c.k_stride[0], c.k_stride[1], c.k_stride[2], c.v_stride[0], c.v_stride[1], c.v_stride[2], c.k_scale, c.v_scale,
+            p.block_tables, p.bt_stride, p.kv_lens, p.dev_status, (int32_t)c.num_blocks, (int32_t)p.max_blocks, (int32_t)c.kv_heads, shift};
     return FDMS_OK;
 }
 

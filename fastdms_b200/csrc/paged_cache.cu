@@ -5,7 +5,7 @@
 // that dividing by one is exact and a code is ONE rounding of the value; a block whose later rows are louder than its
 // earlier ones moves the earlier codes to the larger scale, which is an exponent shift (exact down to e4m3's
 // subnormals).
-#include "common.cuh"
+#include "paged_attn.cuh"
 
 namespace fdms {
 
@@ -442,52 +442,54 @@ __global__ void __launch_bounds__(kStoreWarps * 32) paged_store_kernel(StoreArgs
 
 using namespace fdms;
 
-static int32_t block_shift(int32_t block_size) {
+static int32_t block_shift(int64_t block_size) {
     return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
 }
 
-extern "C" int64_t fdms_paged_metadata_workspace_bytes(int32_t num_seqs) {
-    return num_seqs < 0 ? -1 : (int64_t)num_seqs * (int64_t)sizeof(Served) + 16;
+// One CTA does all of a decode step in one launch.  Beyond kFusedTokens its writes are what takes time, and a second
+// launch spreads them over the GPU.
+constexpr int64_t kFusedTokens = 4 * kScanThreads * kFillTokens;
+static bool metadata_fused(int64_t num_seqs, int64_t total_tokens) { return num_seqs <= kFusedRequests && total_tokens <= kFusedTokens; }
+
+extern "C" int64_t fdms_paged_metadata_workspace_bytes(int64_t num_seqs, int64_t total_tokens) {
+    if (num_seqs < 0 || total_tokens < 0) return -1;
+    return metadata_fused(num_seqs, total_tokens) ? 0 : num_seqs * (int64_t)sizeof(Served);
 }
 
-extern "C" int32_t fdms_paged_metadata(
-    const int32_t* new_lens, const int32_t* kv_lens, int32_t* kv_lens_out, int32_t* block_tables, int64_t bt_stride,
-    int32_t max_blocks, int32_t block_size, const int32_t* free_blocks, int64_t free_capacity, const int32_t* free_count,
-    int32_t* free_count_out, int32_t* cu_seqlens, int32_t* slot_mapping, int64_t* positions, int64_t total_tokens,
-    int32_t num_seqs, void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream) {
+extern "C" int32_t fdms_paged_metadata(const fdms_paged_metadata_args* args, void* stream) {
     clear_error();
-    FDMS_REQUIRE(free_count && free_count_out && cu_seqlens && (free_blocks || free_capacity == 0) &&
-                     ((new_lens && kv_lens && kv_lens_out && (block_tables || max_blocks == 0)) || num_seqs == 0),
+    FDMS_REQUIRE(args, FDMS_E_ARG, "fdms_paged_metadata: null pointer");
+    const fdms_paged_metadata_args& p = *args;
+    FDMS_REQUIRE(p.free_count && p.free_count_out && p.cu_seqlens && (p.free_blocks || p.free_capacity == 0) &&
+                     ((p.new_lens && p.kv_lens && p.kv_lens_out && (p.block_tables || p.max_blocks == 0)) || p.num_seqs == 0) &&
+                     ((p.slot_mapping && p.positions) || p.total_tokens == 0),
                  FDMS_E_ARG, "fdms_paged_metadata: null pointer");
-    const int32_t shift = block_shift(block_size);
-    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_metadata: block_size must be 16, 32, 64 or 128, got %d", block_size);
-    FDMS_REQUIRE(num_seqs >= 0 && max_blocks >= 0 && total_tokens >= 0 && free_capacity >= 0 && bt_stride >= max_blocks, FDMS_E_ARG,
+    const int32_t shift = block_shift(p.block_size);
+    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_metadata: block_size must be 16, 32, 64 or 128, got %lld", (long long)p.block_size);
+    FDMS_REQUIRE(p.num_seqs >= 0 && p.max_blocks >= 0 && p.total_tokens >= 0 && p.free_capacity >= 0 && p.bt_stride >= p.max_blocks, FDMS_E_ARG,
                  "fdms_paged_metadata: negative size, or rows of the block table overlap");
-    FDMS_REQUIRE(total_tokens == 0 || (slot_mapping && positions), FDMS_E_ARG, "fdms_paged_metadata: null pointer");
-    FDMS_REQUIRE(((uintptr_t)slot_mapping & 15) == 0 && ((uintptr_t)positions & 15) == 0, FDMS_E_ARG,
+    FDMS_REQUIRE((((uintptr_t)p.slot_mapping | (uintptr_t)p.positions) & 15) == 0, FDMS_E_ARG,
                  "fdms_paged_metadata: slot_mapping and positions must be 16-byte aligned");
-    FDMS_REQUIRE(total_tokens < (1ll << 31) - 1 && free_capacity <= (0x7fffffffll >> shift) && max_blocks <= (0x7fffffff >> shift), FDMS_E_CAPACITY,
-                 "fdms_paged_metadata: token and slot numbers must fit in 31 bits");
-    const MetaArgs a = {new_lens, kv_lens, kv_lens_out, block_tables, bt_stride, free_blocks, free_capacity, free_count, free_count_out,
-                        cu_seqlens, slot_mapping, positions, dev_status, total_tokens, num_seqs, max_blocks, shift};
-    // One CTA does all of a decode step in one launch.  Beyond kFusedTokens its writes are what takes time, and a second
-    // launch spreads them over the GPU.
-    constexpr int64_t kFusedTokens = 4 * kScanThreads * kFillTokens;
+    FDMS_REQUIRE(p.total_tokens < 0x7fffffff && p.num_seqs < 0x7fffffff && p.free_capacity <= (0x7fffffff >> shift) && p.max_blocks <= (0x7fffffff >> shift),
+                 FDMS_E_CAPACITY, "fdms_paged_metadata: token and slot numbers must fit in 31 bits");
+    const MetaArgs a = {p.new_lens, p.kv_lens, p.kv_lens_out, p.block_tables, p.bt_stride, p.free_blocks, p.free_capacity, p.free_count,
+                        p.free_count_out, p.cu_seqlens, p.slot_mapping, p.positions, p.dev_status, p.total_tokens, (int32_t)p.num_seqs,
+                        (int32_t)p.max_blocks, shift};
     cudaStream_t st = (cudaStream_t)stream;
-    if (num_seqs <= kFusedRequests && total_tokens <= kFusedTokens) {
+    if (metadata_fused(p.num_seqs, p.total_tokens)) {
         paged_scan_kernel<true><<<1, kScanThreads, 0, st>>>(a, nullptr);
         FDMS_CHECK_LAUNCH("paged_scan_kernel");
         return FDMS_OK;
     }
-    FDMS_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= fdms_paged_metadata_workspace_bytes(num_seqs),
-                 FDMS_E_WORKSPACE, "fdms_paged_metadata: workspace missing, unaligned or smaller than %lld bytes",
-                 (long long)fdms_paged_metadata_workspace_bytes(num_seqs));
-    paged_scan_kernel<false><<<1, kScanThreads, 0, st>>>(a, (Served*)workspace);
+    const int64_t need = fdms_paged_metadata_workspace_bytes(p.num_seqs, p.total_tokens);
+    FDMS_REQUIRE((p.workspace || need == 0) && ((uintptr_t)p.workspace & 7) == 0 && p.workspace_bytes >= need, FDMS_E_WORKSPACE,
+                 "fdms_paged_metadata: workspace missing, unaligned or smaller than %lld bytes", (long long)need);
+    paged_scan_kernel<false><<<1, kScanThreads, 0, st>>>(a, (Served*)p.workspace);
     FDMS_CHECK_LAUNCH("paged_scan_kernel");
-    if (total_tokens == 0) return FDMS_OK;
+    if (p.total_tokens == 0) return FDMS_OK;
     const int64_t per = kFillThreads * kFillTokens;
-    FDMS_CUDA_OK(launch_chained(paged_fill_kernel, dim3((unsigned)((total_tokens + per - 1) / per)), dim3(kFillThreads), st, true, a,
-                                (const Served*)workspace));
+    FDMS_CUDA_OK(launch_chained(paged_fill_kernel, dim3((unsigned)((p.total_tokens + per - 1) / per)), dim3(kFillThreads), st, true, a,
+                                (const Served*)p.workspace));
     FDMS_CHECK_LAUNCH("paged_fill_kernel");
     return FDMS_OK;
 }
@@ -513,40 +515,34 @@ extern "C" int32_t fdms_paged_release(
     return FDMS_OK;
 }
 
-extern "C" int32_t fdms_paged_store(
-    const void* k, const void* v, int32_t act_dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
-    uint8_t* k_cache, uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
-    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, float* k_scale, float* v_scale,
-    const int32_t* slot_mapping, int64_t tokens, int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
-    int32_t* dev_status, void* stream) {
+extern "C" int32_t fdms_paged_store(const fdms_paged_store_args* args, void* stream) {
     clear_error();
-    FDMS_REQUIRE(act_dtype == FDMS_BF16 || act_dtype == FDMS_F16, FDMS_E_DTYPE, "fdms_paged_store: bf16 or f16 activations only");
-    const int32_t shift = block_shift(block_size);
-    FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_store: block_size must be 16, 32, 64 or 128, got %d", block_size);
-    FDMS_REQUIRE(head_dim == 64 || head_dim == 128, FDMS_E_ARG, "fdms_paged_store: head_dim must be 64 or 128, got %d", head_dim);
-    FDMS_REQUIRE(tokens >= 0 && num_blocks >= 0 && num_kv_heads > 0, FDMS_E_ARG, "fdms_paged_store: negative size");
-    if (tokens == 0) return FDMS_OK;
-    FDMS_REQUIRE(k && v && k_cache && v_cache && k_scale && v_scale && slot_mapping, FDMS_E_ARG, "fdms_paged_store: null pointer");
-    FDMS_REQUIRE(num_blocks <= (0x7fffffffll >> shift) && num_kv_heads <= 4096, FDMS_E_CAPACITY,
-                 "fdms_paged_store: slot numbers must fit in 31 bits, and at most 4096 KV heads");
-    const uintptr_t act = (uintptr_t)k | (uintptr_t)v | (uintptr_t)(2 * (k_stride_t | k_stride_h | v_stride_t | v_stride_h));
-    const uintptr_t cached = (uintptr_t)k_cache | (uintptr_t)v_cache |
-                             (uintptr_t)(k_stride_b | k_stride_hd | k_stride_r | v_stride_b | v_stride_hd | v_stride_r);
-    FDMS_REQUIRE((act & 15) == 0 && (cached & 15) == 0, FDMS_E_ARG, "fdms_paged_store: pointers and strides must be 16-byte aligned");
-    const int W = block_size / 16, per_cta = kStoreWarps / W;
+    FDMS_REQUIRE(args, FDMS_E_ARG, "fdms_paged_store: null pointer");
+    const fdms_paged_store_args& p = *args;
+    const fdms_paged_cache& c = p.cache;
+    int32_t shift = 0;
+    const int32_t rc = paged_cache_check("fdms_paged_store", c, p.act_dtype, p.tokens == 0, shift);
+    if (rc != FDMS_OK) return rc;
+    FDMS_REQUIRE(p.tokens >= 0, FDMS_E_ARG, "fdms_paged_store: negative size");
+    if (p.tokens == 0 || c.num_blocks == 0) return FDMS_OK;
+    FDMS_REQUIRE(p.k && p.v && p.slot_mapping, FDMS_E_ARG, "fdms_paged_store: null pointer");
+    const uintptr_t act = (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)(2 * (p.k_stride[0] | p.k_stride[1] | p.v_stride[0] | p.v_stride[1]));
+    FDMS_REQUIRE((act & 15) == 0 && p.k_stride[2] == 1 && p.v_stride[2] == 1, FDMS_E_ARG,
+                 "fdms_paged_store: key and value must be contiguous in their last dimension and aligned to 16 bytes in the others");
+    const int W = (int)c.block_size / 16, per_cta = kStoreWarps / W;
     // Tokens per CTA: few runs begin in a prompt's tokens, one at every token of a decode batch.  1024 CTAs keep the GPU
     // busy either way; more than a block's worth of tokens per CTA would only make them unequal.
     int group = 1;
-    while (group < 16 && tokens > (int64_t)group * 1024) group *= 2;
-    StoreArgs a = {{(const uint16_t*)k, (const uint16_t*)v}, {k_stride_t, v_stride_t}, {k_stride_h, v_stride_h}, {k_cache, v_cache},
-                   {k_stride_b, v_stride_b}, {k_stride_hd, v_stride_hd}, {k_stride_r, v_stride_r}, {k_scale, v_scale}, slot_mapping,
-                   dev_status, tokens, num_blocks << shift, num_kv_heads, shift, group};
-    const int64_t ctas = (tokens + group - 1) / group;
+    while (group < 16 && p.tokens > (int64_t)group * 1024) group *= 2;
+    StoreArgs a = {{(const uint16_t*)p.k, (const uint16_t*)p.v}, {p.k_stride[0], p.v_stride[0]}, {p.k_stride[1], p.v_stride[1]}, {c.k, c.v},
+                   {c.k_stride[0], c.v_stride[0]}, {c.k_stride[1], c.v_stride[1]}, {c.k_stride[2], c.v_stride[2]}, {c.k_scale, c.v_scale},
+                   p.slot_mapping, p.dev_status, p.tokens, c.num_blocks << shift, (int32_t)c.kv_heads, shift, group};
+    const int64_t ctas = (p.tokens + group - 1) / group;
     FDMS_REQUIRE(ctas < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_store: too many tokens");
-    const dim3 grid((unsigned)ctas, (unsigned)((2 * num_kv_heads + per_cta - 1) / per_cta));
+    const dim3 grid((unsigned)ctas, (unsigned)((2 * c.kv_heads + per_cta - 1) / per_cta));
     cudaStream_t st = (cudaStream_t)stream;
-    const bool bf = act_dtype == FDMS_BF16;
-    if (head_dim == 64) {
+    const bool bf = p.act_dtype == FDMS_BF16;
+    if (c.head_dim == 64) {
         if (bf) paged_store_kernel<64, true><<<grid, kStoreWarps * 32, 0, st>>>(a);
         else paged_store_kernel<64, false><<<grid, kStoreWarps * 32, 0, st>>>(a);
     } else {

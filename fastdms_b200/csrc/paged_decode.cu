@@ -360,50 +360,43 @@ extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int32_t batch, int32_t
     return decode_parts_bytes(sms, head_dim) + (int64_t)batch * num_kv_heads * ((group + kDecHeads - 1) / kDecHeads) * (int64_t)sizeof(int2);
 }
 
-extern "C" int32_t fdms_paged_attn_decode(
-    const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
-    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
-    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
-    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
-    void* out, int64_t out_stride_b, int64_t out_stride_h, float* lse_out, int64_t lse_stride_b, int64_t lse_stride_h,
-    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
-    void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream) {
+extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream) {
     clear_error();
-    PagedCache c;
-    const int32_t rc = paged_check("fdms_paged_attn_decode", c, q_dtype, k_cache, v_cache, k_stride_b, k_stride_hd, k_stride_r, v_stride_b,
-                                   v_stride_hd, v_stride_r, k_scale, v_scale, num_blocks, block_size, block_tables, bt_stride, max_blocks, kv_lens,
-                                   batch, num_q_heads, num_kv_heads, head_dim, dev_status);
+    DecodeArgs a;
+    const bool idle = args && args->num_seqs == 0;
+    const int32_t rc = paged_attn_check("fdms_paged_attn_decode", args, a.c, idle);
     if (rc != FDMS_OK) return rc;
-    if (batch == 0) return FDMS_OK;
-    FDMS_REQUIRE(q && out && workspace, FDMS_E_ARG, "fdms_paged_attn_decode: null pointer");
-    FDMS_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)(2 * (q_stride_b | q_stride_h | out_stride_b | out_stride_h))) & 15) == 0, FDMS_E_ARG,
-                 "fdms_paged_attn_decode: q and out pointers and strides must be 16-byte aligned");
-    FDMS_REQUIRE(batch <= kDecMaxBatch, FDMS_E_CAPACITY, "fdms_paged_attn_decode: at most %d sequences a call, got %d", kDecMaxBatch, batch);
+    const fdms_paged_attn_args& p = *args;
+    const int num_q_heads = (int)p.num_q_heads, num_kv_heads = a.c.heads, head_dim = (int)p.cache.head_dim;
+    FDMS_REQUIRE(p.tokens == p.num_seqs, FDMS_E_ARG, "fdms_paged_attn_decode: one token per sequence, got %lld for %lld", (long long)p.tokens,
+                 (long long)p.num_seqs);
+    FDMS_REQUIRE(p.num_seqs <= kDecMaxBatch, FDMS_E_CAPACITY, "fdms_paged_attn_decode: at most %d sequences a call, got %lld", kDecMaxBatch,
+                 (long long)p.num_seqs);
+    if (idle) return FDMS_OK;
+    const int batch = (int)p.num_seqs;
     const int sms = paged_sms();
     FDMS_REQUIRE(sms > 0, FDMS_E_CUDA, "fdms_paged_attn_decode: cannot read the device's SM count");
     const int64_t need = fdms_paged_attn_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim);
-    FDMS_REQUIRE(((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, FDMS_E_WORKSPACE,
-                 "fdms_paged_attn_decode: workspace unaligned or smaller than %lld bytes", (long long)need);
-    DecodeArgs a;
-    a.c = c;
-    a.q = (const uint16_t*)q;
-    a.out = (uint16_t*)out;
-    a.lse = lse_out;
-    a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.o_sb = out_stride_b; a.o_sh = out_stride_h; a.lse_sb = lse_stride_b; a.lse_sh = lse_stride_h;
-    a.parts = (float*)workspace;
-    a.cuts = (int2*)((char*)workspace + decode_parts_bytes(sms, head_dim));
+    FDMS_REQUIRE(p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need, FDMS_E_WORKSPACE,
+                 "fdms_paged_attn_decode: workspace missing, unaligned or smaller than %lld bytes", (long long)need);
+    a.q = (const uint16_t*)p.q;
+    a.out = (uint16_t*)p.out;
+    a.lse = p.lse_out;
+    a.q_sb = p.q_stride[0]; a.q_sh = p.q_stride[1]; a.o_sb = p.out_stride[0]; a.o_sh = p.out_stride[1];
+    a.lse_sb = p.lse_stride[0]; a.lse_sh = p.lse_stride[1];
+    a.parts = (float*)p.workspace;
+    a.cuts = (int2*)((char*)p.workspace + decode_parts_bytes(sms, head_dim));
     a.batch = batch;
     a.group = num_q_heads / num_kv_heads;
     a.splits = (a.group + kDecHeads - 1) / kDecHeads;
-    a.scale = scale;
-    const int64_t pages = (int64_t)batch * max_blocks * (block_size / kCachePage) * num_kv_heads * a.splits;
-    FDMS_REQUIRE((int64_t)batch * max_blocks * (block_size / kCachePage) < (1ll << 31), FDMS_E_CAPACITY,
-                 "fdms_paged_attn_decode: the block tables hold too many rows");
-    const int64_t useful = (pages + 2 * kDecWarps - 1) / (2 * kDecWarps);
+    a.scale = (float)p.scale;
+    const int64_t rows_held = (int64_t)batch * p.max_blocks * (p.cache.block_size / kCachePage);
+    FDMS_REQUIRE(rows_held < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_decode: the block tables hold too many rows");
+    const int64_t useful = (rows_held * num_kv_heads * a.splits + 2 * kDecWarps - 1) / (2 * kDecWarps);
     const unsigned grid = (unsigned)(useful < 1 ? 1 : useful < (int64_t)sms * kDecCtasPerSm ? useful : (int64_t)sms * kDecCtasPerSm);
     const size_t smem = (size_t)(batch + 1) * sizeof(int32_t);
     cudaStream_t st = (cudaStream_t)stream;
-    const bool bf = q_dtype == FDMS_BF16;
+    const bool bf = p.dtype == FDMS_BF16;
     const int64_t rows = (int64_t)batch * num_q_heads;
     const dim3 jgrid((unsigned)((rows + 7) / 8));
 #define FDMS_DECODE(DIM, BF)                                                                                        \

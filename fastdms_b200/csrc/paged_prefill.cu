@@ -237,35 +237,24 @@ __global__ void __launch_bounds__(kPreWarps * 32) paged_prefill_kernel(PrefillAr
 
 using namespace fdms;
 
-extern "C" int32_t fdms_paged_attn_prefill(
-    const void* q, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h,
-    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
-    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
-    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
-    const int32_t* cu_seqlens_q, int64_t tokens, void* out, int64_t out_stride_t, int64_t out_stride_h,
-    float* lse_out, int64_t lse_stride_h, int64_t lse_stride_t,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale, int32_t* dev_status, void* stream) {
+extern "C" int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, void* stream) {
     clear_error();
     PagedCache c;
-    const int32_t rc = paged_check("fdms_paged_attn_prefill", c, q_dtype, k_cache, v_cache, k_stride_b, k_stride_hd, k_stride_r, v_stride_b,
-                                   v_stride_hd, v_stride_r, k_scale, v_scale, num_blocks, block_size, block_tables, bt_stride, max_blocks, kv_lens,
-                                   num_seqs, num_q_heads, num_kv_heads, head_dim, dev_status);
+    const bool idle = args && (args->num_seqs == 0 || args->tokens == 0);
+    const int32_t rc = paged_attn_check("fdms_paged_attn_prefill", args, c, idle);
     if (rc != FDMS_OK) return rc;
-    FDMS_REQUIRE(tokens >= 0, FDMS_E_ARG, "fdms_paged_attn_prefill: negative size");
-    if (num_seqs == 0 || tokens == 0) return FDMS_OK;
-    FDMS_REQUIRE(q && out && cu_seqlens_q, FDMS_E_ARG, "fdms_paged_attn_prefill: null pointer");
-    FDMS_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)(2 * (q_stride_t | q_stride_h | out_stride_t | out_stride_h))) & 15) == 0, FDMS_E_ARG,
-                 "fdms_paged_attn_prefill: q and out pointers and strides must be 16-byte aligned");
-    FDMS_REQUIRE(num_kv_heads <= 65535, FDMS_E_CAPACITY, "fdms_paged_attn_prefill: at most 65535 KV heads");
-    const int group = num_q_heads / num_kv_heads;
-    PrefillArgs a = {c, (const uint16_t*)q, (uint16_t*)out, lse_out, cu_seqlens_q, q_stride_t, q_stride_h, out_stride_t, out_stride_h,
-                     lse_stride_h, lse_stride_t, tokens, num_seqs, group, scale};
-    const int64_t tiles = tokens / (kPreRows / group) + num_seqs;
-    FDMS_REQUIRE(tokens < (1ll << 31) && tiles < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_prefill: too many tokens");
-    const dim3 grid((unsigned)tiles, (unsigned)num_kv_heads);
+    if (idle) return FDMS_OK;
+    const fdms_paged_attn_args& p = *args;
+    FDMS_REQUIRE(p.cu_seqlens_q, FDMS_E_ARG, "fdms_paged_attn_prefill: null pointer");
+    const int group = (int)p.num_q_heads / c.heads;
+    PrefillArgs a = {c, (const uint16_t*)p.q, (uint16_t*)p.out, p.lse_out, p.cu_seqlens_q, p.q_stride[0], p.q_stride[1], p.out_stride[0],
+                     p.out_stride[1], p.lse_stride[0], p.lse_stride[1], p.tokens, (int32_t)p.num_seqs, group, (float)p.scale};
+    const int64_t tiles = p.tokens / (kPreRows / group) + p.num_seqs;
+    FDMS_REQUIRE(tiles < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_prefill: too many tokens");
+    const dim3 grid((unsigned)tiles, (unsigned)c.heads);
     cudaStream_t st = (cudaStream_t)stream;
-    const bool bf = q_dtype == FDMS_BF16;
-    if (head_dim == 64) {
+    const bool bf = p.dtype == FDMS_BF16;
+    if (p.cache.head_dim == 64) {
         if (bf) paged_prefill_kernel<64, true><<<grid, kPreWarps * 32, 0, st>>>(a);
         else paged_prefill_kernel<64, false><<<grid, kPreWarps * 32, 0, st>>>(a);
     } else {

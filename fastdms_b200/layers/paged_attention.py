@@ -21,6 +21,8 @@ path: tensors must live on a CUDA device.
 """
 from __future__ import annotations
 
+from struct import Struct
+
 import torch
 
 from fastdms_b200 import _lib
@@ -30,24 +32,55 @@ HEAD_DIMS = (64, 128)
 MAX_DECODE_BATCH = 2048
 MAX_RELEASE_ROWS = 4096
 
+# The argument blocks of include/fastdms_b200.h; every member is 8 bytes wide.
+_METADATA_ARGS = Struct("12P7q")
+_STORE_ARGS = Struct("4P12q4P8q")
+_ATTN_ARGS = Struct("4P12q8P15qd")
+_ROW_DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_F8, _I32, _I64, _F32 = torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32
 
-def _same_device(dev: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"expected {name} on {dev}, got {t.device}")
+
+def _device(named: dict) -> int:
+    """The CUDA device that all tensors live on."""
+    given = {name: t for name, t in named.items() if t is not None}
+    _lib.require_cuda(*given.values())
+    first = next(iter(given.values())).device
+    for name, t in given.items():
+        if t.device != first:
+            raise ValueError(f"expected {name} on {first}, got {t.device}")
+    return first.index
+
+
+def _on_device(dev: int, fn, *args):
+    """Calls a C function with device `dev` current."""
+    if torch._C._cuda_getDevice() == dev:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
+def _launch(fn, args: bytes, dev: int) -> None:
+    """Calls a C entry on the current stream of device `dev`."""
+    rc = _on_device(dev, fn, args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc)
 
 
 def _int_vector(t: torch.Tensor, name: str, size: int | None = None) -> None:
-    if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or (size is not None and t.numel() != size):
+    if t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous() or (size is not None and t.numel() != size):
         shape = "[n]" if size is None else f"[{size}]"
         raise ValueError(f"expected {name} as contiguous int32 {shape}, got {tuple(t.shape)} {t.dtype}")
 
 
-def _check_tables(block_tables: torch.Tensor, rows: int) -> None:
-    if block_tables.ndim != 2 or block_tables.shape[0] != rows or block_tables.dtype != torch.int32:
+def _tables(block_tables: torch.Tensor, rows: int) -> tuple[int, int]:
+    """Columns and row stride of a block table; one row (or none) may carry any stride."""
+    if block_tables.dtype is not _I32 or block_tables.dim() != 2 or block_tables.shape[0] != rows:
         raise ValueError(f"expected block_tables as int32 [{rows}, columns], got {tuple(block_tables.shape)} {block_tables.dtype}")
-    if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
+    cols = block_tables.shape[1]
+    stride = block_tables.stride()
+    if cols > 1 and stride[1] != 1:
         raise ValueError("block_tables must be contiguous in its last dimension")
+    return cols, stride[0] if rows > 1 else cols
 
 
 def _check_block_size(block_size: int) -> None:
@@ -55,34 +88,25 @@ def _check_block_size(block_size: int) -> None:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Stride of a 2-d tensor's rows, which a tensor of one row (or none) may carry any value for."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _check_cache(k_cache, v_cache, k_scale, v_scale) -> None:
-    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape:
-        raise ValueError(f"expected k_cache and v_cache as [blocks, kv_heads, block_size, head_dim], got {tuple(k_cache.shape)} / {tuple(v_cache.shape)}")
-    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+def _cache_shape(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"expected k_cache and v_cache as [blocks, kv_heads, block_size, head_dim], got {tuple(shape)} / {tuple(v_cache.shape)}")
+    if k_cache.dtype is not _F8 or v_cache.dtype is not _F8:
         raise ValueError(f"expected float8_e4m3fn caches, got {k_cache.dtype} / {v_cache.dtype}")
-    blocks, heads, block_size, head_dim = k_cache.shape
-    _check_block_size(block_size)
-    if head_dim not in HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.stride(3) != 1 or any(c.stride(i) % 16 for i in range(3)) or c.data_ptr() % 16:
-            raise ValueError(f"{name} must be contiguous in its last dimension and aligned to 16 bytes in the others")
-    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if s.shape != (blocks, heads) or s.dtype != torch.float32 or not s.is_contiguous():
-            raise ValueError(f"expected {name} as contiguous float32 {(blocks, heads)}, got {tuple(s.shape)} {s.dtype}")
+    scales = shape[:2]
+    if (k_scale.shape != scales or v_scale.shape != scales or k_scale.dtype is not _F32 or v_scale.dtype is not _F32
+            or not k_scale.is_contiguous() or not v_scale.is_contiguous()):
+        raise ValueError(f"expected k_scale and v_scale as contiguous float32 {tuple(scales)}, got {tuple(k_scale.shape)} {k_scale.dtype} / "
+                         f"{tuple(v_scale.shape)} {v_scale.dtype}")
+    return shape
 
 
-def _check_rows(t: torch.Tensor, name: str) -> None:
-    """16-bit rows that the kernels read and write 16 bytes at a time."""
-    if t.dtype not in (torch.bfloat16, torch.float16):
+def _row_dtype(t: torch.Tensor, name: str) -> int:
+    code = _ROW_DTYPES.get(t.dtype)
+    if code is None:
         raise ValueError(f"{name} must be bfloat16 or float16, got {t.dtype}")
-    if t.numel() and (t.stride(2) != 1 or t.stride(0) * 2 % 16 or t.stride(1) * 2 % 16 or t.data_ptr() % 16):
-        raise ValueError(f"{name} must be contiguous in its last dimension and aligned to 16 bytes in the others")
+    return code
 
 
 def build_paged_metadata(
@@ -119,38 +143,41 @@ def build_paged_metadata(
     _int_vector(new_lens, "new_lens", n)
     _int_vector(free_blocks, "free_blocks")
     _int_vector(free_count, "free_count", 1)
-    _check_tables(block_tables, n)
+    cols, stride = _tables(block_tables, n)
     _check_block_size(block_size)
     total_tokens = int(total_tokens)
     if total_tokens < 0:
         raise ValueError(f"total_tokens must not be negative, got {total_tokens}")
-    _lib.require_cuda(new_lens, kv_lens, block_tables, free_blocks, free_count)
-    dev = kv_lens.device
+    dev = kv_lens.get_device()
+    if (dev < 0 or new_lens.get_device() != dev or block_tables.get_device() != dev or free_blocks.get_device() != dev
+            or free_count.get_device() != dev):
+        _device(dict(kv_lens=kv_lens, new_lens=new_lens, block_tables=block_tables, free_blocks=free_blocks, free_count=free_count))
+    for t, name, size in ((kv_lens_out, "kv_lens_out", n), (free_count_out, "free_count_out", 1), (cu_seqlens, "cu_seqlens", n + 1),
+                          (slot_mapping, "slot_mapping", total_tokens)):
+        if t is not None:
+            _int_vector(t, name, size)
+            if t.get_device() != dev:
+                _device({"kv_lens": kv_lens, name: t})
+    if positions is not None:
+        if positions.dtype is not _I64 or positions.shape != (total_tokens,) or not positions.is_contiguous():
+            raise ValueError(f"expected positions as contiguous int64 [{total_tokens}], got {tuple(positions.shape)} {positions.dtype}")
+        if positions.get_device() != dev:
+            _device(dict(kv_lens=kv_lens, positions=positions))
+    device = kv_lens.device
     kv_lens_out = kv_lens if kv_lens_out is None else kv_lens_out
     free_count_out = free_count if free_count_out is None else free_count_out
-    _int_vector(kv_lens_out, "kv_lens_out", n)
-    _int_vector(free_count_out, "free_count_out", 1)
     if cu_seqlens is None:
-        cu_seqlens = torch.empty(n + 1, dtype=torch.int32, device=dev)
-    _int_vector(cu_seqlens, "cu_seqlens", n + 1)
+        cu_seqlens = torch.empty(n + 1, dtype=_I32, device=device)
     if slot_mapping is None:
-        slot_mapping = torch.empty(total_tokens, dtype=torch.int32, device=dev)
-    _int_vector(slot_mapping, "slot_mapping", total_tokens)
+        slot_mapping = torch.empty(total_tokens, dtype=_I32, device=device)
     if positions is None:
-        positions = torch.empty(total_tokens, dtype=torch.int64, device=dev)
-    if positions.dtype != torch.int64 or positions.shape != (total_tokens,) or not positions.is_contiguous():
-        raise ValueError(f"expected positions as contiguous int64 [{total_tokens}], got {tuple(positions.shape)} {positions.dtype}")
-    _same_device(dev, new_lens=new_lens, block_tables=block_tables, free_blocks=free_blocks, free_count=free_count, kv_lens_out=kv_lens_out,
-                 free_count_out=free_count_out, cu_seqlens=cu_seqlens, slot_mapping=slot_mapping, positions=positions)
-    status = _lib.status_word(dev)
-    ws = torch.empty(_lib.lib().fdms_paged_metadata_workspace_bytes(n), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().fdms_paged_metadata(
-            new_lens.data_ptr(), kv_lens.data_ptr(), kv_lens_out.data_ptr(), block_tables.data_ptr(), _row_stride(block_tables),
-            block_tables.shape[1], block_size, free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(), free_count_out.data_ptr(),
-            cu_seqlens.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), total_tokens, n, ws.data_ptr(), ws.numel(),
-            status.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc)
+        positions = torch.empty(total_tokens, dtype=_I64, device=device)
+    need = _lib.lib().fdms_paged_metadata_workspace_bytes(n, total_tokens)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _launch(_lib.lib().fdms_paged_metadata, _METADATA_ARGS.pack(
+        new_lens.data_ptr(), kv_lens.data_ptr(), kv_lens_out.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(),
+        free_count_out.data_ptr(), cu_seqlens.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), ws.data_ptr() if need else 0,
+        _lib.status_word(device).data_ptr(), n, cols, stride, block_size, free_blocks.numel(), total_tokens, need), dev)
     return cu_seqlens, slot_mapping, positions
 
 
@@ -170,19 +197,17 @@ def release_paged_blocks(
     _int_vector(kv_lens, "kv_lens")
     _int_vector(free_blocks, "free_blocks")
     _int_vector(free_count, "free_count", 1)
-    _check_tables(block_tables, n)
+    cols, stride = _tables(block_tables, n)
     _check_block_size(block_size)
     if rows is not None:
         _int_vector(rows, "rows")
-    _lib.require_cuda(kv_lens, block_tables, free_blocks, free_count, rows)
-    dev = kv_lens.device
-    _same_device(dev, block_tables=block_tables, free_blocks=free_blocks, free_count=free_count, rows=rows)
-    status = _lib.status_word(dev)
+    dev = _device(dict(kv_lens=kv_lens, block_tables=block_tables, free_blocks=free_blocks, free_count=free_count, rows=rows))
+    status = _lib.status_word(kv_lens.device)
     with torch.cuda.device(dev):
         rc = _lib.lib().fdms_paged_release(
             _lib.ptr(rows) if rows is not None and rows.numel() else None, n if rows is None else rows.numel(), kv_lens.data_ptr(), n,
-            block_tables.data_ptr(), _row_stride(block_tables), block_tables.shape[1], block_size, free_blocks.data_ptr(),
-            free_blocks.numel(), free_count.data_ptr(), status.data_ptr(), _lib.stream_ptr(dev))
+            block_tables.data_ptr(), stride, cols, block_size, free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(),
+            status.data_ptr(), _lib.stream_ptr(kv_lens.device))
     _lib.check(rc)
 
 
@@ -207,52 +232,68 @@ def store_paged_kvcache(
     A sequence's tokens are consecutive, as `build_paged_metadata` lays them out, and no block is written by two sequences.
     A slot beyond the cache, or next to a token of its own block that it does not follow, is skipped and raises the device
     status bit for bad indices."""
-    if key.ndim != 3 or key.shape != value.shape:
-        raise ValueError(f"expected key and value as [tokens, kv_heads, head_dim], got {tuple(key.shape)} / {tuple(value.shape)}")
-    if key.dtype != value.dtype:
+    blocks, heads, block_size, head_dim = _cache_shape(k_cache, v_cache, k_scale, v_scale)
+    shape = key.shape
+    if len(shape) != 3 or value.shape != shape:
+        raise ValueError(f"expected key and value as [tokens, kv_heads, head_dim], got {tuple(shape)} / {tuple(value.shape)}")
+    if shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"expected key as [tokens, {heads}, {head_dim}], got {tuple(shape)}")
+    if key.dtype is not value.dtype:
         raise ValueError("key and value must share a dtype")
-    _check_cache(k_cache, v_cache, k_scale, v_scale)
-    blocks, heads, block_size, head_dim = k_cache.shape
-    tokens = key.shape[0]
-    if key.shape[1:] != (heads, head_dim):
-        raise ValueError(f"expected key as [tokens, {heads}, {head_dim}], got {tuple(key.shape)}")
-    _check_rows(key, "key")
-    _check_rows(value, "value")
-    _int_vector(slot_mapping, "slot_mapping", tokens)
-    _lib.require_cuda(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
-    dev = k_cache.device
-    _same_device(dev, key=key, value=value, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, slot_mapping=slot_mapping)
-    status = _lib.status_word(dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().fdms_paged_store(
-            key.data_ptr(), value.data_ptr(), _lib.dtype_code(key.dtype), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-            k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-            v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(),
-            tokens, blocks, block_size, heads, head_dim, status.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc)
+    dtype = _row_dtype(key, "key")
+    _int_vector(slot_mapping, "slot_mapping", shape[0])
+    dev = k_cache.get_device()
+    if (dev < 0 or key.get_device() != dev or value.get_device() != dev or v_cache.get_device() != dev or k_scale.get_device() != dev
+            or v_scale.get_device() != dev or slot_mapping.get_device() != dev):
+        _device(dict(k_cache=k_cache, key=key, value=value, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, slot_mapping=slot_mapping))
+    _launch(_lib.lib().fdms_paged_store, _STORE_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, block_size, head_dim,
+        *k_cache.stride(), *v_cache.stride(), key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr(),
+        _lib.status_word(k_cache.device).data_ptr(), shape[0], dtype, *key.stride(), *value.stride()), dev)
 
 
-def _check_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, out, lse_out, lse_shape) -> torch.device:
-    if q.ndim != 3:
-        raise ValueError(f"expected q as [tokens, q_heads, head_dim], got {tuple(q.shape)}")
-    _check_cache(k_cache, v_cache, k_scale, v_scale)
-    heads, head_dim = k_cache.shape[1], k_cache.shape[3]
-    if q.shape[2] != head_dim:
-        raise ValueError(f"cache head_dim {head_dim} does not match q head_dim {q.shape[2]}")
-    if q.shape[1] == 0 or heads == 0 or q.shape[1] % heads != 0 or q.shape[1] // heads > 64:
-        raise ValueError(f"q_heads={q.shape[1]} must be kv_heads={heads} times 1 to 64")
-    _check_rows(q, "q")
+def _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, lse_shape):
+    """Both attentions: with `cu_seqlens_q` the prefill, without it one token per sequence."""
+    blocks, heads, block_size, head_dim = _cache_shape(k_cache, v_cache, k_scale, v_scale)
+    shape = q.shape
+    if shape[2] != head_dim:
+        raise ValueError(f"cache head_dim {head_dim} does not match q head_dim {shape[2]}")
+    tokens, num_q_heads = shape[0], shape[1]
+    if num_q_heads == 0 or heads == 0 or num_q_heads % heads != 0 or num_q_heads // heads > 64:
+        raise ValueError(f"q_heads={num_q_heads} must be kv_heads={heads} times 1 to 64")
+    dtype = _row_dtype(q, "q")
     _int_vector(kv_lens, "kv_lens")
-    _check_tables(block_tables, kv_lens.numel())
-    if out.shape != q.shape or out.dtype != q.dtype:
+    seqs = kv_lens.numel()
+    cols, stride = _tables(block_tables, seqs)
+    dev = q.get_device()
+    if (dev < 0 or k_cache.get_device() != dev or v_cache.get_device() != dev or k_scale.get_device() != dev or v_scale.get_device() != dev
+            or block_tables.get_device() != dev or kv_lens.get_device() != dev or (cu_seqlens_q is not None and cu_seqlens_q.get_device() != dev)):
+        _device(dict(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_tables=block_tables, kv_lens=kv_lens,
+                     cu_seqlens_q=cu_seqlens_q))
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not q.dtype:
         raise ValueError("out must have q's shape and dtype")
-    _check_rows(out, "out")
-    if lse_out is not None and (lse_out.shape != lse_shape or lse_out.dtype != torch.float32):
-        raise ValueError(f"expected float32 lse_out {tuple(lse_shape)}, got {tuple(lse_out.shape)} {lse_out.dtype}")
-    _lib.require_cuda(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, out, lse_out)
-    _same_device(q.device, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_tables=block_tables, kv_lens=kv_lens,
-                 out=out, lse_out=lse_out)
-    return q.device
+    elif out.get_device() != dev:
+        _device(dict(q=q, out=out))
+    lse_ptr, lse_stride = 0, (0, 0)
+    if lse_out is not None:
+        if lse_out.shape != lse_shape or lse_out.dtype is not _F32:
+            raise ValueError(f"expected float32 lse_out {tuple(lse_shape)}, got {tuple(lse_out.shape)} {lse_out.dtype}")
+        if lse_out.get_device() != dev:
+            _device(dict(q=q, lse_out=lse_out))
+        lse_ptr, lse_stride = lse_out.data_ptr(), lse_out.stride()
+    lib, need, ws = _lib.lib(), 0, None
+    if cu_seqlens_q is None:
+        need = _on_device(dev, lib.fdms_paged_attn_decode_workspace_bytes, tokens, num_q_heads, heads, head_dim)
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=q.device)
+    _launch(lib.fdms_paged_attn_decode if cu_seqlens_q is None else lib.fdms_paged_attn_prefill, _ATTN_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, block_size, head_dim,
+        *k_cache.stride(), *v_cache.stride(), q.data_ptr(), out.data_ptr(), lse_ptr, block_tables.data_ptr(), kv_lens.data_ptr(),
+        0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if ws is None else ws.data_ptr(), _lib.status_word(q.device).data_ptr(),
+        tokens, seqs, num_q_heads, dtype, cols, stride, need, *q.stride(), *out.stride(), *lse_stride,
+        head_dim ** -0.5 if scale is None else scale), dev)
+    return out
 
 
 def paged_decode_attention(
@@ -273,31 +314,15 @@ def paged_decode_attention(
     queries, head_dim 64 or 128, at most 2048 sequences.  `scale` defaults to head_dim ** -0.5.  A sequence without rows gets
     zeros.  `lse_out` (float32 `[batch, q_heads]`) receives the natural-log log-sum-exp of the scaled scores.  Table
     entries that are needed and name no block of the cache are left out and raise the device status bit for bad indices."""
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dev = _check_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, out, lse_out, q.shape[:2])
-    batch, num_q_heads, head_dim = q.shape
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"expected q as [batch, q_heads, head_dim], got {tuple(shape)}")
+    batch = shape[0]
     if kv_lens.numel() != batch:
-        raise ValueError(f"expected kv_lens [{batch}], got {tuple(kv_lens.shape)}")
+        raise ValueError(f"expected kv_lens as contiguous int32 [{batch}], got {tuple(kv_lens.shape)} {kv_lens.dtype}")
     if batch > MAX_DECODE_BATCH:
         raise RuntimeError(f"at most {MAX_DECODE_BATCH} sequences a call, got {batch}")
-    if batch == 0:
-        return out
-    blocks, heads, block_size, _ = k_cache.shape
-    status = _lib.status_word(dev)
-    with torch.cuda.device(dev):
-        need = _lib.lib().fdms_paged_attn_decode_workspace_bytes(batch, num_q_heads, heads, head_dim)
-        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=dev)
-        rc = _lib.lib().fdms_paged_attn_decode(
-            q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-            k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size, block_tables.data_ptr(), _row_stride(block_tables),
-            block_tables.shape[1], kv_lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(lse_out),
-            lse_out.stride(0) if lse_out is not None else 0, lse_out.stride(1) if lse_out is not None else 0,
-            batch, num_q_heads, heads, head_dim, float(head_dim ** -0.5 if scale is None else scale), ws.data_ptr(), ws.numel(),
-            status.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc)
-    return out
+    return _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, None, scale, out, lse_out, shape[:2])
 
 
 def paged_prefill_attention(
@@ -319,25 +344,8 @@ def paged_prefill_attention(
     rows stored before the call: with n tokens of a sequence in the step, token i sees its rows 0 .. kv_lens - n + i.  A
     token that sees none gets zeros and a log-sum-exp of -inf.  Tokens behind the last sequence are left as they were in
     `out` and `lse_out` (float32 `[q_heads, tokens]`).  Types, head sizes and table entries as in `paged_decode_attention`."""
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dev = _check_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, out, lse_out, (q.shape[1], q.shape[0]))
-    tokens, num_q_heads, head_dim = q.shape
-    seqs = kv_lens.numel()
-    _int_vector(cu_seqlens_q, "cu_seqlens_q", seqs + 1)
-    _lib.require_cuda(cu_seqlens_q)
-    _same_device(dev, cu_seqlens_q=cu_seqlens_q)
-    if tokens == 0 or seqs == 0:
-        return out
-    blocks, heads, block_size, _ = k_cache.shape
-    status = _lib.status_word(dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().fdms_paged_attn_prefill(
-            q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-            k_scale.data_ptr(), v_scale.data_ptr(), blocks, block_size, block_tables.data_ptr(), _row_stride(block_tables),
-            block_tables.shape[1], kv_lens.data_ptr(), cu_seqlens_q.data_ptr(), tokens, out.data_ptr(), out.stride(0), out.stride(1),
-            _lib.ptr(lse_out), lse_out.stride(0) if lse_out is not None else 0, lse_out.stride(1) if lse_out is not None else 0,
-            seqs, num_q_heads, heads, head_dim, float(head_dim ** -0.5 if scale is None else scale), status.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc)
-    return out
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError(f"expected q as [tokens, q_heads, head_dim], got {tuple(shape)}")
+    _int_vector(cu_seqlens_q, "cu_seqlens_q", kv_lens.numel() + 1)
+    return _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, (shape[1], shape[0]))

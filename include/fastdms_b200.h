@@ -497,13 +497,16 @@ int32_t fdms_linear_decode_allreduce(
  * r % block_size of block block_tables[s * bt_stride + r / block_size].  Slots and lengths are int32, so a pool holds
  * fewer than 2^31 rows.
  *
+ * The calls of a step take their arguments in a struct of pointers and 64-bit numbers: a caller in another language
+ * fills one block of memory instead of converting 20 to 40 arguments one by one, which costs more than the launch.
+ *
  * fdms_paged_metadata: sequence i holds kv_lens[i] rows and gets new_lens[i] more.  The blocks it needs are popped from
  *   free_blocks[0 .. free_count) (the top is the end) into its row of the table, in the order of the sequences; where the
  *   stack runs out a sequence and the later ones that need blocks are not served: slots -1, length and table as before.
  *   cu_seqlens [num_seqs + 1] = prefix sums of new_lens; slot_mapping and positions [total_tokens], 16-byte aligned
  *   (tokens behind the last: -1 and 0).  kv_lens_out / free_count_out may be kv_lens / free_count.  A negative length, one
  *   beyond max_blocks * block_size, or more tokens than total_tokens is not served and raises FDMS_DEV_BAD_INDEX.
- *   workspace: fdms_paged_metadata_workspace_bytes(num_seqs) bytes, 8-byte aligned, any contents.
+ *   workspace: fdms_paged_metadata_workspace_bytes(...) bytes, 8-byte aligned, any contents.
  * fdms_paged_release: the blocks of rows[0 .. num_listed) (NULL: rows 0 .. num_listed) return to the stack; their
  *   table entries become -1 and their lengths 0.  At most 4096 rows; a row listed twice is released once.
  * fdms_paged_store: k, v [tokens, kv_heads, head_dim] (bf16 / f16, strides in elements, 16-byte aligned) into the rows of
@@ -520,39 +523,58 @@ int32_t fdms_linear_decode_allreduce(
  * Both attentions: q_heads = kv_heads times 1 to 64, bf16 / f16; a needed table entry outside [0, num_blocks) is left out
  * and raises FDMS_DEV_BAD_INDEX, as does a length beyond the table.
  * --------------------------------------------------------------------------------------------- */
-int64_t fdms_paged_metadata_workspace_bytes(int32_t num_seqs);
-int32_t fdms_paged_metadata(
-    const int32_t* new_lens, const int32_t* kv_lens, int32_t* kv_lens_out, int32_t* block_tables, int64_t bt_stride,
-    int32_t max_blocks, int32_t block_size, const int32_t* free_blocks, int64_t free_capacity, const int32_t* free_count,
-    int32_t* free_count_out, int32_t* cu_seqlens, int32_t* slot_mapping, int64_t* positions, int64_t total_tokens,
-    int32_t num_seqs, void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream);
+typedef struct fdms_paged_cache {
+    uint8_t *k, *v;                     /* e4m3 [num_blocks, kv_heads, block_size, head_dim] */
+    float *k_scale, *v_scale;           /* [num_blocks, kv_heads], contiguous */
+    int64_t num_blocks, kv_heads, block_size, head_dim;
+    int64_t k_stride[4], v_stride[4];   /* block, head, row (multiples of 16), channel (1), in bytes */
+} fdms_paged_cache;
+
+typedef struct fdms_paged_metadata_args {
+    const int32_t *new_lens, *kv_lens;
+    int32_t *kv_lens_out, *block_tables;
+    const int32_t *free_blocks, *free_count;
+    int32_t *free_count_out, *cu_seqlens, *slot_mapping;
+    int64_t *positions;
+    void *workspace;
+    int32_t *dev_status;
+    int64_t num_seqs, max_blocks, bt_stride, block_size, free_capacity, total_tokens, workspace_bytes;
+} fdms_paged_metadata_args;
+
+typedef struct fdms_paged_store_args {
+    fdms_paged_cache cache;
+    const void *k, *v;
+    const int32_t *slot_mapping;
+    int32_t *dev_status;
+    int64_t tokens, act_dtype;
+    int64_t k_stride[3], v_stride[3];   /* token, head, channel (1), in elements */
+} fdms_paged_store_args;
+
+typedef struct fdms_paged_attn_args {
+    fdms_paged_cache cache;
+    const void *q;
+    void *out;
+    float *lse_out;                     /* or NULL */
+    const int32_t *block_tables, *kv_lens, *cu_seqlens_q;
+    void *workspace;
+    int32_t *dev_status;
+    int64_t tokens, num_seqs, num_q_heads, dtype, max_blocks, bt_stride, workspace_bytes;
+    int64_t q_stride[3], out_stride[3]; /* token, head, channel (1), in elements */
+    int64_t lse_stride[2];              /* decode: sequence, head; prefill: head, token */
+    double scale;
+} fdms_paged_attn_args;
+
+/* Bytes of workspace: 0 where the call needs none. */
+int64_t fdms_paged_metadata_workspace_bytes(int64_t num_seqs, int64_t total_tokens);
+int32_t fdms_paged_metadata(const fdms_paged_metadata_args* args, void* stream);
 int32_t fdms_paged_release(
     const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
     int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
     int32_t* dev_status, void* stream);
-int32_t fdms_paged_store(
-    const void* k, const void* v, int32_t act_dtype, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
-    uint8_t* k_cache, uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
-    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, float* k_scale, float* v_scale,
-    const int32_t* slot_mapping, int64_t tokens, int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
-    int32_t* dev_status, void* stream);
+int32_t fdms_paged_store(const fdms_paged_store_args* args, void* stream);
 int64_t fdms_paged_attn_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
-int32_t fdms_paged_attn_decode(
-    const void* q, int32_t q_dtype, int64_t q_stride_b, int64_t q_stride_h,
-    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
-    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
-    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
-    void* out, int64_t out_stride_b, int64_t out_stride_h, float* lse_out, int64_t lse_stride_b, int64_t lse_stride_h,
-    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
-    void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream);
-int32_t fdms_paged_attn_prefill(
-    const void* q, int32_t q_dtype, int64_t q_stride_t, int64_t q_stride_h,
-    const uint8_t* k_cache, const uint8_t* v_cache, int64_t k_stride_b, int64_t k_stride_hd, int64_t k_stride_r,
-    int64_t v_stride_b, int64_t v_stride_hd, int64_t v_stride_r, const float* k_scale, const float* v_scale, int64_t num_blocks,
-    int32_t block_size, const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks, const int32_t* kv_lens,
-    const int32_t* cu_seqlens_q, int64_t tokens, void* out, int64_t out_stride_t, int64_t out_stride_h,
-    float* lse_out, int64_t lse_stride_h, int64_t lse_stride_t,
-    int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale, int32_t* dev_status, void* stream);
+int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream);
+int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, void* stream);
 
 #ifdef __cplusplus
 }

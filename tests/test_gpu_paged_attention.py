@@ -549,6 +549,31 @@ def test_prefill_of_broken_offsets_stays_inside(dev):
         assert torch.isfinite(out.float()).all()
 
 
+def test_attention_refuses_outputs_and_strides(dev):
+    from fastdms_b200.layers import paged_attention as P
+    kc, vc, ks, vs = make_cache(2, 1, 16, 64, dev)
+    q, table, kv = torch.zeros((2, 4, 64), dtype=torch.bfloat16, device=dev), i32([[0], [1]], dev), i32([3, 4], dev)
+    args = (kc, vc, ks, vs, table, kv)
+    for bad, match in [(dict(out=torch.zeros((2, 4, 64), device=dev)), "out must"), (dict(out=torch.zeros_like(q).cpu()), "CUDA"),
+                       (dict(lse_out=torch.zeros((4, 3), device=dev)), "lse_out"),
+                       (dict(out=torch.zeros((2, 4, 128), dtype=torch.bfloat16, device=dev)[:, :, ::2]), "contiguous")]:
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            P.paged_decode_attention(q, *args, **bad)
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            P.paged_prefill_attention(q, *args, i32([0, 1, 2], dev), **bad)
+    odd = torch.zeros((2, 4, 66), dtype=torch.bfloat16, device=dev)[:, :, 1:65]
+    with pytest.raises(ValueError, match="aligned"):
+        P.paged_decode_attention(odd, *args)
+    with pytest.raises(ValueError, match="aligned"):
+        P.store_paged_kvcache(odd[:, :1], odd[:, :1], kc, vc, ks, vs, i32([0, 16], dev))
+    with pytest.raises(ValueError, match="cu_seqlens_q"):
+        P.paged_prefill_attention(q, *args, i32([0, 1], dev))
+    with pytest.raises(RuntimeError, match="2048"):
+        P.paged_decode_attention(q[:1].expand(2049, 4, 64).contiguous(), kc, vc, ks, vs, table[:1].expand(2049, 1).contiguous(), kv[:1].expand(2049).contiguous())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.paged_decode_attention(q, kc, vc, ks.cpu(), vs, table, kv)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 class Run:

@@ -47,16 +47,14 @@ def _bad(**change):
     (dict(q=torch.zeros((2, 130, 64), dtype=torch.float16)), "times 1 to 64"),
     (dict(q=torch.zeros((2, 0, 64), dtype=torch.float16)), "times 1 to 64"),
     (dict(q=torch.zeros((2, 4, 128), dtype=torch.float16)), "head_dim"),
-    (dict(q=torch.zeros((2, 4, 66), dtype=torch.float16)[:, :, 1:65]), "aligned"),
-    (dict(q=torch.zeros((2, 64), dtype=torch.float16)), "tokens, q_heads"),
+    (dict(q=torch.zeros((2, 64), dtype=torch.float16)), "q_heads, head_dim"),
     (dict(kv=torch.tensor([3, 4])), "int32"),
     (dict(kv=ints(3, 0, 4)[::2]), "contiguous"),
     (dict(table=torch.zeros((2, 2))), "int32"),
     (dict(table=torch.zeros((3, 2), dtype=torch.int32)), r"\[2, columns\]"),
     (dict(table=torch.zeros((2, 4), dtype=torch.int32)[:, ::2]), "last dimension"),
-    (dict(cache=cache(bs=24)), "block_size"),
-    (dict(cache=cache(d=80)), "head_dim"),
     (dict(cache=[c.view(torch.uint8) if c.element_size() == 1 else c for c in cache()]), "float8"),
+    (dict(cache=cache(d=128)), "head_dim"),
     (dict(cache=cache()[:3] + [torch.ones((4, 3))]), "v_scale"),
     (dict(cache=cache()[:2] + [torch.ones((2, 4)).t()] + cache()[3:]), "k_scale"),
     (dict(cache=[cache(heads=1)[0]] + cache()[1:]), "kv_heads, block_size"),
@@ -67,19 +65,6 @@ def test_attention_refuses(change, match):
         P.paged_decode_attention(a["q"], *a["cache"], a["table"], a["kv"])
     with pytest.raises(ValueError, match=match):
         P.paged_prefill_attention(a["q"], *a["cache"], a["table"], a["kv"], ints(0, 1, 2))
-
-
-def test_attention_refuses_outputs_and_lengths():
-    a = _bad()
-    args = (a["q"], *a["cache"], a["table"], a["kv"])
-    with pytest.raises(ValueError, match="out must"):
-        P.paged_decode_attention(*args, out=torch.zeros((2, 4, 64)))
-    with pytest.raises(ValueError, match="lse_out"):
-        P.paged_decode_attention(*args, lse_out=torch.zeros((4, 2)))
-    with pytest.raises(ValueError, match="lse_out"):
-        P.paged_prefill_attention(*args, ints(0, 1, 2), lse_out=torch.zeros((2, 4)))
-    with pytest.raises(ValueError, match="aligned"):
-        P.paged_decode_attention(*args, out=torch.zeros((2, 4, 128), dtype=torch.bfloat16)[:, :, ::2])
 
 
 def test_store_refuses():
@@ -107,46 +92,69 @@ def test_tables_refuse():
         P.release_paged_blocks(kv, table, free, count, block_size=16, rows=torch.tensor([0]))
 
 
-def test_c_entries_refuse_without_a_gpu():
+PTR = 1 << 12
+CACHE = dict(k=PTR, v=PTR, ks=PTR, vs=PTR, blocks=4, heads=2, bs=16, d=64, k0=2048, k1=1024, k2=64, k3=1, v0=2048, v1=1024, v2=64, v3=1)
+METADATA = dict(new=PTR, kv=PTR, kv_out=PTR, bt=PTR, free=PTR, count=PTR, count_out=PTR, cu=PTR, slots=PTR, pos=PTR, ws=0, status=0, n=2, cols=4,
+                stride=4, bs=16, capacity=8, total=4, ws_bytes=0)
+STORE = dict(CACHE, key=PTR, value=PTR, slots=PTR, status=0, tokens=2, dtype=1, s0=128, s1=64, s2=1, t0=128, t1=64, t2=1)
+ATTN = dict(CACHE, q=PTR, out=PTR, lse=0, bt=PTR, kv=PTR, cu=PTR, ws=PTR, status=0, tokens=2, seqs=2, hq=4, dtype=1, cols=4, stride=4, ws_bytes=1 << 30,
+            q0=256, q1=64, q2=1, o0=256, o1=64, o2=1, l0=0, l1=0, scale=0.125)
+E, T, C, W = _lib.FDMS_E_ARG, _lib.FDMS_E_DTYPE, _lib.FDMS_E_CAPACITY, _lib.FDMS_E_WORKSPACE
+
+
+@pytest.mark.parametrize("change,code,words", [
+    (dict(new=0), E, b"null pointer"), (dict(pos=0), E, b"null pointer"), (dict(bs=17), E, b"block_size"), (dict(stride=3), E, b"overlap"),
+    (dict(n=-1), E, b"negative"), (dict(slots=PTR + 4), E, b"aligned"), (dict(total=1 << 31), C, b"31 bits"), (dict(capacity=1 << 28), C, b"31 bits"),
+    (dict(total=1 << 20), W, b"workspace"), (dict(total=1 << 20, ws=PTR + 4, ws_bytes=99), W, b"workspace")])
+def test_c_metadata_refuses(change, code, words):
     lib = _lib.lib()
-    p = 1 << 12
-    meta = [p, p, p, p, 4, 4, 16, p, 8, p, p, p, p, p, 4, 2, None, 0, None, None]
+    assert lib.fdms_paged_metadata(P._METADATA_ARGS.pack(*(METADATA | change).values()), None) == code and words in lib.fdms_last_error()
+    assert lib.fdms_paged_metadata_workspace_bytes(-1, 4) < 0 and lib.fdms_paged_metadata_workspace_bytes(4, 4) == 0
+    assert lib.fdms_paged_metadata(None, None) == E
 
-    def refused(fn, args, change, code, words):
-        a = list(args)
-        for i, x in change.items():
-            a[i] = x
-        assert fn(*a) == code and words in lib.fdms_last_error(), lib.fdms_last_error()
 
-    refused(lib.fdms_paged_metadata, meta, {0: None}, _lib.FDMS_E_ARG, b"null pointer")
-    refused(lib.fdms_paged_metadata, meta, {6: 17}, _lib.FDMS_E_ARG, b"block_size")
-    refused(lib.fdms_paged_metadata, meta, {4: 3}, _lib.FDMS_E_ARG, b"overlap")
-    refused(lib.fdms_paged_metadata, meta, {12: p + 4}, _lib.FDMS_E_ARG, b"aligned")
-    refused(lib.fdms_paged_metadata, meta, {14: 1 << 31}, _lib.FDMS_E_CAPACITY, b"31 bits")
-    refused(lib.fdms_paged_metadata, meta, {14: 1 << 20}, _lib.FDMS_E_WORKSPACE, b"workspace")
-    assert lib.fdms_paged_metadata_workspace_bytes(-1) < 0
-    rel = [p, 2, p, 2, p, 4, 4, 16, p, 8, p, None, None]
-    refused(lib.fdms_paged_release, rel, {1: 5000}, _lib.FDMS_E_CAPACITY, b"rows a call")
-    refused(lib.fdms_paged_release, rel, {0: None, 1: 3}, _lib.FDMS_E_ARG, b"more rows")
-    st = [p, p, 1, 128, 64, 128, 64, p, p, 2048, 1024, 64, 2048, 1024, 64, p, p, p, 2, 4, 16, 2, 64, None, None]
-    refused(lib.fdms_paged_store, st, {2: 0}, _lib.FDMS_E_DTYPE, b"bf16 or f16")
-    refused(lib.fdms_paged_store, st, {22: 96}, _lib.FDMS_E_ARG, b"head_dim")
-    refused(lib.fdms_paged_store, st, {3: 129}, _lib.FDMS_E_ARG, b"aligned")
-    refused(lib.fdms_paged_store, st, {11: 8}, _lib.FDMS_E_ARG, b"aligned")
-    refused(lib.fdms_paged_store, st, {19: 1 << 28}, _lib.FDMS_E_CAPACITY, b"31 bits")
-    dec = [p, 1, 256, 64, p, p, 2048, 1024, 64, 2048, 1024, 64, p, p, 4, 16, p, 4, 4, p, p, 256, 64, None, 0, 0, 2, 4, 2, 64, 0.1, p, 1 << 30, None, None]
-    refused(lib.fdms_paged_attn_decode, dec, {1: 0}, _lib.FDMS_E_DTYPE, b"bf16 or f16")
-    refused(lib.fdms_paged_attn_decode, dec, {27: 5}, _lib.FDMS_E_ARG, b"times 1 to 64")
-    refused(lib.fdms_paged_attn_decode, dec, {31: None}, _lib.FDMS_E_ARG, b"null pointer")
-    refused(lib.fdms_paged_attn_decode, dec, {26: 2049}, _lib.FDMS_E_CAPACITY, b"2048")
-    refused(lib.fdms_paged_attn_decode, dec, {20: p + 2}, _lib.FDMS_E_ARG, b"aligned")
-    pre = [p, 1, 256, 64, p, p, 2048, 1024, 64, 2048, 1024, 64, p, p, 4, 16, p, 4, 4, p, p, 9, p, 256, 64, None, 0, 0, 2, 4, 2, 64, 0.1, None, None]
-    refused(lib.fdms_paged_attn_prefill, pre, {15: 20}, _lib.FDMS_E_ARG, b"block_size")
-    refused(lib.fdms_paged_attn_prefill, pre, {21: -1}, _lib.FDMS_E_ARG, b"negative")
-    refused(lib.fdms_paged_attn_prefill, pre, {20: None}, _lib.FDMS_E_ARG, b"null pointer")
-    refused(lib.fdms_paged_attn_prefill, pre, {7: 1000}, _lib.FDMS_E_ARG, b"aligned")
-    rel[1] = 0
-    assert lib.fdms_paged_release(*rel) == _lib.FDMS_OK and lib.fdms_last_error() == b""
+BAD_CACHE = [(dict(dtype=0), T, b"bf16 or f16"), (dict(d=96), E, b"head_dim"), (dict(bs=24), E, b"block_size"), (dict(heads=0), E, b"no KV heads"),
+             (dict(blocks=1 << 28), C, b"31 bits"), (dict(k=0), E, b"null pointer"), (dict(v=PTR + 8), E, b"aligned"), (dict(k2=72), E, b"aligned"),
+             (dict(v3=2), E, b"contiguous")]
+
+
+@pytest.mark.parametrize("change,code,words", BAD_CACHE + [
+    (dict(tokens=-1), E, b"negative"), (dict(key=0), E, b"null pointer"), (dict(s0=129), E, b"aligned"), (dict(t2=2), E, b"contiguous"),
+    (dict(value=PTR + 2), E, b"aligned")])
+def test_c_store_refuses(change, code, words):
+    lib = _lib.lib()
+    assert lib.fdms_paged_store(P._STORE_ARGS.pack(*(STORE | change).values()), None) == code and words in lib.fdms_last_error()
+    assert lib.fdms_paged_store(None, None) == E
+
+
+BAD_ATTN = BAD_CACHE + [(dict(hq=5), E, b"times 1 to 64"), (dict(hq=130), E, b"times 1 to 64"), (dict(q=0), E, b"null pointer"), (dict(kv=0), E, b"null pointer"),
+                        (dict(bt=0), E, b"null pointer"), (dict(out=PTR + 2), E, b"aligned"), (dict(q1=66), E, b"aligned"), (dict(o2=2), E, b"contiguous"),
+                        (dict(cols=1 << 28), C, b"31 bits"), (dict(seqs=-1), E, b"negative")]
+
+
+@pytest.mark.parametrize("change,code,words", BAD_ATTN + [
+    (dict(tokens=3), E, b"one token per sequence"), (dict(tokens=2049, seqs=2049), C, b"2048")])
+def test_c_decode_refuses(change, code, words):
+    lib = _lib.lib()
+    assert lib.fdms_paged_attn_decode(P._ATTN_ARGS.pack(*(ATTN | change).values()), None) == code and words in lib.fdms_last_error()
+    assert lib.fdms_paged_attn_decode(None, None) == E
+    assert lib.fdms_paged_attn_decode_workspace_bytes(2, 3, 2, 64) < 0
+
+
+@pytest.mark.parametrize("change,code,words", BAD_ATTN + [(dict(cu=0), E, b"null pointer"), (dict(tokens=-1), E, b"negative")])
+def test_c_prefill_refuses(change, code, words):
+    lib = _lib.lib()
+    assert lib.fdms_paged_attn_prefill(P._ATTN_ARGS.pack(*(ATTN | change).values()), None) == code and words in lib.fdms_last_error()
+    assert lib.fdms_paged_attn_prefill(None, None) == E
+
+
+def test_c_release_refuses():
+    lib = _lib.lib()
+    rel = dict(rows=PTR, listed=2, kv=PTR, n=2, bt=PTR, stride=4, cols=4, bs=16, free=PTR, capacity=8, count=PTR, status=None, stream=None)
+    for change, code, words in [(dict(listed=5000), C, b"rows a call"), (dict(rows=None, listed=3), E, b"more rows"), (dict(bs=8), E, b"block_size"),
+                                (dict(count=None), E, b"null pointer"), (dict(stride=3), E, b"overlap")]:
+        assert lib.fdms_paged_release(*(rel | change).values()) == code and words in lib.fdms_last_error()
+    assert lib.fdms_paged_release(*(rel | dict(listed=0)).values()) == _lib.FDMS_OK and lib.fdms_last_error() == b""
 
 
 def test_plain_statement():
