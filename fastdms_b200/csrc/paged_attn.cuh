@@ -93,87 +93,17 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
     return f16x2_of(a, b);
 }
 
-// D(16x8, f32) += A(16x16, f16) B(16x8, f16), all of the fragment's rows.
+// D(16x8, f32) += A(16x16, f16) B(16x8, f16).
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// The same with rows 8..15 of A zero: only c0, c1 (row lane / 4) carry data.
-__device__ __forceinline__ void mma_816(float& c0, float& c1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-    float d2, d3;
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%10,%10};"
-        : "+f"(c0), "+f"(c1), "=f"(d2), "=f"(d3) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.0f));
-}
-
-// One 16-row page as matrix operands.  Lane (g, t) = (lane / 4, lane % 4).
-//   Scores: B holds K^T.  Column c of the two 8-column tiles is key 4 (c / 2) + c % 2 and the same + 2, so that a lane's
-//   four scores are keys 4t .. 4t + 3, which is what the second product wants from it.  The k index is permuted: in chunk
-//   n (64 bytes of a row) lane t brings bytes 64 n + 16 t + [0, 16), four of them for each of four steps; a query fragment
-//   is loaded in the same order.
-//   Output: A holds P, its k index the keys in the order above; B holds V, column g of tile j being channel (D / 8) g + j,
-//   so that a lane loads D / 8 consecutive bytes of keys 4t .. 4t + 3 and ends up with consecutive channels.
-template <int D>
-struct PageRegs {
-    uint4 k[2][D / 64];         // keys a, a + 2; chunks
-    uint4 v[D == 128 ? 4 : 2];  // keys 4t .. 4t + 3, D / 8 bytes each (D = 64: two keys per vector)
-};
-
-template <int D>
-__device__ __forceinline__ void load_k(PageRegs<D>& p, const uint8_t* k, int64_t sr, int lane) {
-    const int g = lane >> 2, t = lane & 3, key = 4 * (g >> 1) + (g & 1);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int n = 0; n < D / 64; ++n) p.k[i][n] = __ldg((const uint4*)(k + (key + 2 * i) * sr + 64 * n + 16 * t));
-}
-template <int D>
-__device__ __forceinline__ void load_v(PageRegs<D>& p, const uint8_t* v, int64_t sr, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    if (D == 128) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p.v[i] = __ldg((const uint4*)(v + (4 * t + i) * sr + 16 * g));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint2 a = __ldg((const uint2*)(v + (4 * t + 2 * i) * sr + 8 * g));
-            const uint2 b = __ldg((const uint2*)(v + (4 * t + 2 * i + 1) * sr + 8 * g));
-            p.v[i] = make_uint4(a.x, a.y, b.x, b.y);
-        }
-    }
-}
-template <int D>
-__device__ __forceinline__ void zero_page(PageRegs<D>& p) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int n = 0; n < D / 64; ++n) p.k[i][n] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < (D == 128 ? 4 : 2); ++i) p.v[i] = make_uint4(0, 0, 0, 0);
-}
-// Word w (channels 4w .. 4w + 3 of the lane's) of key 4t + i.
-template <int D>
-__device__ __forceinline__ uint32_t v_word(const PageRegs<D>& p, int i, int w) {
-    const uint4& x = D == 128 ? p.v[i] : p.v[i >> 1];
-    const int n = D == 128 ? w : (i & 1) * 2 + w;
-    return n == 0 ? x.x : n == 1 ? x.y : n == 2 ? x.z : x.w;
-}
-// Rows at and beyond `rows` hold whatever the memory held: zero, so that P = 0 leaves no trace of them.
-template <int D>
-__device__ __forceinline__ void mask_v(PageRegs<D>& p, int rows, int lane) {
-    const int t = lane & 3;
-    if (D == 128) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (4 * t + i >= rows) p.v[i] = make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (4 * t + 2 * i >= rows) p.v[i].x = p.v[i].y = 0;
-            if (4 * t + 2 * i + 1 >= rows) p.v[i].z = p.v[i].w = 0;
-        }
-    }
+// An 8x8 matrix of 16-bit values, lane (g, t) holding row g, columns 2t and 2t + 1, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 // Checks of a cache that every entry makes; `idle`: the call has nothing to do, so its pointers may be null.
@@ -212,6 +142,8 @@ inline int32_t paged_attn_check(const char* name, const fdms_paged_attn_args* ar
         FDMS_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)(2 * strides)) & 15) == 0 && p.q_stride[2] == 1 && p.out_stride[2] == 1, FDMS_E_ARG,
                      "%s: q and out must be contiguous in their last dimension and aligned to 16 bytes in the others", name);
     }
+    FDMS_REQUIRE(c.num_blocks == 0 || (c.k_stride[0] < (1ll << 32) && c.v_stride[0] < (1ll << 32) && c.k_stride[2] <= (1 << 24) && c.v_stride[2] <= (1 << 24)),
+                 FDMS_E_CAPACITY, "%s: a block's stride must fit in 32 bits, a row's in 24", name);
     view = {c.k, c.v, c.k_stride[0], c.k_stride[1], c.k_stride[2], c.v_stride[0], c.v_stride[1], c.v_stride[2], c.k_scale, c.v_scale,
             p.block_tables, p.bt_stride, p.kv_lens, p.dev_status, (int32_t)c.num_blocks, (int32_t)p.max_blocks, (int32_t)c.kv_heads, shift};
     return FDMS_OK;

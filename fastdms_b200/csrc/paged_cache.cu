@@ -276,10 +276,12 @@ __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
 // Store.  A token begins a run when its slot opens a block or does not follow the token before it; a run ends with its
 // block, so that a (run, head) of K or of V is one piece of work with a scale of its own: amax over the run's rows,
 // 2^k the least with amax <= 448 * 2^k, the maximum with the block's scale where it holds earlier rows.
-// One warp per 16 rows of the block keeps its rows in registers between the two passes (amax, rounding), so that every
-// row is read once; larger blocks exchange their maxima through shared memory.
+// A warp keeps 16 rows of the block in registers between the two passes (amax, rounding).  Steps of many tokens give
+// every 16 rows of a block a warp of their own, so that each row is read once, and exchange the maxima through shared
+// memory; in small steps, where one token per block is the rule, a warp takes the whole block.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kStoreWarps = 8;
+constexpr int64_t kStoreSmall = 1024;           // tokens
 constexpr int kScaleExpMin = -60, kScaleExpMax = 40;
 
 struct StoreArgs {
@@ -292,7 +294,7 @@ struct StoreArgs {
     int32_t* status;
     int64_t tokens;
     int64_t num_slots;
-    int32_t heads, shift, group;                // group: tokens per CTA
+    int32_t heads, shift, group, warps;         // tokens per CTA, warps per (run, head)
 };
 
 // Exponent k of the scale for a largest magnitude.
@@ -327,14 +329,13 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
 
 // D: head_dim.  A lane holds 8 elements of every (32 / (D / 8))-th row of the warp's 16.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kStoreWarps * 32) paged_store_kernel(StoreArgs a) {
+__global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreArgs a) {
     constexpr int kLanes = D / 8;               // lanes per row
     constexpr int kRows = 32 / kLanes;          // rows per step
     constexpr int kSteps = 16 / kRows;
     __shared__ float s_max[kStoreWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int W = (1 << a.shift) >> 4;          // warps per piece of work
-    const int per_cta = kStoreWarps / W;
+    const int W = a.warps, per_cta = kStoreWarps / W;
     const int item = blockIdx.y * per_cta + warp / W, part = warp % W;
     const bool have = item < 2 * a.heads;
     const int which = have && item >= a.heads ? 1 : 0, head = have ? item - which * a.heads : 0;
@@ -365,6 +366,8 @@ __global__ void __launch_bounds__(kStoreWarps * 32) paged_store_kernel(StoreArgs
         const int64_t t0 = first + src_lane;
         const int32_t slot = __shfl_sync(0xffffffffu, my_slot, src_lane);
         const int block = slot >> a.shift, off = slot & (bs - 1);
+        float* scale = a.scale[which] + (int64_t)block * a.heads + head;
+        const float old = have && off > 0 ? *scale : 0.0f;
         int count = 1;                          // rows of the run: slots that follow one another, inside the block
         for (int base = 1; base < bs - off; base += 32) {
             const int i = base + lane;
@@ -374,29 +377,35 @@ __global__ void __launch_bounds__(kStoreWarps * 32) paged_store_kernel(StoreArgs
             count += run;
             if (run < 32) break;
         }
+        // the 16-row parts of the block that this warp writes
+        const int lo = W > 1 ? part : off >> 4, hi = W > 1 ? part : (off + count - 1) >> 4;
+        const uint16_t* src = a.src[which] + t0 * a.src_st[which] + (int64_t)head * a.src_sh[which] + col;
+        uint8_t* dst = a.cache[which] + (int64_t)block * a.sb[which] + (int64_t)head * a.sh[which] + col;
         uint4 x[kSteps];
+        auto load = [&](int p) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int r = p * 16 + j * kRows + row0 - off;      // row of the run
+                x[j] = make_uint4(0, 0, 0, 0);
+                if (have && r >= 0 && r < count) x[j] = __ldg((const uint4*)(src + r * a.src_st[which]));
+            }
+        };
         float top = 0.0f;
-        const uint16_t* src = a.src[which] + (int64_t)head * a.src_sh[which] + col;
+        for (int p = lo; p <= hi; ++p) {
+            load(p);
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const int r = part * 16 + j * kRows + row0 - off;       // row of the run
-            x[j] = make_uint4(0, 0, 0, 0);
-            if (have && r >= 0 && r < count) x[j] = __ldcs((const uint4*)(src + (t0 + r) * a.src_st[which]));
-        }
+            for (int j = 0; j < kSteps; ++j) {
+                const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float f, g;
-                unpack2<BF16>(w[i], f, g);
-                top = fmaxf(top, fmaxf(fabsf(f), fabsf(g)));        // a NaN does not count
+                for (int i = 0; i < 4; ++i) {
+                    float f, g;
+                    unpack2<BF16>(w[i], f, g);
+                    top = fmaxf(top, fmaxf(fabsf(f), fabsf(g)));    // a NaN does not count
+                }
             }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float* scale = a.scale[which] + (int64_t)block * a.heads + head;
-        const float old = have && off > 0 ? *scale : 0.0f;
         if (W > 1) {
             if (lane == 0) s_max[warp] = top;
             __syncthreads();
@@ -404,25 +413,28 @@ __global__ void __launch_bounds__(kStoreWarps * 32) paged_store_kernel(StoreArgs
             __syncthreads();
         }
         if (!have) continue;
-        const float fresh = pow2(scale_exponent(top));
-        const float now = fmaxf(old, fresh);
+        const float now = fmaxf(old, pow2(scale_exponent(top)));
         const float inv = __frcp_rn(now);       // exact for a power of two
-        uint8_t* dst = a.cache[which] + (int64_t)block * a.sb[which] + (int64_t)head * a.sh[which] + col;
-        const bool moves = old > 0.0f && old < now;
-        const float ratio = old * inv;
+        for (int p = lo; p <= hi; ++p) {
+            if (lo < hi) load(p);
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const int br = part * 16 + j * kRows + row0, r = br - off;
-            uint2* p = (uint2*)(dst + (int64_t)br * a.sr[which]);
-            if (r >= 0 && r < count) {
+            for (int j = 0; j < kSteps; ++j) {
+                const int br = p * 16 + j * kRows + row0, r = br - off;
+                if (r < 0 || r >= count) continue;
                 const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) unpack2<BF16>(w[i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] *= inv;
-                *p = make_uint2(pack_e4m3x4(f[0], f[1], f[2], f[3]), pack_e4m3x4(f[4], f[5], f[6], f[7]));
-            } else if (r < 0 && moves) {        // an earlier row of the block moves to the larger scale
+                *(uint2*)(dst + br * a.sr[which]) = make_uint2(pack_e4m3x4(f[0], f[1], f[2], f[3]), pack_e4m3x4(f[4], f[5], f[6], f[7]));
+            }
+        }
+        if (old > 0.0f && old < now) {          // the earlier rows of the block move to the larger scale
+            const float ratio = old * inv;
+            const int end = min(off, W > 1 ? 16 * part + 16 : off);
+            for (int br = (W > 1 ? 16 * part : 0) + row0; br < end; br += kRows) {
+                uint2* p = (uint2*)(dst + br * a.sr[which]);
                 const uint2 c = *p;
                 float f[8];
 #pragma unroll
@@ -529,14 +541,15 @@ extern "C" int32_t fdms_paged_store(const fdms_paged_store_args* args, void* str
     const uintptr_t act = (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)(2 * (p.k_stride[0] | p.k_stride[1] | p.v_stride[0] | p.v_stride[1]));
     FDMS_REQUIRE((act & 15) == 0 && p.k_stride[2] == 1 && p.v_stride[2] == 1, FDMS_E_ARG,
                  "fdms_paged_store: key and value must be contiguous in their last dimension and aligned to 16 bytes in the others");
-    const int W = (int)c.block_size / 16, per_cta = kStoreWarps / W;
+    // Small steps: a warp per (run, head); large ones: one per 16 rows of it.
+    const int W = p.tokens <= kStoreSmall ? 1 : (int)c.block_size / 16, per_cta = kStoreWarps / W;
     // Tokens per CTA: few runs begin in a prompt's tokens, one at every token of a decode batch.  1024 CTAs keep the GPU
     // busy either way; more than a block's worth of tokens per CTA would only make them unequal.
     int group = 1;
     while (group < 16 && p.tokens > (int64_t)group * 1024) group *= 2;
     StoreArgs a = {{(const uint16_t*)p.k, (const uint16_t*)p.v}, {p.k_stride[0], p.v_stride[0]}, {p.k_stride[1], p.v_stride[1]}, {c.k, c.v},
                    {c.k_stride[0], c.v_stride[0]}, {c.k_stride[1], c.v_stride[1]}, {c.k_stride[2], c.v_stride[2]}, {c.k_scale, c.v_scale},
-                   p.slot_mapping, p.dev_status, p.tokens, c.num_blocks << shift, (int32_t)c.kv_heads, shift, group};
+                   p.slot_mapping, p.dev_status, p.tokens, c.num_blocks << shift, (int32_t)c.kv_heads, shift, group, W};
     const int64_t ctas = (p.tokens + group - 1) / group;
     FDMS_REQUIRE(ctas < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_store: too many tokens");
     const dim3 grid((unsigned)ctas, (unsigned)((2 * c.kv_heads + per_cta - 1) / per_cta));

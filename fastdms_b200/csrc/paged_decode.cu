@@ -29,6 +29,242 @@ struct DecodeArgs {
     float scale;
 };
 
+// One 16-row page as matrix operands; lane (g, t) = (lane / 4, lane % 4).  Both products run transposed, the page's codes
+// being the 16-row operand and up to 8 q heads the 8 columns, so that no row of a fragment is idle:
+//   S^T = K Q^T: A holds keys g and g + 8; in chunk n (64 bytes of a row) lane t brings bytes 64 n + 16 t + [0, 16), four of
+//   them for each of four steps of 16 channels, and the query fragment is loaded in the same order.
+//   O^T = V^T P^T: A holds channels; of keys 2t, 2t + 1, 2t + 8, 2t + 9 a lane loads D / 8 consecutive bytes, tile j taking
+//   channels (D / 8) g + 2j and + 1 as its rows g and g + 8.  P^T comes out of S^T's layout by an 8x8 transpose in the warp.
+template <int D>
+struct PageRegs {
+    uint4 k[2][D / 64];         // keys g, g + 8; chunks
+    uint4 v[D == 128 ? 4 : 2];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 (D = 64: two keys per vector)
+};
+
+template <int D>
+__device__ __forceinline__ void load_k(PageRegs<D>& p, const uint8_t* k, uint32_t sr) {     // k: the lane's first vector
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) p.k[i][n] = __ldg((const uint4*)(k + 8 * i * sr + 64 * n));
+}
+template <int D>
+__device__ __forceinline__ void load_v(PageRegs<D>& p, const uint8_t* v, uint32_t sr) {
+    if (D == 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.v[i] = __ldg((const uint4*)(v + ((i & 1) + 8 * (i >> 1)) * sr));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint2 a = __ldg((const uint2*)(v + 8 * i * sr)), b = __ldg((const uint2*)(v + (8 * i + 1) * sr));
+            p.v[i] = make_uint4(a.x, a.y, b.x, b.y);
+        }
+    }
+}
+// Word w (channels 4w .. 4w + 3 of the lane's) of the lane's key i.
+template <int D>
+__device__ __forceinline__ uint32_t v_word(const PageRegs<D>& p, int i, int w) {
+    const uint4& x = D == 128 ? p.v[i] : p.v[i >> 1];
+    const int n = D == 128 ? w : (i & 1) * 2 + w;
+    return n == 0 ? x.x : n == 1 ? x.y : n == 2 ? x.z : x.w;
+}
+// Rows at and beyond `rows` hold whatever the memory held: zero, so that P = 0 leaves no trace of them.
+template <int D>
+__device__ __forceinline__ void mask_v(PageRegs<D>& p, int rows, int t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (2 * t + (i & 1) + 8 * (i >> 1) >= rows) {
+            if (D == 128) p.v[i] = make_uint4(0, 0, 0, 0);
+            else if (i & 1) p.v[i >> 1].z = p.v[i >> 1].w = 0;
+            else p.v[i >> 1].x = p.v[i >> 1].y = 0;
+        }
+}
+
+// What a warp keeps of a unit: lane (g, t) holds heads 2t and 2t + 1, channels (D / 8) g + [0, D / 8) in o (o[j]: channel
+// 2j of both heads, channel 2j + 1 of both), M of the two heads and its share of l.
+template <int D>
+struct UnitState {
+    float o[D / 16][4];
+    float m[2], l[2];
+};
+
+template <int D>
+__device__ __forceinline__ void clear(UnitState<D>& u) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) u.o[j][0] = u.o[j][1] = u.o[j][2] = u.o[j][3] = 0.0f;
+    u.m[0] = u.m[1] = -INFINITY;
+    u.l[0] = u.l[1] = 0.0f;
+}
+
+// Query fragments of head `row` (column g of the products), brought to a power of two; the factor of the scores of heads
+// 2t and 2t + 1 comes from the lanes that loaded them.
+template <int D, bool BF16>
+__device__ __forceinline__ void load_q(const uint16_t* q, float scale, uint32_t (&qb)[D / 16][2], float (&factor)[2], int lane) {
+    const int t = lane & 3;
+    uint4 w[D / 64][2];
+    float top = 0.0f;
+#pragma unroll
+    for (int n = 0; n < D / 64; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[n][i] = *(const uint4*)(q + 64 * n + 16 * t + 8 * i);
+#pragma unroll
+    for (int n = 0; n < D / 64; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t x[4] = {w[n][i].x, w[n][i].y, w[n][i].z, w[n][i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float e, f;
+                unpack_pair<BF16>(x[j], e, f);
+                top = fmaxf(top, fmaxf(fabsf(e), fabsf(f)));
+            }
+        }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float up, down;
+    row_power(top, up, down);
+    down *= scale * kPagedLog2e;
+    factor[0] = __shfl_sync(0xffffffffu, down, 8 * t);
+    factor[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+    for (int n = 0; n < D / 64; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t x[4] = {w[n][i].x, w[n][i].y, w[n][i].z, w[n][i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {       // element 16 t + 8 i + 2 j of the chunk: step 2 i + j / 2, half j % 2
+                float e, f;
+                unpack_pair<BF16>(x[j], e, f);
+                qb[4 * n + 2 * i + (j >> 1)][j & 1] = f16x2_of(e * up, f * up);
+            }
+        }
+}
+
+// S^T of a page.
+template <int D>
+__device__ __forceinline__ void page_scores(const PageRegs<D>& p, const uint32_t (&qb)[D / 16][2], float (&s)[4]) {
+    s[0] = s[1] = s[2] = s[3] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < D / 64; ++n) {
+        const uint32_t x[4] = {p.k[0][n].x, p.k[0][n].y, p.k[0][n].z, p.k[0][n].w}, y[4] = {p.k[1][n].x, p.k[1][n].y, p.k[1][n].z, p.k[1][n].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_f16(x[j], a0, a2);
+            e4m3x4_f16(y[j], a1, a3);
+            mma_16816(s, a0, a1, a2, a3, qb[4 * n + j][0], qb[4 * n + j][1]);
+        }
+    }
+}
+
+// Scores to weights, l, and P^T; `rows` of the page count.  M follows the maximum only when that is ahead by more than 2^8:
+// P stays below 256 and most pages need no maximum over the keys and rescale nothing.
+template <int D>
+__device__ __forceinline__ void page_weights(UnitState<D>& u, float (&s)[4], float ks, float lvs, float ivs, const float (&factor)[2], int rows,
+                                             int lane, uint32_t& b0, uint32_t& b1) {
+    const int g = lane >> 2;
+    const float f0 = ks * factor[0], f1 = ks * factor[1];
+    float x[4] = {fmaf(s[0], f0, lvs), fmaf(s[1], f1, lvs), fmaf(s[2], f0, lvs), fmaf(s[3], f1, lvs)};
+    if (rows < kCachePage) {
+        if (g >= rows) x[0] = x[1] = -INFINITY;
+        if (g + 8 >= rows) x[2] = x[3] = -INFINITY;
+    }
+    const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
+    if (__any_sync(0xffffffffu, t0 > u.m[0] + 8.0f || t1 > u.m[1] + 8.0f)) {
+        float top[2] = {t0, t1};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+            const float next = fmaxf(u.m[i], top[i]);
+            const float r = next == -INFINITY ? 1.0f : paged_ex2(u.m[i] - next);
+            u.m[i] = next;
+            u.l[i] *= r;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) { u.o[j][i] *= r; u.o[j][2 + i] *= r; }
+        }
+    }
+    const float r0 = u.m[0] == -INFINITY ? 0.0f : u.m[0], r1 = u.m[1] == -INFINITY ? 0.0f : u.m[1];
+    x[0] = paged_ex2(x[0] - r0);
+    x[2] = paged_ex2(x[2] - r0);
+    x[1] = paged_ex2(x[1] - r1);
+    x[3] = paged_ex2(x[3] - r1);
+    u.l[0] = fmaf(x[0] + x[2], ivs, u.l[0]);
+    u.l[1] = fmaf(x[1] + x[3], ivs, u.l[1]);
+    b0 = transpose_8x8(f16x2_of(x[0], x[1]));
+    b1 = transpose_8x8(f16x2_of(x[2], x[3]));
+}
+
+// O^T of a page.
+template <int D>
+__device__ __forceinline__ void page_values(UnitState<D>& u, const PageRegs<D>& p, uint32_t b0, uint32_t b1) {
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+        const uint32_t k0 = v_word<D>(p, 0, w), k1 = v_word<D>(p, 1, w), k2 = v_word<D>(p, 2, w), k3 = v_word<D>(p, 3, w);
+        uint32_t a[2][4];
+        e4m3x4_f16(__byte_perm(k0, k1, 0x5140), a[0][0], a[0][1]);
+        e4m3x4_f16(__byte_perm(k0, k1, 0x7362), a[1][0], a[1][1]);
+        e4m3x4_f16(__byte_perm(k2, k3, 0x5140), a[0][2], a[0][3]);
+        e4m3x4_f16(__byte_perm(k2, k3, 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma_16816(u.o[2 * w + j], a[j][0], a[j][1], a[j][2], a[j][3], b0, b1);
+    }
+}
+
+// The warp's pages first, first + step, ... (`count` of them) of a sequence's KV head, whose first `len` rows count.  32 of
+// them at a time, one per lane, are looked up in the table.
+template <int D>
+__device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u, const uint32_t (&qb)[D / 16][2], const float (&factor)[2],
+                                           int seq, int head, int first, int step, int count, int len) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int ppb = c.shift - 4, in_block = (1 << ppb) - 1;
+    const uint32_t k_sr = (uint32_t)c.k_sr, v_sr = (uint32_t)c.v_sr;
+    const uint8_t* kb = c.k + head * c.k_sh + g * c.k_sr + 16 * t;
+    const uint8_t* vb = c.v + head * c.v_sh + 2 * t * c.v_sr + (D / 8) * g;
+    const int32_t* table = c.tables + seq * c.table_stride;
+    for (int base = 0; base < count; base += 32) {
+        int my_block = -1;
+        float my_ks = 0.0f, my_vs = 1.0f;
+        if (base + lane < count) {
+            my_block = table[(first + step * (base + lane)) >> ppb];
+            if (my_block < 0 || my_block >= c.num_blocks) {
+                my_block = -1;
+                if (c.status) atomicOr(c.status, FDMS_DEV_BAD_INDEX);
+            } else {
+                my_ks = c.k_scale[(int64_t)my_block * c.heads + head];
+                my_vs = c.v_scale[(int64_t)my_block * c.heads + head];
+            }
+        }
+        const float my_lvs = paged_lg2(my_vs), my_ivs = __frcp_rn(my_vs);
+        const int n = min(32, count - base);
+        PageRegs<D> pg;
+        auto block_of = [&](int i) { return __shfl_sync(0xffffffffu, my_block, i); };
+        auto row_of = [&](int i) { return (uint32_t)((first + step * (base + i)) & in_block) * kCachePage; };
+        // a page that is left out reads block 0, and none of its rows count
+        auto fetch_k = [&](int i) {
+            load_k<D>(pg, kb + (uint64_t)(uint32_t)max(block_of(i), 0) * (uint32_t)c.k_sb + row_of(i) * k_sr, k_sr);
+        };
+        auto fetch_v = [&](int i) {
+            load_v<D>(pg, vb + (uint64_t)(uint32_t)max(block_of(i), 0) * (uint32_t)c.v_sb + row_of(i) * v_sr, v_sr);
+        };
+        if (c.num_blocks == 0) return;          // nothing to read, not even block 0
+        fetch_k(0);
+        fetch_v(0);
+        for (int i = 0; i < n; ++i) {
+            const int rows = block_of(i) < 0 ? 0 : min(kCachePage, len - (first + step * (base + i)) * kCachePage);
+            float s[4];
+            page_scores<D>(pg, qb, s);
+            if (i + 1 < n) fetch_k(i + 1);
+            uint32_t b0, b1;
+            page_weights<D>(u, s, __shfl_sync(0xffffffffu, my_ks, i), __shfl_sync(0xffffffffu, my_lvs, i), __shfl_sync(0xffffffffu, my_ivs, i),
+                            factor, rows, lane, b0, b1);
+            if (rows < kCachePage) mask_v<D>(pg, rows, t);
+            page_values<D>(u, pg, b0, b1);
+            if (i + 1 < n) fetch_v(i + 1);
+        }
+    }
+}
+
 // Pages before sequence b for all b (and in total), in shared memory; by all threads of the CTA.
 __device__ __forceinline__ void page_prefix(const DecodeArgs& a, int32_t* s_first, int32_t* s_warp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -69,6 +305,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
     __shared__ float s_o[kDecWarps][kDecHeads][D];
     __shared__ float s_m[kDecWarps][kDecHeads], s_l[kDecWarps][kDecHeads];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    static_assert(kDecWarps == kDecHeads, "the merge gives a head to a warp");
     pdl_trigger();
     page_prefix(a, s_first, s_warp);
     const int per_seq = a.c.heads * a.splits;
@@ -97,7 +334,6 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         }
         seq = lo;
     }
-    const int ppb = a.c.shift - 4;              // log2(pages per block)
     int64_t at = begin;
     while (at < end) {
         while ((int64_t)s_first[seq + 1] * per_seq <= at) ++seq;
@@ -108,182 +344,58 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         const int p0 = (int)(at - unit_begin), p1 = (int)min((int64_t)pages, end - unit_begin);
         const int head = u / a.splits, h0 = (u % a.splits) * kDecHeads, nh = min(kDecHeads, a.group - h0);
         const int len = min(paged_len(a.c, seq), pages * kCachePage);
-
-        // query fragments: row g of the unit's heads
-        uint32_t qa[D / 16][2];
-        float factor = 0.0f;
-        {
-            const uint16_t* q = a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh;
-            uint4 w[D / 64][2];
-            float top = 0.0f;
+        uint32_t qb[D / 16][2];
+        float factor[2];
+        load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
+        UnitState<D> st;
+        clear<D>(st);
+        walk_pages<D>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len);
+        // merge the warps
 #pragma unroll
-            for (int n = 0; n < D / 64; ++n)
+        for (int i = 0; i < 2; ++i) {
+            float l = st.l[i];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    w[n][i] = *(const uint4*)(q + 64 * n + 16 * t + 8 * i);
-                    const uint32_t x[4] = {w[n][i].x, w[n][i].y, w[n][i].z, w[n][i].w};
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (g == 0) { s_m[warp][2 * t + i] = st.m[i]; s_l[warp][2 * t + i] = l; }
+            if (2 * t + i < nh)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float e, f;
-                        unpack_pair<BF16>(x[j], e, f);
-                        top = fmaxf(top, fmaxf(fabsf(e), fabsf(f)));
-                    }
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            float up;
-            row_power(top, up, factor);
-            factor *= a.scale * kPagedLog2e;
-#pragma unroll
-            for (int n = 0; n < D / 64; ++n)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t x[4] = {w[n][i].x, w[n][i].y, w[n][i].z, w[n][i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float e, f;
-                        unpack_pair<BF16>(x[j], e, f);
-                        // element 16 t + 8 i + 2 j of the chunk: step 2 i + j / 2, half j % 2
-                        qa[4 * n + 2 * i + (j >> 1)][j & 1] = f16x2_of(e * up, f * up);
-                    }
-                }
+                for (int j = 0; j < D / 16; j += 2)
+                    *(float4*)&s_o[warp][2 * t + i][(D / 8) * g + 2 * j] =
+                        make_float4(st.o[j][i], st.o[j][2 + i], st.o[j + 1][i], st.o[j + 1][2 + i]);
         }
-        float o[D / 8][2], m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = 0.0f;
-
-        // the warp's pages: p0 + warp + 8 i; 32 of them at a time, one per lane, are looked up in the table
-        const int mine = p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0;
-        for (int base = 0; base < mine; base += 32) {
-            int my_block = -1;
-            float my_ks = 0.0f, my_vs = 1.0f;
-            if (base + lane < mine) {
-                const int p = p0 + warp + kDecWarps * (base + lane);
-                my_block = a.c.tables[seq * a.c.table_stride + (p >> ppb)];
-                if (my_block < 0 || my_block >= a.c.num_blocks) {
-                    my_block = -1;
-                    if (a.c.status) atomicOr(a.c.status, FDMS_DEV_BAD_INDEX);
-                } else {
-                    my_ks = a.c.k_scale[(int64_t)my_block * a.c.heads + head];
-                    my_vs = a.c.v_scale[(int64_t)my_block * a.c.heads + head];
-                }
-            }
-            const float my_lvs = paged_lg2(my_vs), my_ivs = __frcp_rn(my_vs);
-            const int n = min(32, mine - base);
-            PageRegs<D> pg;
-            auto fetch_k = [&](int i) {
-                const int blk = __shfl_sync(0xffffffffu, my_block, i);
-                const int p = p0 + warp + kDecWarps * (base + i);
-                const int row = (p & ((1 << ppb) - 1)) * kCachePage;
-                if (blk >= 0) load_k<D>(pg, a.c.k + (int64_t)blk * a.c.k_sb + head * a.c.k_sh + row * a.c.k_sr, a.c.k_sr, lane);
-            };
-            auto fetch_v = [&](int i) {
-                const int blk = __shfl_sync(0xffffffffu, my_block, i);
-                const int p = p0 + warp + kDecWarps * (base + i);
-                const int row = (p & ((1 << ppb) - 1)) * kCachePage;
-                if (blk >= 0) load_v<D>(pg, a.c.v + (int64_t)blk * a.c.v_sb + head * a.c.v_sh + row * a.c.v_sr, a.c.v_sr, lane);
-            };
-            zero_page<D>(pg);
-            fetch_k(0);
-            fetch_v(0);
-            for (int i = 0; i < n; ++i) {
-                const int blk = __shfl_sync(0xffffffffu, my_block, i);
-                const float ks = __shfl_sync(0xffffffffu, my_ks, i) * factor;
-                const float lvs = __shfl_sync(0xffffffffu, my_lvs, i), ivs = __shfl_sync(0xffffffffu, my_ivs, i);
-                const int p = p0 + warp + kDecWarps * (base + i);
-                const int rows = blk < 0 ? 0 : min(kCachePage, len - p * kCachePage);
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t b0, b1;
-                        e4m3x4_f16(j == 0 ? pg.k[0][c].x : j == 1 ? pg.k[0][c].y : j == 2 ? pg.k[0][c].z : pg.k[0][c].w, b0, b1);
-                        mma_816(s[0], s[1], qa[4 * c + j][0], qa[4 * c + j][1], b0, b1);
-                        e4m3x4_f16(j == 0 ? pg.k[1][c].x : j == 1 ? pg.k[1][c].y : j == 2 ? pg.k[1][c].z : pg.k[1][c].w, b0, b1);
-                        mma_816(s[2], s[3], qa[4 * c + j][0], qa[4 * c + j][1], b0, b1);
-                    }
-                }
-                if (i + 1 < n) fetch_k(i + 1);
-                float top = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[j] = 4 * t + j < rows ? fmaf(s[j], ks, lvs) : -INFINITY;
-                    top = fmaxf(top, s[j]);
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // M follows the maximum only when it lags by more than 2^8: P stays below 256, and most pages rescale nothing
-                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                    const float next = fmaxf(m, top);
-                    const float r = next == -INFINITY ? 1.0f : paged_ex2(m - next);
-                    m = next;
-                    l *= r;
-#pragma unroll
-                    for (int j = 0; j < D / 8; ++j) { o[j][0] *= r; o[j][1] *= r; }
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[j] = paged_ex2(s[j] - ref);
-                l = fmaf((s[0] + s[1]) + (s[2] + s[3]), ivs, l);
-                const uint32_t a0 = f16x2_of(s[0], s[1]), a2 = f16x2_of(s[2], s[3]);
-                if (rows < kCachePage) mask_v<D>(pg, rows, lane);
-#pragma unroll
-                for (int w = 0; w < D / 32; ++w) {
-                    const uint32_t k0 = v_word<D>(pg, 0, w), k1 = v_word<D>(pg, 1, w), k2 = v_word<D>(pg, 2, w), k3 = v_word<D>(pg, 3, w);
-                    uint32_t b0[4], b1[4];
-                    e4m3x4_f16(__byte_perm(k0, k1, 0x5140), b0[0], b0[1]);
-                    e4m3x4_f16(__byte_perm(k0, k1, 0x7362), b0[2], b0[3]);
-                    e4m3x4_f16(__byte_perm(k2, k3, 0x5140), b1[0], b1[1]);
-                    e4m3x4_f16(__byte_perm(k2, k3, 0x7362), b1[2], b1[3]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_816(o[4 * w + j][0], o[4 * w + j][1], a0, a2, b0[j], b1[j]);
-                }
-                if (i + 1 < n) fetch_v(i + 1);
-            }
-        }
-        // merge the warps: lane (g, t) holds head g, channels (D/8) (2t) + j and (D/8) (2t + 1) + j
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) { s_m[warp][g] = m; s_l[warp][g] = l; }
-#pragma unroll
-        for (int j = 0; j < D / 8; j += 4)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                *(float4*)&s_o[warp][g][(D / 8) * (2 * t + i) + j] = make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
         __syncthreads();
         const bool whole = p0 == 0 && p1 == pages;
         const int slot = blockIdx.x * 2 + (at == begin ? 0 : 1);
-        constexpr int kVec = kDecHeads * D / kDecThreads;       // channels per thread: a head is D / kVec threads
-        const int hd = threadIdx.x / (D / kVec), ch = (threadIdx.x % (D / kVec)) * kVec;
-        float mm = -INFINITY;
+        constexpr int kVec = kDecHeads * D / kDecThreads;       // channels per thread: a head is a warp
+        const int hd = warp, ch = lane * kVec;
+        if (hd < nh) {
+            float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][hd]);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        float ll = 0.0f, acc[kVec];
+            for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][hd]);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+            float ll = 0.0f, acc[kVec];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) {
-            const float r = paged_ex2(s_m[w][hd] - ref);
-            ll = fmaf(s_l[w][hd], r, ll);
+            for (int w = 0; w < kDecWarps; ++w) {
+                const float r = paged_ex2(s_m[w][hd] - ref);
+                ll = fmaf(s_l[w][hd], r, ll);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) acc[i] = fmaf(s_o[w][hd][ch + i], r, acc[i]);
-        }
-        if (whole) {
-            if (hd < nh) {
-                const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
+                for (int i = 0; i < kVec; ++i) acc[i] = fmaf(s_o[w][hd][ch + i], r, acc[i]);
+            }
+            if (whole) {
+                const float inv = ll > 0.0f || ll != ll ? __frcp_rn(ll) : 0.0f;
                 uint16_t* out = a.out + seq * a.o_sb + (int64_t)(head * a.group + h0 + hd) * a.o_sh + ch;
 #pragma unroll
                 for (int i = 0; i < kVec; i += 2) *(uint32_t*)(out + i) = pack_pair<BF16>(acc[i] * inv, acc[i + 1] * inv);
-                if (a.lse && ch == 0)
+                if (a.lse && lane == 0)
                     a.lse[seq * a.lse_sb + (int64_t)(head * a.group + h0 + hd) * a.lse_sh] = kPagedLn2 * (mm + paged_lg2(ll));
-            }
-        } else {
-            float* part = a.parts + ((int64_t)slot * kDecHeads + hd) * (D + 4);
+            } else {
+                float* part = a.parts + ((int64_t)slot * kDecHeads + hd) * (D + 4);
 #pragma unroll
-            for (int i = 0; i < kVec; i += 2) *(float2*)(part + ch + i) = make_float2(acc[i], acc[i + 1]);
-            if (ch == 0) *(float2*)(part + D) = make_float2(mm, ll);
+                for (int i = 0; i < kVec; i += 2) *(float2*)(part + ch + i) = make_float2(acc[i], acc[i + 1]);
+                if (lane == 0) *(float2*)(part + D) = make_float2(mm, ll);
+            }
         }
         if (p0 == 0 && threadIdx.x == 0) {
             const int2 cut = whole ? make_int2(0, -1) : make_int2(slot, owner(unit_begin + pages - 1, ctas, total));

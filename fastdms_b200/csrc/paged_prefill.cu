@@ -8,6 +8,75 @@ namespace fdms {
 constexpr int kPreWarps = 4;
 constexpr int kPreRows = kPreWarps * 16;        // (token, q head) rows of a CTA, heads of a token together
 
+// One 16-row page as matrix operands.  Lane (g, t) = (lane / 4, lane % 4).
+//   Scores: B holds K^T.  Column c of the two 8-column tiles is key 4 (c / 2) + c % 2 and the same + 2, so that a lane's
+//   four scores are keys 4t .. 4t + 3, which is what the second product wants from it.  The k index is permuted: in chunk
+//   n (64 bytes of a row) lane t brings bytes 64 n + 16 t + [0, 16), four of them for each of four steps; a query fragment
+//   is loaded in the same order.
+//   Output: A holds P, its k index the keys in the order above; B holds V, column g of tile j being channel (D / 8) g + j,
+//   so that a lane loads D / 8 consecutive bytes of keys 4t .. 4t + 3 and ends up with consecutive channels.
+template <int D>
+struct PageRegs {
+    uint4 k[2][D / 64];         // keys a, a + 2; chunks
+    uint4 v[D == 128 ? 4 : 2];  // keys 4t .. 4t + 3, D / 8 bytes each (D = 64: two keys per vector)
+};
+
+template <int D>
+__device__ __forceinline__ void load_k(PageRegs<D>& p, const uint8_t* k, int64_t sr, int lane) {
+    const int g = lane >> 2, t = lane & 3, key = 4 * (g >> 1) + (g & 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) p.k[i][n] = __ldg((const uint4*)(k + (key + 2 * i) * sr + 64 * n + 16 * t));
+}
+template <int D>
+__device__ __forceinline__ void load_v(PageRegs<D>& p, const uint8_t* v, int64_t sr, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    if (D == 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.v[i] = __ldg((const uint4*)(v + (4 * t + i) * sr + 16 * g));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint2 a = __ldg((const uint2*)(v + (4 * t + 2 * i) * sr + 8 * g));
+            const uint2 b = __ldg((const uint2*)(v + (4 * t + 2 * i + 1) * sr + 8 * g));
+            p.v[i] = make_uint4(a.x, a.y, b.x, b.y);
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ void zero_page(PageRegs<D>& p) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) p.k[i][n] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < (D == 128 ? 4 : 2); ++i) p.v[i] = make_uint4(0, 0, 0, 0);
+}
+// Word w (channels 4w .. 4w + 3 of the lane's) of key 4t + i.
+template <int D>
+__device__ __forceinline__ uint32_t v_word(const PageRegs<D>& p, int i, int w) {
+    const uint4& x = D == 128 ? p.v[i] : p.v[i >> 1];
+    const int n = D == 128 ? w : (i & 1) * 2 + w;
+    return n == 0 ? x.x : n == 1 ? x.y : n == 2 ? x.z : x.w;
+}
+// Rows at and beyond `rows` hold whatever the memory held: zero, so that P = 0 leaves no trace of them.
+template <int D>
+__device__ __forceinline__ void mask_v(PageRegs<D>& p, int rows, int lane) {
+    const int t = lane & 3;
+    if (D == 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * t + i >= rows) p.v[i] = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (4 * t + 2 * i >= rows) p.v[i].x = p.v[i].y = 0;
+            if (4 * t + 2 * i + 1 >= rows) p.v[i].z = p.v[i].w = 0;
+        }
+    }
+}
+
 struct PrefillArgs {
     PagedCache c;
     const uint16_t* q;
