@@ -1,81 +1,27 @@
 // Prefill attention over the block-scaled paged cache: the tokens of a step, packed sequence by sequence, against their
 // sequence's cached rows.  Token i of a sequence with n tokens in the step and kv rows in the cache sees rows
 // 0 .. kv - n + i; a token that sees no row gets zeros and a log-sum-exp of -inf.
+//
+// A CTA takes two tiles of 128 rows ((token, q head) pairs of one KV head, the heads of a token together) and walks the
+// sequence's rows in tiles of 128 keys:
+//   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: scores out of tensor memory, weights P back into it as f16
+//   warps 8-11       convert the keys' K and V codes to f16 (exact) in shared memory, two stages of each
+//   warp 12          one thread issues the tensor-core products S = Q K^T and O += P V (tcgen05, accumulators in tensor
+//                    memory: 128 columns of S and D of O per tile, P over S), whichever tile is ready first, so that one
+//                    tile's products run under the other's softmax
+// Two tiles per CTA halve the conversions and keep the operand reads at what shared memory delivers.  Every wait is
+// bounded; when one runs out the CTA raises FDMS_DEV_WAIT_TIMEOUT, gives its tensor memory back and returns.
 #include "paged_attn.cuh"
 
 namespace fdms {
 
-constexpr int kPreWarps = 4;
-constexpr int kPreRows = kPreWarps * 16;        // (token, q head) rows of a CTA, heads of a token together
-
-// One 16-row page as matrix operands.  Lane (g, t) = (lane / 4, lane % 4).
-//   Scores: B holds K^T.  Column c of the two 8-column tiles is key 4 (c / 2) + c % 2 and the same + 2, so that a lane's
-//   four scores are keys 4t .. 4t + 3, which is what the second product wants from it.  The k index is permuted: in chunk
-//   n (64 bytes of a row) lane t brings bytes 64 n + 16 t + [0, 16), four of them for each of four steps; a query fragment
-//   is loaded in the same order.
-//   Output: A holds P, its k index the keys in the order above; B holds V, column g of tile j being channel (D / 8) g + j,
-//   so that a lane loads D / 8 consecutive bytes of keys 4t .. 4t + 3 and ends up with consecutive channels.
-template <int D>
-struct PageRegs {
-    uint4 k[2][D / 64];         // keys a, a + 2; chunks
-    uint4 v[D == 128 ? 4 : 2];  // keys 4t .. 4t + 3, D / 8 bytes each (D = 64: two keys per vector)
-};
-
-template <int D>
-__device__ __forceinline__ void load_k(PageRegs<D>& p, const uint8_t* k, int64_t sr, int lane) {
-    const int g = lane >> 2, t = lane & 3, key = 4 * (g >> 1) + (g & 1);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int n = 0; n < D / 64; ++n) p.k[i][n] = __ldg((const uint4*)(k + (key + 2 * i) * sr + 64 * n + 16 * t));
-}
-template <int D>
-__device__ __forceinline__ void load_v(PageRegs<D>& p, const uint8_t* v, int64_t sr, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    if (D == 128) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p.v[i] = __ldg((const uint4*)(v + (4 * t + i) * sr + 16 * g));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint2 a = __ldg((const uint2*)(v + (4 * t + 2 * i) * sr + 8 * g));
-            const uint2 b = __ldg((const uint2*)(v + (4 * t + 2 * i + 1) * sr + 8 * g));
-            p.v[i] = make_uint4(a.x, a.y, b.x, b.y);
-        }
-    }
-}
-template <int D>
-__device__ __forceinline__ void zero_page(PageRegs<D>& p) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int n = 0; n < D / 64; ++n) p.k[i][n] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < (D == 128 ? 4 : 2); ++i) p.v[i] = make_uint4(0, 0, 0, 0);
-}
-// Word w (channels 4w .. 4w + 3 of the lane's) of key 4t + i.
-template <int D>
-__device__ __forceinline__ uint32_t v_word(const PageRegs<D>& p, int i, int w) {
-    const uint4& x = D == 128 ? p.v[i] : p.v[i >> 1];
-    const int n = D == 128 ? w : (i & 1) * 2 + w;
-    return n == 0 ? x.x : n == 1 ? x.y : n == 2 ? x.z : x.w;
-}
-// Rows at and beyond `rows` hold whatever the memory held: zero, so that P = 0 leaves no trace of them.
-template <int D>
-__device__ __forceinline__ void mask_v(PageRegs<D>& p, int rows, int lane) {
-    const int t = lane & 3;
-    if (D == 128) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (4 * t + i >= rows) p.v[i] = make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (4 * t + 2 * i >= rows) p.v[i].x = p.v[i].y = 0;
-            if (4 * t + 2 * i + 1 >= rows) p.v[i].z = p.v[i].w = 0;
-        }
-    }
-}
+constexpr int kTileRows = 128;                  // query rows per tile, keys per step
+constexpr int kPreThreads = 13 * 32;
+constexpr int kConvWarp = 8, kMmaWarp = 12;
+constexpr int kConstRing = 4;                   // steps whose page constants are held: the softmax may lag two behind
+constexpr int kPreWaitNs = 20000;
+constexpr int kPreWaitLimit = 50000;            // of waits of up to kPreWaitNs: about a second
+constexpr uint32_t kTmemCols = 512;
 
 struct PrefillArgs {
     PagedCache c;
@@ -121,185 +67,481 @@ __device__ __forceinline__ bool find_tile(const PrefillArgs& a, int64_t x, int p
     return false;
 }
 
+// ---- barriers, tensor memory, matrix instructions --------------------------------------------------------------
+__device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_addr(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(s_addr(b)), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded wait; gives up at once when another warp has.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* give_up) {
+    for (int i = 0; i < kPreWaitLimit; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(s_addr(b)), "r"(parity), "r"(kPreWaitNs) : "memory");
+        if (ok) return true;
+        if (*give_up) return false;
+    }
+    *give_up = 1;
+    return false;
+}
+// The same by a warp, with one answer for all of it.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, volatile int* give_up) {
+    return __all_sync(0xffffffffu, bar_wait(b, parity, give_up));
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_addr(b)) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D (tensor memory, f32) (+)= A B: A and B in shared memory, or A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+
+#define FDMS_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define FDMS_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 16 columns of the thread's lane, 32 of them written.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : FDMS_R8(r, 0), FDMS_R8(r, 8) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), FDMS_W8(r, 0), FDMS_W8(r, 8) : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+        "%27,%28,%29,%30,%31,%32};" ::"r"(addr), FDMS_W8(r, 0), FDMS_W8(r, 8), FDMS_W8(r, 16), FDMS_W8(r, 24) : "memory");
+}
+
+// Operands in shared memory lie in slabs of 64 elements (128 bytes) per row, rows one after the other, 16-byte chunks
+// permuted by the row's last three bits (the 128-byte swizzle).  Q and K are read along their rows (K-major), V across
+// them (its channels are the product's columns); both see the same layout.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t leading, uint32_t stride) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// f16 operands, float32 result, 128 rows, n columns; `across`: B is read across its rows.
+__host__ __device__ constexpr uint32_t instruction(int n, bool across) {
+    return 1u << 4 | (across ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kTileRows >> 4) << 24;
+}
+constexpr uint32_t kSlab = kTileRows * 128;     // bytes
+
+template <int D>
+struct PrefillSmem {
+    static constexpr uint32_t kTile = kTileRows * D * 2;        // one operand tile
+    static constexpr uint32_t kQ = 0, kK = 2 * kTile, kV = 4 * kTile, kEnd = 6 * kTile;
+    // 1 KB for the alignment of the tiles; D = 64 asks for more than half of the SM's shared memory all the same, because a
+    // second CTA would wait for tensor memory that the first holds
+    static constexpr uint32_t kBytes = (kEnd + 1024 + 1024) > 120 * 1024 ? kEnd + 2048 : 120 * 1024;
+};
+
+struct PrefillShared {
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    float4 page[kConstRing][kTileRows / kCachePage];            // ks, log2 vs, 1 / vs of the step's pages
+    uint32_t tmem;
+    int give_up, nan_lo, nan_hi;
+};
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kPreWarps * 32) paged_prefill_kernel(PrefillArgs a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int per = kPreRows / a.group;         // tokens per tile
+__global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillArgs a) {
+    extern __shared__ uint8_t dyn[];
+    __shared__ PrefillShared sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = kTileRows / a.group;        // tokens per tile of rows
     int seq;
     int64_t first, begin, count;
     // the last tiles of a sequence see the most rows: they start first
-    if (!find_tile(a, (int64_t)gridDim.x - 1 - blockIdx.x, per, seq, first, begin, count)) return;
+    if (!find_tile(a, (int64_t)gridDim.x - 1 - blockIdx.x, 2 * per, seq, first, begin, count)) return;
     const int head = blockIdx.y;
     const int kv = paged_len(a.c, seq);
-    // this lane's rows
-    int64_t tok[2], last[2];                    // token of the step, last cached row it sees
-    int hq[2];
-    bool live[2];
-    float up[2], factor[2];
-    uint32_t qa[D / 16][4];
+    const int64_t shift = (int64_t)kv - count;  // token j of the sequence's step sees rows 0 .. shift + j
+    const int64_t end = min(first + 2 * per, count);
+    const int tiles = first + per < count ? 2 : 1;
+    const int steps = (int)((max(shift + end, (int64_t)0) + kTileRows - 1) / kTileRows);
+    // keys below `open` are seen by every row of the CTA
+    const int64_t open = max(shift + first + 1, (int64_t)0);
+    uint8_t* tile = (uint8_t*)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
+    using L = PrefillSmem<D>;
+
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&sh.tmem)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (threadIdx.x == 0) {
+        bar_init(&sh.q_full, 8);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&sh.k_full[i], 4);
+            bar_init(&sh.v_full[i], 4);
+            bar_init(&sh.k_empty[i], tiles);
+            bar_init(&sh.v_empty[i], tiles);
+            bar_init(&sh.s_full[i], 1);
+            bar_init(&sh.p_full[i], 4);
+            bar_init(&sh.pv_done[i], 1);
+        }
+        sh.give_up = 0;
+        sh.nan_lo = 0x7fffffff;
+        sh.nan_hi = -1;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;              // S of tile i at 128 i, O at 256 + 128 i
+    volatile int* give_up = &sh.give_up;
+
+    if (warp < kConvWarp) {
+        // ---- softmax: a thread per row ----
+        const int ti = warp >> 2, r = threadIdx.x & 127;
+        const int64_t j = first + ti * per + r / a.group;
+        const bool live = r < per * a.group && j < count;
+        const int hq = head * a.group + (live ? r % a.group : 0);
+        const int64_t tok = begin + (live ? j : first);
+        const int64_t last = live ? shift + j : (int64_t)1 << 40;          // a row that nobody reads is not worth a mask
+        float factor;
+        {
+            const uint16_t* q = a.q + tok * a.q_st + (int64_t)hq * a.q_sh;
+            uint4 w[D / 8];
+            float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = warp * 16 + g + 8 * i;
-        const int64_t j = first + r / a.group;
-        live[i] = r < per * a.group && j < count;
-        tok[i] = begin + (live[i] ? j : first);
-        hq[i] = head * a.group + (live[i] ? r % a.group : 0);
-        last[i] = live[i] ? (int64_t)kv - count + j : -1;
-        const uint16_t* q = a.q + tok[i] * a.q_st + (int64_t)hq[i] * a.q_sh;
-        uint4 w[D / 64][2];
-        float top = 0.0f;
+            for (int i = 0; i < D / 8; ++i) w[i] = live ? *(const uint4*)(q + 8 * i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < D / 64; ++n)
+            for (int i = 0; i < D / 8; ++i) {
+                const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                w[n][k] = *(const uint4*)(q + 64 * n + 16 * t + 8 * k);
-                const uint32_t x[4] = {w[n][k].x, w[n][k].y, w[n][k].z, w[n][k].w};
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
+                for (int k = 0; k < 4; ++k) {
                     float e, f;
-                    unpack_pair<BF16>(x[v], e, f);
+                    unpack_pair<BF16>(x[k], e, f);
                     top = fmaxf(top, fmaxf(fabsf(e), fabsf(f)));
                 }
             }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        row_power(top, up[i], factor[i]);
-        factor[i] *= a.scale * kPagedLog2e;
+            float up;
+            row_power(top, up, factor);
+            factor *= a.scale * kPagedLog2e;
+            uint8_t* dst = tile + L::kQ + ti * L::kTile + r * 128;
 #pragma unroll
-        for (int n = 0; n < D / 64; ++n)
+            for (int i = 0; i < D / 8; ++i) {
+                const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                uint32_t y[4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t x[4] = {w[n][k].x, w[n][k].y, w[n][k].z, w[n][k].w};
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
+                for (int k = 0; k < 4; ++k) {
                     float e, f;
-                    unpack_pair<BF16>(x[v], e, f);
-                    qa[4 * n + 2 * k + (v >> 1)][2 * (v & 1) + i] = f16x2_of(e * up[i], f * up[i]);
+                    unpack_pair<BF16>(x[k], e, f);
+                    y[k] = f16x2_of(e * up, f * up);
                 }
+                *(uint4*)(dst + (i >> 3) * kSlab + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
             }
-    }
-    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-    int64_t most = max(last[0], last[1]);
-    int64_t least = min(live[0] ? last[0] : (int64_t)kv, live[1] ? last[1] : (int64_t)kv);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, s));
-        least = min(least, __shfl_xor_sync(0xffffffffu, least, s));
-    }
-    const int pages = (int)((most + kCachePage) / kCachePage);
-    const int ppb = a.c.shift - 4;
-    for (int p = 0; p < pages; ++p) {
-        const int blk = a.c.tables[seq * a.c.table_stride + (p >> ppb)];
-        if (blk < 0 || blk >= a.c.num_blocks) {
-            if (lane == 0 && a.c.status) atomicOr(a.c.status, FDMS_DEV_BAD_INDEX);
-            continue;
         }
-        const int row = (p & ((1 << ppb) - 1)) * kCachePage;
-        PageRegs<D> pg;
-        const uint8_t* vp = a.c.v + (int64_t)blk * a.c.v_sb + head * a.c.v_sh + row * a.c.v_sr;
-        load_k<D>(pg, a.c.k + (int64_t)blk * a.c.k_sb + head * a.c.k_sh + row * a.c.k_sr, a.c.k_sr, lane);
-        load_v<D>(pg, vp, a.c.v_sr, lane);
-        const float ks = a.c.k_scale[(int64_t)blk * a.c.heads + head], vs = a.c.v_scale[(int64_t)blk * a.c.heads + head];
-        const float lvs = paged_lg2(vs), ivs = __frcp_rn(vs);
-        float s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};       // keys 4t, 4t + 1 and 4t + 2, 4t + 3 of rows g and g + 8
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh.q_full);
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;                  // the warp's 32 lanes of tensor memory
+        const uint32_t s_at = tmem + lanes + 128 * ti, o_at = tmem + lanes + 256 + 128 * ti;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = ti < tiles;
+        for (int step = 0; ok && step < steps; ++step) {
+            ok = warp_wait(&sh.s_full[ti], step & 1, give_up);
+            if (!ok) break;
+            tc_fence_after();
+            const float4* page = sh.page[step & (kConstRing - 1)];
+            const int seen = (int)min(last - (int64_t)step * kTileRows, (int64_t)kTileRows);       // last key of the step that the row sees
+            const bool cut = __any_sync(0xffffffffu, seen < kTileRows - 1);
+            uint32_t p[64];
+            float sum;
+            // weights with the running M, and the largest exponent above it
+            auto weigh = [&](float ref) {
+                float top = -INFINITY;
+                sum = 0.0f;
+                uint32_t s[2][16];              // a page's scores, the next page's on their way
+                tmem_load(s_at, s[0]);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
+                for (int c = 0; c < kTileRows / 16; ++c) {
+                    tc_wait_ld();
+                    if (c + 1 < kTileRows / 16) tmem_load(s_at + 16 * (c + 1), s[(c + 1) & 1]);
+                    const float4 pc = page[c];
+                    const float f = factor * pc.x, b = pc.y - ref;
+                    float x[16], part = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t(&q4)[4] = qa[4 * c + j];
-                uint32_t b0, b1;
-                e4m3x4_f16(j == 0 ? pg.k[0][c].x : j == 1 ? pg.k[0][c].y : j == 2 ? pg.k[0][c].z : pg.k[0][c].w, b0, b1);
-                mma_16816(s0, q4[0], q4[1], q4[2], q4[3], b0, b1);
-                e4m3x4_f16(j == 0 ? pg.k[1][c].x : j == 1 ? pg.k[1][c].y : j == 2 ? pg.k[1][c].z : pg.k[1][c].w, b0, b1);
-                mma_16816(s1, q4[0], q4[1], q4[2], q4[3], b0, b1);
-            }
-        uint32_t pa[4];
-        const int key = p * kCachePage + 4 * t;
+                    for (int i = 0; i < 16; ++i) x[i] = fmaf(__uint_as_float(s[c & 1][i]), f, b);
+                    if (cut) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float s[4] = {s0[2 * i], s0[2 * i + 1], s1[2 * i], s1[2 * i + 1]}, top = -INFINITY;
+                        for (int i = 0; i < 16; ++i)
+                            if (16 * c + i > seen) x[i] = -INFINITY;
+                    }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[j] = key + j <= last[i] ? fmaf(s[j], ks * factor[i], lvs) : -INFINITY;
-                top = fmaxf(top, s[j]);
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (__any_sync(0xffffffffu, top > m[i] + 8.0f)) {
-                const float next = fmaxf(m[i], top);
-                const float r = next == -INFINITY ? 1.0f : paged_ex2(m[i] - next);
-                m[i] = next;
-                l[i] *= r;
+                    for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(x[i], x[i + 1]));
 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) { o[j][2 * i] *= r; o[j][2 * i + 1] *= r; }
-            }
-            const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+                    for (int i = 0; i < 16; ++i) x[i] = paged_ex2(x[i]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] = paged_ex2(s[j] - ref);
-            l[i] = fmaf((s[0] + s[1]) + (s[2] + s[3]), ivs, l[i]);
-            pa[i] = f16x2_of(s[0], s[1]);
-            pa[2 + i] = f16x2_of(s[2], s[3]);
-        }
-        if ((p + 1) * kCachePage > least + 1) {
-            // Some row does not see all of the page.  What it does not see may be anything, a NaN code among it: such
-            // codes count as zero in the product and are put into the rows that do see them.
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < D / 32; ++w) {
-                    const uint32_t x = v_word<D>(pg, i, w) & 0x7f7f7f7fu;
-                    odd = odd || ((x + 0x01010101u) & 0x80808080u) != 0;
+                    for (int i = 0; i < 16; i += 2) {
+                        part += x[i] + x[i + 1];
+                        p[8 * c + (i >> 1)] = f16x2_of(x[i], x[i + 1]);
+                    }
+                    sum = fmaf(part, pc.z, sum);
                 }
-            if (__any_sync(0xffffffffu, odd)) {
+                return top;
+            };
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float top = weigh(ref);
+            if (__any_sync(0xffffffffu, m == -INFINITY ? top > -INFINITY : top > 8.0f)) {
+                // M moves: O and l follow, and the step's weights are taken again.  O is at rest: the scores of a step are
+                // issued only after the products of the step before are complete.
+                const float next = fmaxf(m, top + ref);
+                const float scale = next == -INFINITY ? 1.0f : paged_ex2(m - next);
+                m = next;
+                l *= scale;
+                if (step > 0) {
 #pragma unroll
-                for (int i = 0; i < (D == 128 ? 4 : 2); ++i) {
-                    uint32_t* x = (uint32_t*)&pg.v[i];
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_load(o_at + 16 * c, o);
+                        tc_wait_ld();
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t nan = ((x[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;      // top bit of each NaN byte
-                        x[w] &= ~((nan >> 7) * 0xffu);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
+                        tmem_store(o_at + 16 * c, o);
                     }
                 }
-                for (int k = 0; k < kCachePage; ++k)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (p * kCachePage + k <= last[i])
-#pragma unroll
-                            for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                                for (int n = 0; n < 2; ++n)
-                                    if ((vp[k * a.c.v_sr + (D / 8) * (2 * t + n) + j] & 0x7f) == 0x7f) o[j][2 * i + n] = NAN;
+                weigh(m == -INFINITY ? 0.0f : m);
             }
+            l += sum;
+            {
+                uint32_t half[32];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) half[i] = p[32 * h + i];
+                    tmem_store(s_at + 32 * h, half);
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.p_full[ti]);
         }
+        if (ti < tiles) {
+            if (steps > 0 && ok) ok = warp_wait(&sh.pv_done[ti], (steps - 1) & 1, give_up);
+            tc_fence_after();
+            const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
+            uint16_t* out = a.out + tok * a.o_st + (int64_t)hq * a.o_sh;
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-            const uint32_t k0 = v_word<D>(pg, 0, w), k1 = v_word<D>(pg, 1, w), k2 = v_word<D>(pg, 2, w), k3 = v_word<D>(pg, 3, w);
-            uint32_t b0[4], b1[4];
-            e4m3x4_f16(__byte_perm(k0, k1, 0x5140), b0[0], b0[1]);
-            e4m3x4_f16(__byte_perm(k0, k1, 0x7362), b0[2], b0[3]);
-            e4m3x4_f16(__byte_perm(k2, k3, 0x5140), b1[0], b1[1]);
-            e4m3x4_f16(__byte_perm(k2, k3, 0x7362), b1[2], b1[3]);
+            for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma_16816(o[4 * w + j], pa[0], pa[1], pa[2], pa[3], b0[j], b1[j]);
+                for (int i = 0; i < 16; ++i) o[i] = 0;
+                if (steps > 0) {
+                    tmem_load(o_at + 16 * c, o);
+                    tc_wait_ld();
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            y[k] = pack_pair<BF16>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+                        *(uint4*)(out + 16 * c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+            }
+            if (live && a.lse) a.lse[(int64_t)hq * a.lse_sh + tok * a.lse_st] = kPagedLn2 * (m + paged_lg2(l));
+            // NaN codes of V in steps that not every row sees whole were left out of the products: into the rows that see them
+            const int lo = *(volatile int*)&sh.nan_lo, hi = *(volatile int*)&sh.nan_hi;
+            if (live && lo <= hi)
+                for (int64_t key = (int64_t)lo * kTileRows; key < (int64_t)(hi + 1) * kTileRows && key <= last; ++key) {
+                    const int blk = a.c.tables[seq * a.c.table_stride + (key >> a.c.shift)];
+                    if (blk < 0 || blk >= a.c.num_blocks) continue;
+                    const uint8_t* v = a.c.v + (int64_t)blk * a.c.v_sb + head * a.c.v_sh + (key & ((1 << a.c.shift) - 1)) * a.c.v_sr;
+                    for (int ch = 0; ch < D; ++ch)
+                        if ((v[ch] & 0x7f) == 0x7f) out[ch] = BF16 ? 0x7fff : 0x7fff;
+                }
+        }
+    } else if (warp < kMmaWarp) {
+        // ---- codes to f16 in shared memory ----
+        constexpr int kPer = D / 16;                                        // 16-byte vectors per thread, K and V each
+        constexpr int kRowLanes = D / 16;                                   // threads per row
+        constexpr int kPass = 128 / kRowLanes;                              // rows per pass
+        const int ct = threadIdx.x - kConvWarp * 32, row0 = ct / kRowLanes, piece = ct % kRowLanes;
+        const int32_t* table = a.c.tables + seq * a.c.table_stride;
+        const int pages = (kv + kCachePage - 1) / kCachePage, ppb = a.c.shift - 4, in_block = (1 << a.c.shift) - 1;
+        // block of page `lane` of a step, -1 where there is none
+        auto look_up = [&](int step) {
+            const int p = step * (kTileRows / kCachePage) + lane;
+            int b = -1;
+            if (lane < kTileRows / kCachePage && p < pages) {
+                b = table[p >> ppb];
+                if (b < 0 || b >= a.c.num_blocks) {
+                    b = -1;
+                    if (a.c.status) atomicOr(a.c.status, FDMS_DEV_BAD_INDEX);
+                }
+            }
+            return b;
+        };
+        auto fetch = [&](uint4 (&x)[kPer], const uint8_t* base, int64_t sb, int64_t sr, int step, int blocks, int rows) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int row = i * kPass + row0;
+                const int blk = __shfl_sync(0xffffffffu, blocks, row / kCachePage);
+                x[i] = make_uint4(0, 0, 0, 0);
+                if (blk >= 0 && row < rows)
+                    x[i] = __ldg((const uint4*)(base + blk * sb + ((step * kTileRows + row) & in_block) * sr + 16 * piece));
+            }
+        };
+        auto put = [&](uint32_t at, const uint4 (&x)[kPer]) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int row = i * kPass + row0;
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                uint32_t y[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e4m3x4_f16(w[k], y[2 * k], y[2 * k + 1]);
+                uint8_t* dst = tile + at + (piece >> 2) * kSlab + row * 128;
+                const int c = (piece & 3) * 2, odd = (piece >> 2) & 1;      // the second slab's lanes write their odd chunk first: no bank twice
+                *(uint4*)(dst + (((c + odd) ^ (row & 7)) << 4)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+                *(uint4*)(dst + (((c + 1 - odd) ^ (row & 7)) << 4)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+            }
+        };
+        const uint8_t* kb = a.c.k + head * a.c.k_sh;
+        const uint8_t* vb = a.c.v + head * a.c.v_sh;
+        uint4 xk[kPer], xv[kPer];
+        int blocks = steps > 0 ? look_up(0) : -1;
+        float4 consts = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);           // a page that is left out: every score -inf
+        auto scales = [&]() {
+            consts = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            if (warp == kConvWarp && blocks >= 0) {
+                const float vs = a.c.v_scale[(int64_t)blocks * a.c.heads + head];
+                consts = make_float4(a.c.k_scale[(int64_t)blocks * a.c.heads + head], paged_lg2(vs), __frcp_rn(vs), 0.0f);
+            }
+        };
+        scales();
+        fetch(xk, kb, a.c.k_sb, a.c.k_sr, 0, blocks, kv);
+        fetch(xv, vb, a.c.v_sb, a.c.v_sr, 0, blocks, kv);
+        bool ok = true;
+        for (int step = 0; ok && step < steps; ++step) {
+            const int st = step & 1;
+            const bool more = step + 1 < steps;
+            if (step >= 2) ok = warp_wait(&sh.k_empty[st], ((step >> 1) - 1) & 1, give_up);
+            if (!ok) break;
+            put(L::kK + st * L::kTile, xk);
+            if (warp == kConvWarp && lane < kTileRows / kCachePage) sh.page[step & (kConstRing - 1)][lane] = consts;
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.k_full[st]);
+            blocks = more ? look_up(step + 1) : -1;
+            if (more) {
+                scales();
+                fetch(xk, kb, a.c.k_sb, a.c.k_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+            }
+            if (step >= 2) ok = warp_wait(&sh.v_empty[st], ((step >> 1) - 1) & 1, give_up);
+            if (!ok) break;
+            if ((int64_t)(step + 1) * kTileRows > open) {
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    uint32_t* w = (uint32_t*)&xv[i];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t nan = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;      // top bit of each NaN byte
+                        odd = odd || nan != 0;
+                        w[k] &= ~((nan >> 7) * 0xffu);
+                    }
+                }
+                if (odd) {
+                    atomicMin(&sh.nan_lo, step);
+                    atomicMax(&sh.nan_hi, step);
+                }
+            }
+            put(L::kV + st * L::kTile, xv);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.v_full[st]);
+            if (more) fetch(xv, vb, a.c.v_sb, a.c.v_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+        }
+    } else if (lane == 0 && steps > 0) {
+        // ---- products ----
+        constexpr uint32_t kScores = instruction(kTileRows, false), kValues = instruction(D, true);
+        const uint32_t base = s_addr(tile);
+        auto scores = [&](int ti, int step) {
+            const uint32_t q = base + L::kQ + ti * L::kTile, k = base + L::kK + (step & 1) * L::kTile;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const uint32_t at = (i >> 2) * kSlab + (i & 3) * 32;
+                mma_ss(tmem + 128 * ti, operand(q + at, 16, 1024), operand(k + at, 16, 1024), kScores, i > 0);
+            }
+            tc_commit(&sh.s_full[ti]);
+            tc_commit(&sh.k_empty[step & 1]);
+        };
+        auto values = [&](int ti, int step) {
+            const uint32_t v = base + L::kV + (step & 1) * L::kTile;
+#pragma unroll
+            for (int i = 0; i < kTileRows / 16; ++i)
+                mma_ts(tmem + 256 + 128 * ti, tmem + 128 * ti + 8 * i, operand(v + i * 2048, kSlab, 1024), kValues, step > 0 || i > 0);
+            tc_commit(&sh.pv_done[ti]);
+            tc_commit(&sh.v_empty[step & 1]);
+        };
+        bool ok = bar_wait(&sh.q_full, 0, give_up);
+        // state of each tile: the step it is at, and whether its scores are out (its weights are awaited) or not
+        int at[2] = {0, tiles > 1 ? 0 : steps};
+        bool out[2] = {false, false};
+        int idle = 0;
+        while (ok && (at[0] < steps || at[1] < steps)) {
+            bool did = false;
+#pragma unroll
+            for (int ti = 0; ti < 2; ++ti) {
+                const int step = at[ti];
+                if (step >= steps) continue;
+                if (!out[ti]) {
+                    // the scores go where the weights of the step before were: those must have been read
+                    if ((step == 0 || bar_test(&sh.pv_done[ti], (step - 1) & 1)) && bar_test(&sh.k_full[step & 1], (step >> 1) & 1)) {
+                        tc_fence_after();
+                        scores(ti, step);
+                        out[ti] = true;
+                        did = true;
+                    }
+                } else if (bar_test(&sh.p_full[ti], step & 1) && bar_test(&sh.v_full[step & 1], (step >> 1) & 1)) {
+                    tc_fence_after();
+                    values(ti, step);
+                    out[ti] = false;
+                    at[ti] = step + 1;
+                    did = true;
+                }
+            }
+            if (did) idle = 0;
+            else if (++idle > (1 << 25)) { *give_up = 1; ok = false; }
+            else if ((idle & 1023) == 0 && *give_up) ok = false;
+        }
+        // nothing of this CTA may be in flight when its memory goes
+        if (ok) for (int ti = 0; ti < tiles; ++ti) ok = bar_wait(&sh.pv_done[ti], (steps - 1) & 1, give_up) && ok;
+        else {
+            // after a wait that ran out: let what was issued complete
+            tc_commit(&sh.q_full);
+            for (int i = 0; i < 100 && !bar_test(&sh.q_full, 1); ++i) __nanosleep(10000);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (!live[i]) continue;
-        const float inv = l[i] > 0.0f || l[i] != l[i] ? __frcp_rn(l[i]) : 0.0f;
-        uint16_t* out = a.out + tok[i] * a.o_st + (int64_t)hq[i] * a.o_sh;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int j = 0; j < D / 8; j += 2)
-                *(uint32_t*)(out + (D / 8) * (2 * t + n) + j) = pack_pair<BF16>(o[j][2 * i + n] * inv, o[j + 1][2 * i + n] * inv);
-        if (a.lse && t == 0) a.lse[(int64_t)hq[i] * a.lse_sh + tok[i] * a.lse_st] = kPagedLn2 * (m[i] + paged_lg2(l[i]));
-    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (threadIdx.x == 0 && sh.give_up && a.c.status) atomicOr(a.c.status, FDMS_DEV_WAIT_TIMEOUT);
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
 }  // namespace fdms
@@ -318,18 +560,23 @@ extern "C" int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, voi
     const int group = (int)p.num_q_heads / c.heads;
     PrefillArgs a = {c, (const uint16_t*)p.q, (uint16_t*)p.out, p.lse_out, p.cu_seqlens_q, p.q_stride[0], p.q_stride[1], p.out_stride[0],
                      p.out_stride[1], p.lse_stride[0], p.lse_stride[1], p.tokens, (int32_t)p.num_seqs, group, (float)p.scale};
-    const int64_t tiles = p.tokens / (kPreRows / group) + p.num_seqs;
+    const int64_t tiles = p.tokens / (2 * (kTileRows / group)) + p.num_seqs;
     FDMS_REQUIRE(tiles < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_prefill: too many tokens");
     const dim3 grid((unsigned)tiles, (unsigned)c.heads);
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = p.dtype == FDMS_BF16;
+#define FDMS_PREFILL(DIM, BF)                                                                                                           \
+    do {                                                                                                                                \
+        constexpr int bytes = (int)PrefillSmem<DIM>::kBytes;                                                                            \
+        FDMS_CUDA_OK(cudaFuncSetAttribute(paged_prefill_kernel<DIM, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));           \
+        paged_prefill_kernel<DIM, BF><<<grid, kPreThreads, bytes, st>>>(a);                                                             \
+    } while (0)
     if (p.cache.head_dim == 64) {
-        if (bf) paged_prefill_kernel<64, true><<<grid, kPreWarps * 32, 0, st>>>(a);
-        else paged_prefill_kernel<64, false><<<grid, kPreWarps * 32, 0, st>>>(a);
+        if (bf) FDMS_PREFILL(64, true); else FDMS_PREFILL(64, false);
     } else {
-        if (bf) paged_prefill_kernel<128, true><<<grid, kPreWarps * 32, 0, st>>>(a);
-        else paged_prefill_kernel<128, false><<<grid, kPreWarps * 32, 0, st>>>(a);
+        if (bf) FDMS_PREFILL(128, true); else FDMS_PREFILL(128, false);
     }
+#undef FDMS_PREFILL
     FDMS_CHECK_LAUNCH("paged_prefill_kernel");
     return FDMS_OK;
 }
