@@ -104,7 +104,6 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint64_t* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_addr(b)) : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D (tensor memory, f32) (+)= A B: A and B in shared memory, or A in tensor memory.
@@ -119,7 +118,38 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 
 #define FDMS_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FDMS_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
-// 16 columns of the thread's lane, 32 of them written.
+// Pairs of float32 values in one 64-bit register.
+__device__ __forceinline__ uint64_t pair(float a, float b) { return (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32; }
+__device__ __forceinline__ uint64_t both(float a) { return pair(a, a); }
+__device__ __forceinline__ float low(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 32, 16 or 8 columns of the thread's lane.  What a load brings is there after a wait that names it: the wait takes the
+// registers as operands, so that nothing that uses them moves ahead of it.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+        "%27,%28,%29,%30,%31}, [%32];"
+        : FDMS_R8(r, 0), FDMS_R8(r, 8), FDMS_R8(r, 16), FDMS_R8(r, 24) : "r"(addr) : "memory");
+}
+#define FDMS_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : FDMS_RW8(r, 0), FDMS_RW8(r, 8), FDMS_RW8(r, 16), FDMS_RW8(r, 24) : : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : FDMS_RW8(r, 0), FDMS_RW8(r, 8) : : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[8]) { asm volatile("tcgen05.wait::ld.sync.aligned;" : FDMS_RW8(r, 0) : : "memory"); }
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : FDMS_R8(r, 0), FDMS_R8(r, 8) : "r"(addr) : "memory");
@@ -128,10 +158,36 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(addr), FDMS_W8(r, 0), FDMS_W8(r, 8) : "memory");
 }
-__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
-        "%27,%28,%29,%30,%31,%32};" ::"r"(addr), FDMS_W8(r, 0), FDMS_W8(r, 8), FDMS_W8(r, 16), FDMS_W8(r, 24) : "memory");
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : FDMS_R8(r, 0) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), FDMS_W8(r, 0) : "memory");
+}
+
+// The rare path of the softmax, kept out of its loop: a row of O, or a page of P, times a power of two.
+template <int D>
+__device__ __noinline__ void rescale_o(uint32_t at, float r) {
+    for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        tmem_load(at + 16 * c, o);
+        tc_wait_ld(o);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * r);
+        tmem_store(at + 16 * c, o);
+    }
+}
+__device__ __noinline__ void rescale_p(uint32_t at, float r) {
+    uint32_t p[8];
+    tmem_load(at, p);
+    tc_wait_ld(p);
+    const __half2 h = __float2half2_rn(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __half2 y = __hmul2(*(__half2*)&p[i], h);
+        p[i] = *(const uint32_t*)&y;
+    }
+    tmem_store(at, p);
 }
 
 // Operands in shared memory lie in slabs of 64 elements (128 bytes) per row, rows one after the other, 16-byte chunks
@@ -161,6 +217,35 @@ struct PrefillShared {
     uint32_t tmem;
     int give_up, nan_lo, nan_hi;
 };
+
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Scores of tile ti against the keys of stage st; the weights of tile ti times its values.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, PrefillShared& sh) {
+    using L = PrefillSmem<D>;
+    const uint64_t q = operand(base + L::kQ + ti * L::kTile, 16, 1024), k = operand(base + L::kK + st * L::kTile, 16, 1024);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        const uint32_t step = ((i >> 2) * kSlab + (i & 3) * 32) >> 4;      // addresses are in units of 16 bytes
+        mma_ss(tmem + 128 * ti, q + step, k + step, instruction(kTileRows, false), i > 0);
+    }
+    tc_commit(&sh.s_full[ti]);
+    tc_commit(&sh.k_empty[st]);
+}
+template <int D>
+__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, bool add, PrefillShared& sh) {
+    using L = PrefillSmem<D>;
+    const uint64_t v = operand(base + L::kV + st * L::kTile, kSlab, 1024);
+#pragma unroll
+    for (int i = 0; i < kTileRows / 16; ++i)
+        mma_ts(tmem + 256 + 128 * ti, tmem + 128 * ti + 8 * i, v + (i * 2048 >> 4), instruction(D, true), i > 0 || add);
+    tc_commit(&sh.pv_done[ti]);
+    tc_commit(&sh.v_empty[st]);
+}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillArgs a) {
@@ -220,13 +305,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         float factor;
         {
             const uint16_t* q = a.q + tok * a.q_st + (int64_t)hq * a.q_sh;
-            uint4 w[D / 8];
             float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) w[i] = live ? *(const uint4*)(q + 8 * i) : make_uint4(0, 0, 0, 0);
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < D / 8; ++i) {
-                const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                const uint4 w = live ? *(const uint4*)(q + 8 * i) : make_uint4(0, 0, 0, 0);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float e, f;
@@ -238,9 +321,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             row_power(top, up, factor);
             factor *= a.scale * kPagedLog2e;
             uint8_t* dst = tile + L::kQ + ti * L::kTile + r * 128;
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < D / 8; ++i) {
-                const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                const uint4 w = live ? *(const uint4*)(q + 8 * i) : make_uint4(0, 0, 0, 0);
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
                 uint32_t y[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -265,72 +349,71 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             const float4* page = sh.page[step & (kConstRing - 1)];
             const int seen = (int)min(last - (int64_t)step * kTileRows, (int64_t)kTileRows);       // last key of the step that the row sees
             const bool cut = __any_sync(0xffffffffu, seen < kTileRows - 1);
-            uint32_t p[64];
-            float sum;
-            // weights with the running M, and the largest exponent above it
-            auto weigh = [&](float ref) {
-                float top = -INFINITY;
-                sum = 0.0f;
-                uint32_t s[2][16];              // a page's scores, the next page's on their way
-                tmem_load(s_at, s[0]);
+            // Page by page: P takes the columns of scores that have been read.  M is a whole number, so that when it has to
+            // move, O, l and the step's earlier weights follow by an exact factor.
+            uint32_t sc[2][32];                 // two pages' scores, the next two pages' on their way
+            tmem_load(s_at, sc[0]);
 #pragma unroll
-                for (int c = 0; c < kTileRows / 16; ++c) {
-                    tc_wait_ld();
-                    if (c + 1 < kTileRows / 16) tmem_load(s_at + 16 * (c + 1), s[(c + 1) & 1]);
-                    const float4 pc = page[c];
-                    const float f = factor * pc.x, b = pc.y - ref;
-                    float x[16], part = 0.0f;
+            for (int c = 0; c < kTileRows / 32; ++c) {
+                tc_wait_ld(sc[c & 1]);
+                if (c + 1 < kTileRows / 32) tmem_load(s_at + 32 * (c + 1), sc[(c + 1) & 1]);
+                const float4 p0 = page[2 * c], p1 = page[2 * c + 1];
+                const float ref = m == -INFINITY ? 0.0f : m;
+                uint64_t x[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = fmaf(__uint_as_float(s[c & 1][i]), f, b);
-                    if (cut) {
+                for (int i = 0; i < 16; ++i) x[i] = (uint64_t)sc[c & 1][2 * i] | (uint64_t)sc[c & 1][2 * i + 1] << 32;
+                {
+                    const uint64_t f0 = both(factor * p0.x), b0 = both(p0.y - ref), f1 = both(factor * p1.x), b1 = both(p1.y - ref);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (16 * c + i > seen) x[i] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(x[i], x[i + 1]));
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = paged_ex2(x[i]);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        part += x[i] + x[i + 1];
-                        p[8 * c + (i >> 1)] = f16x2_of(x[i], x[i + 1]);
-                    }
-                    sum = fmaf(part, pc.z, sum);
-                }
-                return top;
-            };
-            const float ref = m == -INFINITY ? 0.0f : m;
-            float top = weigh(ref);
-            if (__any_sync(0xffffffffu, m == -INFINITY ? top > -INFINITY : top > 8.0f)) {
-                // M moves: O and l follow, and the step's weights are taken again.  O is at rest: the scores of a step are
-                // issued only after the products of the step before are complete.
-                const float next = fmaxf(m, top + ref);
-                const float scale = next == -INFINITY ? 1.0f : paged_ex2(m - next);
-                m = next;
-                l *= scale;
-                if (step > 0) {
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16];
-                        tmem_load(o_at + 16 * c, o);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
-                        tmem_store(o_at + 16 * c, o);
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = fma2(x[i], f0, b0);
+                        x[8 + i] = fma2(x[8 + i], f1, b1);
                     }
                 }
-                weigh(m == -INFINITY ? 0.0f : m);
-            }
-            l += sum;
-            {
-                uint32_t half[32];
+                if (cut) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) half[i] = p[32 * h + i];
-                    tmem_store(s_at + 32 * h, half);
+                    for (int i = 0; i < 16; ++i)
+                        x[i] = pair(32 * c + 2 * i > seen ? -INFINITY : low(x[i]), 32 * c + 2 * i + 1 > seen ? -INFINITY : high(x[i]));
                 }
+                float t[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    t[i] = fmaxf(low(x[4 * i]), high(x[4 * i]));
+#pragma unroll
+                    for (int k = 1; k < 4; ++k) t[i] = fmaxf(t[i], fmaxf(low(x[4 * i + k]), high(x[4 * i + k])));
+                }
+                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                if (__any_sync(0xffffffffu, m == -INFINITY ? top > -INFINITY : top > 8.0f)) {
+                    if (c + 1 < kTileRows / 32) tc_wait_ld(sc[(c + 1) & 1]);
+                    const float next = fmaxf(m, ceilf(top + ref));
+                    const float r = next == -INFINITY ? 1.0f : paged_ex2(m - next);
+                    const uint64_t down = both(next == -INFINITY ? 0.0f : ref - next);
+                    m = next;
+                    l *= r;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = add2(x[i], down);
+                    // O is at rest: the scores of a step are issued only after the products of the step before are complete
+                    if (step > 0) rescale_o<D>(o_at, r);
+                    tc_wait_st();
+                    for (int e = 0; e < 2 * c; ++e) rescale_p(s_at + 8 * e, r);
+                }
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = paged_ex2(low(x[i])), f = paged_ex2(high(x[i]));
+                    x[i] = pair(e, f);
+                    p[i] = f16x2_of(e, f);
+                }
+                tmem_store(s_at + 16 * c, p);
+#pragma unroll
+                for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+                    for (int i = 0; i < n; ++i) {
+                        x[i] = add2(x[i], x[i + n]);
+                        x[8 + i] = add2(x[8 + i], x[8 + i + n]);
+                    }
+                l = fmaf(low(x[0]) + high(x[0]), p0.z, l);
+                l = fmaf(low(x[8]) + high(x[8]), p1.z, l);
             }
             tc_wait_st();
             tc_fence_before();
@@ -349,7 +432,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                 for (int i = 0; i < 16; ++i) o[i] = 0;
                 if (steps > 0) {
                     tmem_load(o_at + 16 * c, o);
-                    tc_wait_ld();
+                    tc_wait_ld(o);
                 }
                 if (live) {
 #pragma unroll
@@ -475,30 +558,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (lane == 0) bar_arrive(&sh.v_full[st]);
             if (more) fetch(xv, vb, a.c.v_sb, a.c.v_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
         }
-    } else if (lane == 0 && steps > 0) {
-        // ---- products ----
-        constexpr uint32_t kScores = instruction(kTileRows, false), kValues = instruction(D, true);
-        const uint32_t base = s_addr(tile);
-        auto scores = [&](int ti, int step) {
-            const uint32_t q = base + L::kQ + ti * L::kTile, k = base + L::kK + (step & 1) * L::kTile;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                const uint32_t at = (i >> 2) * kSlab + (i & 3) * 32;
-                mma_ss(tmem + 128 * ti, operand(q + at, 16, 1024), operand(k + at, 16, 1024), kScores, i > 0);
-            }
-            tc_commit(&sh.s_full[ti]);
-            tc_commit(&sh.k_empty[step & 1]);
-        };
-        auto values = [&](int ti, int step) {
-            const uint32_t v = base + L::kV + (step & 1) * L::kTile;
-#pragma unroll
-            for (int i = 0; i < kTileRows / 16; ++i)
-                mma_ts(tmem + 256 + 128 * ti, tmem + 128 * ti + 8 * i, operand(v + i * 2048, kSlab, 1024), kValues, step > 0 || i > 0);
-            tc_commit(&sh.pv_done[ti]);
-            tc_commit(&sh.v_empty[step & 1]);
-        };
-        bool ok = bar_wait(&sh.q_full, 0, give_up);
-        // state of each tile: the step it is at, and whether its scores are out (its weights are awaited) or not
+    } else if (steps > 0) {
+        // ---- products ----  The whole warp runs this, one elected thread issues: what the instructions take is then the same
+        // for all lanes and stays in uniform registers.
+        const uint32_t base = s_addr(tile), t0 = __shfl_sync(0xffffffffu, tmem, 0);
+        bool ok = warp_wait(&sh.q_full, 0, give_up);
+        // of each tile: the step it is at, and whether its scores are out (its weights are awaited) or not
         int at[2] = {0, tiles > 1 ? 0 : steps};
         bool out[2] = {false, false};
         int idle = 0;
@@ -511,14 +576,21 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                 if (!out[ti]) {
                     // the scores go where the weights of the step before were: those must have been read
                     if ((step == 0 || bar_test(&sh.pv_done[ti], (step - 1) & 1)) && bar_test(&sh.k_full[step & 1], (step >> 1) & 1)) {
+                        __syncwarp();
                         tc_fence_after();
-                        scores(ti, step);
-                        out[ti] = true;
-                        did = true;
+                        if (elected()) {
+                            if (step & 1) issue_scores<D>(base, t0, ti, 1, sh); else issue_scores<D>(base, t0, ti, 0, sh);
+                        }
+                        __syncwarp();
+                        out[ti] = did = true;
                     }
                 } else if (bar_test(&sh.p_full[ti], step & 1) && bar_test(&sh.v_full[step & 1], (step >> 1) & 1)) {
+                    __syncwarp();
                     tc_fence_after();
-                    values(ti, step);
+                    if (elected()) {
+                        if (step & 1) issue_values<D>(base, t0, ti, 1, true, sh); else issue_values<D>(base, t0, ti, 0, step > 0, sh);
+                    }
+                    __syncwarp();
                     out[ti] = false;
                     at[ti] = step + 1;
                     did = true;
@@ -527,12 +599,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (did) idle = 0;
             else if (++idle > (1 << 25)) { *give_up = 1; ok = false; }
             else if ((idle & 1023) == 0 && *give_up) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
         }
         // nothing of this CTA may be in flight when its memory goes
-        if (ok) for (int ti = 0; ti < tiles; ++ti) ok = bar_wait(&sh.pv_done[ti], (steps - 1) & 1, give_up) && ok;
-        else {
-            // after a wait that ran out: let what was issued complete
-            tc_commit(&sh.q_full);
+        if (ok) {
+            for (int ti = 0; ti < tiles; ++ti) warp_wait(&sh.pv_done[ti], (steps - 1) & 1, give_up);
+        } else {                                // after a wait that ran out: let what was issued complete
+            if (elected()) tc_commit(&sh.q_full);
             for (int i = 0; i < 100 && !bar_test(&sh.q_full, 1); ++i) __nanosleep(10000);
         }
     }
