@@ -176,8 +176,8 @@ __device__ __forceinline__ void page_weights(UnitState<D>& u, float (&s)[4], flo
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-            const float next = fmaxf(u.m[i], top[i]);
-            const float r = next == -INFINITY ? 1.0f : paged_ex2(u.m[i] - next);
+            const float next = top[i] > u.m[i] + 8.0f ? top[i] : u.m[i];      // heads do not follow their neighbours
+            const float r = next == u.m[i] ? 1.0f : paged_ex2(u.m[i] - next);
             u.m[i] = next;
             u.l[i] *= r;
 #pragma unroll

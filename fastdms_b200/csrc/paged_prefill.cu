@@ -6,17 +6,21 @@
 // sequence's rows in tiles of 128 keys:
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: scores out of tensor memory, weights P back into it as f16
 //   warps 8-11       convert the keys' K and V codes to f16 (exact) in shared memory, two stages of each
-//   warp 12          one thread issues the tensor-core products S = Q K^T and O += P V (tcgen05, accumulators in tensor
-//                    memory: 128 columns of S and D of O per tile, P over S), whichever tile is ready first, so that one
-//                    tile's products run under the other's softmax
-// Two tiles per CTA halve the conversions and keep the operand reads at what shared memory delivers.  Every wait is
-// bounded; when one runs out the CTA raises FDMS_DEV_WAIT_TIMEOUT, gives its tensor memory back and returns.
+//   warps 12, 13     issue a tile's tensor-core products S = Q K^T and O += P V (tcgen05, accumulators in tensor memory),
+//                    whichever is ready first.  One warp for both tiles spent more on looking and issuing (800 cycles for
+//                    each of the eight batches of 128 keys) than the products take
+// Tensor memory holds O of both tiles (2 x D columns) and two buffers of S for each, 64 keys wide, P over the S it comes
+// from: the scores of 64 keys are computed while the 64 before them are weighed, so that the softmax, which bounds this
+// kernel (one exponential per score: 16 a cycle and SM), does not wait for the products.  Two tiles per CTA halve the
+// conversions.  Every wait is bounded; when one runs out the CTA raises FDMS_DEV_WAIT_TIMEOUT, gives its tensor memory back
+// and returns.
 #include "paged_attn.cuh"
 
 namespace fdms {
 
 constexpr int kTileRows = 128;                  // query rows per tile, keys per step
-constexpr int kPreThreads = 13 * 32;
+constexpr int kHalf = kTileRows / 2;            // keys per buffer of scores
+constexpr int kPreThreads = 14 * 32;
 constexpr int kConvWarp = 8, kMmaWarp = 12;
 constexpr int kConstRing = 4;                   // steps whose page constants are held: the softmax may lag two behind
 constexpr int kPreWaitNs = 20000;
@@ -165,6 +169,50 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[8]
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), FDMS_W8(r, 0) : "memory");
 }
 
+constexpr float kMostWeight = 16384.0f;         // a sum of weights below this keeps each inside f16
+
+// Exponents of 32 scores: x = s * factor * ks + log2 vs - ref, keys behind `seen` masked.
+__device__ __forceinline__ void exponents(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, float ref, bool cut, int seen,
+                                          uint64_t (&x)[16]) {
+    const uint64_t f0 = both(factor * p0.x), b0 = both(p0.y - ref), f1 = both(factor * p1.x), b1 = both(p1.y - ref);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        x[i] = fma2((uint64_t)s[2 * i] | (uint64_t)s[2 * i + 1] << 32, i < 8 ? f0 : f1, i < 8 ? b0 : b1);
+    if (cut) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = pair(2 * i > seen ? -INFINITY : low(x[i]), 2 * i + 1 > seen ? -INFINITY : high(x[i]));
+    }
+}
+// Weights of 32 scores as f16 and their sums over each of the two pages.
+__device__ __forceinline__ void weigh(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, float m, bool cut, int seen,
+                                      uint32_t (&p)[16], float& sum0, float& sum1) {
+    uint64_t x[16];
+    exponents(s, factor, p0, p1, m == -INFINITY ? 0.0f : m, cut, seen, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float e = paged_ex2(low(x[i])), f = paged_ex2(high(x[i]));
+        x[i] = pair(e, f);
+        p[i] = f16x2_of(e, f);
+    }
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            x[i] = add2(x[i], x[i + n]);
+            x[8 + i] = add2(x[8 + i], x[8 + i + n]);
+        }
+    sum0 = low(x[0]) + high(x[0]);
+    sum1 = low(x[8]) + high(x[8]);
+}
+__device__ __forceinline__ float largest(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, bool cut, int seen) {
+    uint64_t x[16];
+    exponents(s, factor, p0, p1, 0.0f, cut, seen, x);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(low(x[i]), high(x[i])));
+    return top;
+}
+
 // The rare path of the softmax, kept out of its loop: a row of O, or a page of P, times a power of two.
 template <int D>
 __device__ __noinline__ void rescale_o(uint32_t at, float r) {
@@ -212,7 +260,7 @@ struct PrefillSmem {
 };
 
 struct PrefillShared {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2];
     float4 page[kConstRing][kTileRows / kCachePage];            // ks, log2 vs, 1 / vs of the step's pages
     uint32_t tmem;
     int give_up, nan_lo, nan_hi;
@@ -223,27 +271,27 @@ __device__ __forceinline__ bool elected() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// Scores of tile ti against the keys of stage st; the weights of tile ti times its values.
+// Scores of tile ti against the half h of the keys in stage st; the weights of tile ti times the values of that half.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, PrefillShared& sh) {
+__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, int h, PrefillShared& sh) {
     using L = PrefillSmem<D>;
-    const uint64_t q = operand(base + L::kQ + ti * L::kTile, 16, 1024), k = operand(base + L::kK + st * L::kTile, 16, 1024);
+    const uint64_t q = operand(base + L::kQ + ti * L::kTile, 16, 1024), k = operand(base + L::kK + st * L::kTile + h * (kHalf * 128), 16, 1024);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
         const uint32_t step = ((i >> 2) * kSlab + (i & 3) * 32) >> 4;      // addresses are in units of 16 bytes
-        mma_ss(tmem + 128 * ti, q + step, k + step, instruction(kTileRows, false), i > 0);
+        mma_ss(tmem + 128 * ti + kHalf * h, q + step, k + step, instruction(kHalf, false), i > 0);
     }
-    tc_commit(&sh.s_full[ti]);
+    tc_commit(&sh.s_full[ti][h]);
     tc_commit(&sh.k_empty[st]);
 }
 template <int D>
-__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, bool add, PrefillShared& sh) {
+__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, int h, bool add, PrefillShared& sh) {
     using L = PrefillSmem<D>;
-    const uint64_t v = operand(base + L::kV + st * L::kTile, kSlab, 1024);
+    const uint64_t v = operand(base + L::kV + st * L::kTile + h * (kHalf * 128), kSlab, 1024);
 #pragma unroll
-    for (int i = 0; i < kTileRows / 16; ++i)
-        mma_ts(tmem + 256 + 128 * ti, tmem + 128 * ti + 8 * i, v + (i * 2048 >> 4), instruction(D, true), i > 0 || add);
-    tc_commit(&sh.pv_done[ti]);
+    for (int i = 0; i < kHalf / 16; ++i)
+        mma_ts(tmem + 256 + 128 * ti, tmem + 128 * ti + kHalf * h + 8 * i, v + (i * 2048 >> 4), instruction(D, true), i > 0 || add);
+    tc_commit(&sh.pv_done[ti][h]);
     tc_commit(&sh.v_empty[st]);
 }
 
@@ -263,6 +311,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     const int64_t end = min(first + 2 * per, count);
     const int tiles = first + per < count ? 2 : 1;
     const int steps = (int)((max(shift + end, (int64_t)0) + kTileRows - 1) / kTileRows);
+    const int halves = (int)((max(shift + end, (int64_t)0) + kHalf - 1) / kHalf);
     // keys below `open` are seen by every row of the CTA
     const int64_t open = max(shift + first + 1, (int64_t)0);
     uint8_t* tile = (uint8_t*)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
@@ -277,11 +326,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         for (int i = 0; i < 2; ++i) {
             bar_init(&sh.k_full[i], 4);
             bar_init(&sh.v_full[i], 4);
-            bar_init(&sh.k_empty[i], tiles);
-            bar_init(&sh.v_empty[i], tiles);
-            bar_init(&sh.s_full[i], 1);
-            bar_init(&sh.p_full[i], 4);
-            bar_init(&sh.pv_done[i], 1);
+            bar_init(&sh.k_empty[i], 2 * tiles);
+            bar_init(&sh.v_empty[i], 2 * tiles);
+            for (int k = 0; k < 2; ++k) {
+                bar_init(&sh.s_full[i][k], 1);
+                bar_init(&sh.p_full[i][k], 4);
+                bar_init(&sh.pv_done[i][k], 1);
+            }
         }
         sh.give_up = 0;
         sh.nan_lo = 0x7fffffff;
@@ -291,7 +342,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;              // S of tile i at 128 i, O at 256 + 128 i
+    const uint32_t tmem = sh.tmem;              // S of tile i at 128 i and 128 i + 64, O at 256 + 128 i
     volatile int* give_up = &sh.give_up;
 
     if (warp < kConvWarp) {
@@ -339,89 +390,60 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         __syncwarp();
         if (lane == 0) bar_arrive(&sh.q_full);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                  // the warp's 32 lanes of tensor memory
-        const uint32_t s_at = tmem + lanes + 128 * ti, o_at = tmem + lanes + 256 + 128 * ti;
+        const uint32_t o_at = tmem + lanes + 256 + 128 * ti;
         float m = -INFINITY, l = 0.0f;
         bool ok = ti < tiles;
-        for (int step = 0; ok && step < steps; ++step) {
-            ok = warp_wait(&sh.s_full[ti], step & 1, give_up);
+        for (int half = 0; ok && half < halves; ++half) {
+            ok = warp_wait(&sh.s_full[ti][half & 1], (half >> 1) & 1, give_up);
             if (!ok) break;
             tc_fence_after();
-            const float4* page = sh.page[step & (kConstRing - 1)];
-            const int seen = (int)min(last - (int64_t)step * kTileRows, (int64_t)kTileRows);       // last key of the step that the row sees
-            const bool cut = __any_sync(0xffffffffu, seen < kTileRows - 1);
-            // Page by page: P takes the columns of scores that have been read.  M is a whole number, so that when it has to
-            // move, O, l and the step's earlier weights follow by an exact factor.
-            uint32_t sc[2][32];                 // two pages' scores, the next two pages' on their way
+            const uint32_t s_at = tmem + lanes + 128 * ti + kHalf * (half & 1);
+            const float4* page = &sh.page[(half >> 1) & (kConstRing - 1)][(half & 1) * (kHalf / kCachePage)];
+            const int seen = (int)min(last - (int64_t)half * kHalf, (int64_t)kHalf);         // last key of the half that the row sees
+            const bool cut = __any_sync(0xffffffffu, seen < kHalf - 1);
+            // 32 keys at a time.  P takes the columns of scores that have been read.  M follows the maximum only when a
+            // weight might leave f16 (the sum of 32 tells) and is a whole number: O, l and the earlier weights of the half then
+            // follow by an exact factor.  Most keys need no maximum at all.
+            uint32_t sc[2][32];
             tmem_load(s_at, sc[0]);
+            tmem_load(s_at + 32, sc[1]);
 #pragma unroll
-            for (int c = 0; c < kTileRows / 32; ++c) {
-                tc_wait_ld(sc[c & 1]);
-                if (c + 1 < kTileRows / 32) tmem_load(s_at + 32 * (c + 1), sc[(c + 1) & 1]);
+            for (int c = 0; c < 2; ++c) {
+                tc_wait_ld(sc[c]);
                 const float4 p0 = page[2 * c], p1 = page[2 * c + 1];
-                const float ref = m == -INFINITY ? 0.0f : m;
-                uint64_t x[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = (uint64_t)sc[c & 1][2 * i] | (uint64_t)sc[c & 1][2 * i + 1] << 32;
-                {
-                    const uint64_t f0 = both(factor * p0.x), b0 = both(p0.y - ref), f1 = both(factor * p1.x), b1 = both(p1.y - ref);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[i] = fma2(x[i], f0, b0);
-                        x[8 + i] = fma2(x[8 + i], f1, b1);
-                    }
-                }
-                if (cut) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[i] = pair(32 * c + 2 * i > seen ? -INFINITY : low(x[i]), 32 * c + 2 * i + 1 > seen ? -INFINITY : high(x[i]));
-                }
-                float t[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    t[i] = fmaxf(low(x[4 * i]), high(x[4 * i]));
-#pragma unroll
-                    for (int k = 1; k < 4; ++k) t[i] = fmaxf(t[i], fmaxf(low(x[4 * i + k]), high(x[4 * i + k])));
-                }
-                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-                if (__any_sync(0xffffffffu, m == -INFINITY ? top > -INFINITY : top > 8.0f)) {
-                    if (c + 1 < kTileRows / 32) tc_wait_ld(sc[(c + 1) & 1]);
-                    const float next = fmaxf(m, ceilf(top + ref));
-                    const float r = next == -INFINITY ? 1.0f : paged_ex2(m - next);
-                    const uint64_t down = both(next == -INFINITY ? 0.0f : ref - next);
+                uint32_t p[16];
+                float sum0, sum1;
+                weigh(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, sum0, sum1);
+                const bool moves = m == -INFINITY || sum0 + sum1 > kMostWeight;         // rows do not follow their neighbours
+                if (__any_sync(0xffffffffu, moves)) {
+                    if (c == 0) tc_wait_ld(sc[1]);
+                    tmem_load(s_at + 32 * c, sc[c]);
+                    tc_wait_ld(sc[c]);
+                    const float top = largest(sc[c], factor, p0, p1, cut, seen - 32 * c);
+                    const float next = moves ? fmaxf(m, ceilf(top)) : m;
+                    const float r = next == m ? 1.0f : paged_ex2(m - next);
                     m = next;
                     l *= r;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = add2(x[i], down);
-                    // O is at rest: the scores of a step are issued only after the products of the step before are complete
-                    if (step > 0) rescale_o<D>(o_at, r);
+                    if (half > 0) {             // the products of the half before must be complete before O is touched
+                        ok = warp_wait(&sh.pv_done[ti][(half - 1) & 1], ((half - 1) >> 1) & 1, give_up);
+                        tc_fence_after();
+                        rescale_o<D>(o_at, r);
+                    }
                     tc_wait_st();
                     for (int e = 0; e < 2 * c; ++e) rescale_p(s_at + 8 * e, r);
-                }
-                uint32_t p[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = paged_ex2(low(x[i])), f = paged_ex2(high(x[i]));
-                    x[i] = pair(e, f);
-                    p[i] = f16x2_of(e, f);
+                    weigh(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, sum0, sum1);
                 }
                 tmem_store(s_at + 16 * c, p);
-#pragma unroll
-                for (int n = 4; n > 0; n >>= 1)
-#pragma unroll
-                    for (int i = 0; i < n; ++i) {
-                        x[i] = add2(x[i], x[i + n]);
-                        x[8 + i] = add2(x[8 + i], x[8 + i + n]);
-                    }
-                l = fmaf(low(x[0]) + high(x[0]), p0.z, l);
-                l = fmaf(low(x[8]) + high(x[8]), p1.z, l);
+                l = fmaf(sum0, p0.z, l);
+                l = fmaf(sum1, p1.z, l);
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(&sh.p_full[ti]);
+            if (lane == 0) bar_arrive(&sh.p_full[ti][half & 1]);
         }
         if (ti < tiles) {
-            if (steps > 0 && ok) ok = warp_wait(&sh.pv_done[ti], (steps - 1) & 1, give_up);
+            if (halves > 0 && ok) ok = warp_wait(&sh.pv_done[ti][(halves - 1) & 1], ((halves - 1) >> 1) & 1, give_up);
             tc_fence_after();
             const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
             uint16_t* out = a.out + tok * a.o_st + (int64_t)hq * a.o_sh;
@@ -430,7 +452,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                 uint32_t o[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[i] = 0;
-                if (steps > 0) {
+                if (halves > 0) {
                     tmem_load(o_at + 16 * c, o);
                     tc_wait_ld(o);
                 }
@@ -478,14 +500,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             }
             return b;
         };
-        auto fetch = [&](uint4 (&x)[kPer], const uint8_t* base, int64_t sb, int64_t sr, int step, int blocks, int rows) {
+        auto fetch = [&](uint4 (&x)[kPer], const uint8_t* base, uint32_t sb, uint32_t sr, int step, int blocks, int rows) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int row = i * kPass + row0;
                 const int blk = __shfl_sync(0xffffffffu, blocks, row / kCachePage);
                 x[i] = make_uint4(0, 0, 0, 0);
                 if (blk >= 0 && row < rows)
-                    x[i] = __ldg((const uint4*)(base + blk * sb + ((step * kTileRows + row) & in_block) * sr + 16 * piece));
+                    x[i] = __ldg((const uint4*)(base + (uint64_t)(uint32_t)blk * sb + (uint32_t)((step * kTileRows + row) & in_block) * sr));
             }
         };
         auto put = [&](uint32_t at, const uint4 (&x)[kPer]) {
@@ -502,21 +524,24 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                 *(uint4*)(dst + (((c + 1 - odd) ^ (row & 7)) << 4)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
             }
         };
-        const uint8_t* kb = a.c.k + head * a.c.k_sh;
-        const uint8_t* vb = a.c.v + head * a.c.v_sh;
+        const uint8_t* kb = a.c.k + head * a.c.k_sh + 16 * piece;
+        const uint8_t* vb = a.c.v + head * a.c.v_sh + 16 * piece;
+        const uint32_t k_sb = (uint32_t)a.c.k_sb, k_sr = (uint32_t)a.c.k_sr, v_sb = (uint32_t)a.c.v_sb, v_sr = (uint32_t)a.c.v_sr;
+        // one step ahead: the codes and scales of the next step; two ahead: its blocks
         uint4 xk[kPer], xv[kPer];
-        int blocks = steps > 0 ? look_up(0) : -1;
-        float4 consts = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);           // a page that is left out: every score -inf
+        float ks = 0.0f, vs = 0.0f;             // 0: a page that is left out, every score -inf
+        int blocks = look_up(0);
         auto scales = [&]() {
-            consts = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            ks = vs = 0.0f;
             if (warp == kConvWarp && blocks >= 0) {
-                const float vs = a.c.v_scale[(int64_t)blocks * a.c.heads + head];
-                consts = make_float4(a.c.k_scale[(int64_t)blocks * a.c.heads + head], paged_lg2(vs), __frcp_rn(vs), 0.0f);
+                ks = __ldg(a.c.k_scale + (int64_t)blocks * a.c.heads + head);
+                vs = __ldg(a.c.v_scale + (int64_t)blocks * a.c.heads + head);
             }
         };
         scales();
-        fetch(xk, kb, a.c.k_sb, a.c.k_sr, 0, blocks, kv);
-        fetch(xv, vb, a.c.v_sb, a.c.v_sr, 0, blocks, kv);
+        fetch(xk, kb, k_sb, k_sr, 0, blocks, kv);
+        fetch(xv, vb, v_sb, v_sr, 0, blocks, kv);
+        blocks = look_up(1);
         bool ok = true;
         for (int step = 0; ok && step < steps; ++step) {
             const int st = step & 1;
@@ -524,14 +549,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (step >= 2) ok = warp_wait(&sh.k_empty[st], ((step >> 1) - 1) & 1, give_up);
             if (!ok) break;
             put(L::kK + st * L::kTile, xk);
-            if (warp == kConvWarp && lane < kTileRows / kCachePage) sh.page[step & (kConstRing - 1)][lane] = consts;
+            if (warp == kConvWarp && lane < kTileRows / kCachePage)
+                sh.page[step & (kConstRing - 1)][lane] = vs > 0.0f ? make_float4(ks, paged_lg2(vs), __frcp_rn(vs), 0.0f) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.k_full[st]);
-            blocks = more ? look_up(step + 1) : -1;
             if (more) {
                 scales();
-                fetch(xk, kb, a.c.k_sb, a.c.k_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+                fetch(xk, kb, k_sb, k_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
             }
             if (step >= 2) ok = warp_wait(&sh.v_empty[st], ((step >> 1) - 1) & 1, give_up);
             if (!ok) break;
@@ -556,45 +581,42 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             fence_async_shared();
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.v_full[st]);
-            if (more) fetch(xv, vb, a.c.v_sb, a.c.v_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+            if (more) {
+                fetch(xv, vb, v_sb, v_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+                blocks = look_up(step + 2);
+            }
         }
-    } else if (steps > 0) {
-        // ---- products ----  The whole warp runs this, one elected thread issues: what the instructions take is then the same
+    } else if (steps > 0 && warp - kMmaWarp < tiles) {
+        // ---- products of a tile ----  The whole warp runs this, one elected thread issues: what the instructions take is then the same
         // for all lanes and stays in uniform registers.
+        const int ti = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
         const uint32_t base = s_addr(tile), t0 = __shfl_sync(0xffffffffu, tmem, 0);
         bool ok = warp_wait(&sh.q_full, 0, give_up);
-        // of each tile: the step it is at, and whether its scores are out (its weights are awaited) or not
-        int at[2] = {0, tiles > 1 ? 0 : steps};
-        bool out[2] = {false, false};
-        int idle = 0;
-        while (ok && (at[0] < steps || at[1] < steps)) {
+        int a = 0, b = 0, idle = 0;             // halves whose scores, and whose values, have been issued
+        while (ok && b < halves) {
             bool did = false;
-#pragma unroll
-            for (int ti = 0; ti < 2; ++ti) {
-                const int step = at[ti];
-                if (step >= steps) continue;
-                if (!out[ti]) {
-                    // the scores go where the weights of the step before were: those must have been read
-                    if ((step == 0 || bar_test(&sh.pv_done[ti], (step - 1) & 1)) && bar_test(&sh.k_full[step & 1], (step >> 1) & 1)) {
-                        __syncwarp();
-                        tc_fence_after();
-                        if (elected()) {
-                            if (step & 1) issue_scores<D>(base, t0, ti, 1, sh); else issue_scores<D>(base, t0, ti, 0, sh);
-                        }
-                        __syncwarp();
-                        out[ti] = did = true;
-                    }
-                } else if (bar_test(&sh.p_full[ti], step & 1) && bar_test(&sh.v_full[step & 1], (step >> 1) & 1)) {
-                    __syncwarp();
-                    tc_fence_after();
-                    if (elected()) {
-                        if (step & 1) issue_values<D>(base, t0, ti, 1, true, sh); else issue_values<D>(base, t0, ti, 0, step > 0, sh);
-                    }
-                    __syncwarp();
-                    out[ti] = false;
-                    at[ti] = step + 1;
-                    did = true;
+            // scores go where the weights of two halves ago were: those must have been read
+            if (a < halves && (a < 2 || bar_test(&sh.pv_done[ti][a & 1], ((a >> 1) - 1) & 1)) && bar_test(&sh.k_full[(a >> 1) & 1], (a >> 2) & 1)) {
+                __syncwarp();
+                tc_fence_after();
+                if (elected()) {
+                    if (a & 2) { if (a & 1) issue_scores<D>(base, t0, ti, 1, 1, sh); else issue_scores<D>(base, t0, ti, 1, 0, sh); }
+                    else { if (a & 1) issue_scores<D>(base, t0, ti, 0, 1, sh); else issue_scores<D>(base, t0, ti, 0, 0, sh); }
                 }
+                __syncwarp();
+                ++a;
+                did = true;
+            }
+            if (b < a && bar_test(&sh.p_full[ti][b & 1], (b >> 1) & 1) && bar_test(&sh.v_full[(b >> 1) & 1], (b >> 2) & 1)) {
+                __syncwarp();
+                tc_fence_after();
+                if (elected()) {
+                    if (b & 2) { if (b & 1) issue_values<D>(base, t0, ti, 1, 1, true, sh); else issue_values<D>(base, t0, ti, 1, 0, true, sh); }
+                    else { if (b & 1) issue_values<D>(base, t0, ti, 0, 1, true, sh); else issue_values<D>(base, t0, ti, 0, 0, b > 0, sh); }
+                }
+                __syncwarp();
+                ++b;
+                did = true;
             }
             if (did) idle = 0;
             else if (++idle > (1 << 25)) { *give_up = 1; ok = false; }
@@ -603,7 +625,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         }
         // nothing of this CTA may be in flight when its memory goes
         if (ok) {
-            for (int ti = 0; ti < tiles; ++ti) warp_wait(&sh.pv_done[ti], (steps - 1) & 1, give_up);
+            warp_wait(&sh.pv_done[ti][(halves - 1) & 1], ((halves - 1) >> 1) & 1, give_up);
         } else {                                // after a wait that ran out: let what was issued complete
             if (elected()) tc_commit(&sh.q_full);
             for (int i = 0; i < 100 && !bar_test(&sh.q_full, 1); ++i) __nanosleep(10000);
