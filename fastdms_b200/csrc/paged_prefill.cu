@@ -7,8 +7,8 @@
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: scores out of tensor memory, weights P back into it as f16
 //   warps 8-11       convert the keys' K and V codes to f16 (exact) in shared memory, two stages of each
 //   warps 12, 13     issue a tile's tensor-core products S = Q K^T and O += P V (tcgen05, accumulators in tensor memory),
-//                    whichever is ready first.  One warp for both tiles spent more on looking and issuing (800 cycles for
-//                    each of the eight batches of 128 keys) than the products take
+//                    one warp per tile: one for both spent more on waiting and issuing (800 cycles for each of the eight
+//                    batches of 128 keys) than the products take
 // Tensor memory holds O of both tiles (2 x D columns) and two buffers of S for each, 64 keys wide, P over the S it comes
 // from: the scores of 64 keys are computed while the 64 before them are weighed, so that the softmax, which bounds this
 // kernel (one exponential per score: 16 a cycle and SM), does not wait for the products.  Two tiles per CTA halve the
@@ -23,8 +23,7 @@ constexpr int kHalf = kTileRows / 2;            // keys per buffer of scores
 constexpr int kPreThreads = 14 * 32;
 constexpr int kConvWarp = 8, kMmaWarp = 12;
 constexpr int kConstRing = 4;                   // steps whose page constants are held: the softmax may lag two behind
-constexpr int kPreWaitNs = 20000;
-constexpr int kPreWaitLimit = 50000;            // of waits of up to kPreWaitNs: about a second
+constexpr uint64_t kPreWaitNs = 1000000000;     // a wait gives up after a second
 constexpr uint32_t kTmemCols = 512;
 
 struct PrefillArgs {
@@ -85,18 +84,24 @@ __device__ __forceinline__ bool bar_test(uint64_t* b, uint32_t parity) {
                  : "=r"(ok) : "r"(s_addr(b)), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded wait; gives up at once when another warp has.
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* give_up) {
-    for (int i = 0; i < kPreWaitLimit; ++i) {
+// Bounded wait; gives up when another warp has, or after kPreWaitNs of its own.
+__device__ __noinline__ bool bar_wait_long(uint64_t* b, uint32_t parity, volatile int* give_up) {
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+    for (;;) {
         uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(s_addr(b)), "r"(parity), "r"(kPreWaitNs) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(s_addr(b)), "r"(parity) : "memory");
         if (ok) return true;
         if (*give_up) return false;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        if (t - t0 > kPreWaitNs) break;
     }
     *give_up = 1;
     return false;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* give_up) {
+    return bar_test(b, parity) || bar_wait_long(b, parity, give_up);
 }
 // The same by a warp, with one answer for all of it.
 __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, volatile int* give_up) {
@@ -482,9 +487,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     } else if (warp < kMmaWarp) {
         // ---- codes to f16 in shared memory ----
         constexpr int kPer = D / 16;                                        // 16-byte vectors per thread, K and V each
-        constexpr int kRowLanes = D / 16;                                   // threads per row
-        constexpr int kPass = 128 / kRowLanes;                              // rows per pass
-        const int ct = threadIdx.x - kConvWarp * 32, row0 = ct / kRowLanes, piece = ct % kRowLanes;
+        constexpr int kPass = 128 / kPer;                                   // rows per pass
+        // A thread's vector is 16 channels of a row and becomes two 16-byte chunks.  Eight lanes in a row take four
+        // vectors of two rows, whose chunks fall into different banks.
+        const int ct = threadIdx.x - kConvWarp * 32;
+        const int piece = D == 128 ? (ct & 3) | (ct >> 1 & 4) : ct & 3, row0 = D == 128 ? (ct >> 2 & 1) | (ct >> 4 << 1) : ct >> 2;
+        uint8_t* chunk0 = tile + (piece >> 2) * kSlab + row0 * 128 + ((((piece & 3) * 2) ^ (row0 & 7)) << 4);
+        uint8_t* chunk1 = tile + (piece >> 2) * kSlab + row0 * 128 + ((((piece & 3) * 2 + 1) ^ (row0 & 7)) << 4);
         const int32_t* table = a.c.tables + seq * a.c.table_stride;
         const int pages = (kv + kCachePage - 1) / kCachePage, ppb = a.c.shift - 4, in_block = (1 << a.c.shift) - 1;
         // block of page `lane` of a step, -1 where there is none
@@ -501,27 +510,36 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             return b;
         };
         auto fetch = [&](uint4 (&x)[kPer], const uint8_t* base, uint32_t sb, uint32_t sr, int step, int blocks, int rows) {
+            const bool whole = rows >= kTileRows && (__ballot_sync(0xffffffffu, blocks >= 0) & 0xff) == 0xff;
+            const uint8_t* at[kPer];
+            bool use[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int row = i * kPass + row0;
-                const int blk = __shfl_sync(0xffffffffu, blocks, row / kCachePage);
-                x[i] = make_uint4(0, 0, 0, 0);
-                if (blk >= 0 && row < rows)
-                    x[i] = __ldg((const uint4*)(base + (uint64_t)(uint32_t)blk * sb + (uint32_t)((step * kTileRows + row) & in_block) * sr));
+                const int blk = __shfl_sync(0xffffffffu, blocks, i * (kPass / kCachePage) + row0 / kCachePage);
+                use[i] = blk >= 0 && row < rows;
+                at[i] = base + (uint64_t)(uint32_t)blk * sb + (uint32_t)((step * kTileRows + row) & in_block) * sr;
+            }
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) x[i] = __ldg((const uint4*)at[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (use[i]) x[i] = __ldg((const uint4*)at[i]);
+                }
             }
         };
         auto put = [&](uint32_t at, const uint4 (&x)[kPer]) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int row = i * kPass + row0;
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                 uint32_t y[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) e4m3x4_f16(w[k], y[2 * k], y[2 * k + 1]);
-                uint8_t* dst = tile + at + (piece >> 2) * kSlab + row * 128;
-                const int c = (piece & 3) * 2, odd = (piece >> 2) & 1;      // the second slab's lanes write their odd chunk first: no bank twice
-                *(uint4*)(dst + (((c + odd) ^ (row & 7)) << 4)) = odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
-                *(uint4*)(dst + (((c + 1 - odd) ^ (row & 7)) << 4)) = odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+                *(uint4*)(chunk0 + at + i * kPass * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+                *(uint4*)(chunk1 + at + i * kPass * 128) = make_uint4(y[4], y[5], y[6], y[7]);
             }
         };
         const uint8_t* kb = a.c.k + head * a.c.k_sh + 16 * piece;
@@ -592,36 +610,34 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         const int ti = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
         const uint32_t base = s_addr(tile), t0 = __shfl_sync(0xffffffffu, tmem, 0);
         bool ok = warp_wait(&sh.q_full, 0, give_up);
-        int a = 0, b = 0, idle = 0;             // halves whose scores, and whose values, have been issued
-        while (ok && b < halves) {
-            bool did = false;
-            // scores go where the weights of two halves ago were: those must have been read
-            if (a < halves && (a < 2 || bar_test(&sh.pv_done[ti][a & 1], ((a >> 1) - 1) & 1)) && bar_test(&sh.k_full[(a >> 1) & 1], (a >> 2) & 1)) {
-                __syncwarp();
-                tc_fence_after();
-                if (elected()) {
-                    if (a & 2) { if (a & 1) issue_scores<D>(base, t0, ti, 1, 1, sh); else issue_scores<D>(base, t0, ti, 1, 0, sh); }
-                    else { if (a & 1) issue_scores<D>(base, t0, ti, 0, 1, sh); else issue_scores<D>(base, t0, ti, 0, 0, sh); }
-                }
-                __syncwarp();
-                ++a;
-                did = true;
+        auto scores = [&](int h) {
+            if (elected()) {
+                if (h & 2) { if (h & 1) issue_scores<D>(base, t0, ti, 1, 1, sh); else issue_scores<D>(base, t0, ti, 1, 0, sh); }
+                else { if (h & 1) issue_scores<D>(base, t0, ti, 0, 1, sh); else issue_scores<D>(base, t0, ti, 0, 0, sh); }
             }
-            if (b < a && bar_test(&sh.p_full[ti][b & 1], (b >> 1) & 1) && bar_test(&sh.v_full[(b >> 1) & 1], (b >> 2) & 1)) {
-                __syncwarp();
-                tc_fence_after();
-                if (elected()) {
-                    if (b & 2) { if (b & 1) issue_values<D>(base, t0, ti, 1, 1, true, sh); else issue_values<D>(base, t0, ti, 1, 0, true, sh); }
-                    else { if (b & 1) issue_values<D>(base, t0, ti, 0, 1, true, sh); else issue_values<D>(base, t0, ti, 0, 0, b > 0, sh); }
-                }
-                __syncwarp();
-                ++b;
-                did = true;
+            __syncwarp();
+        };
+        ok = ok && warp_wait(&sh.k_full[0], 0, give_up);
+        tc_fence_after();
+        if (ok) {
+            scores(0);
+            if (halves > 1) scores(1);
+        }
+        for (int h = 0; ok && h < halves; ++h) {
+            ok = warp_wait(&sh.p_full[ti][h & 1], (h >> 1) & 1, give_up) && warp_wait(&sh.v_full[(h >> 1) & 1], (h >> 2) & 1, give_up);
+            if (!ok) break;
+            tc_fence_after();
+            if (elected()) {
+                if (h & 2) { if (h & 1) issue_values<D>(base, t0, ti, 1, 1, true, sh); else issue_values<D>(base, t0, ti, 1, 0, true, sh); }
+                else { if (h & 1) issue_values<D>(base, t0, ti, 0, 1, true, sh); else issue_values<D>(base, t0, ti, 0, 0, h > 0, sh); }
             }
-            if (did) idle = 0;
-            else if (++idle > (1 << 25)) { *give_up = 1; ok = false; }
-            else if ((idle & 1023) == 0 && *give_up) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
+            __syncwarp();
+            if (h + 2 < halves) {               // the scores of two halves on go where the weights of this one are: they must have been read
+                ok = warp_wait(&sh.pv_done[ti][h & 1], (h >> 1) & 1, give_up) && warp_wait(&sh.k_full[((h + 2) >> 1) & 1], ((h + 2) >> 2) & 1, give_up);
+                if (!ok) break;
+                tc_fence_after();
+                scores(h + 2);
+            }
         }
         // nothing of this CTA may be in flight when its memory goes
         if (ok) {
