@@ -1,12 +1,16 @@
 // Decode attention over the block-scaled paged cache: one new token per sequence, its q heads against the sequence's
 // cached rows (the new one among them).
 //
-// The work is the cache's bytes, each to be read once: the pages (16 rows) of all (sequence, KV head) units are laid end to
-// end and every CTA takes an equal share of them, so that ragged lengths leave no SM idle and no host has to know a
-// length.  A CTA walks the units its share touches; its eight warps take every eighth page and keep (M, l, O) of the
-// unit's q heads in registers, merged through shared memory at the end of a unit.  A unit that one CTA holds whole is
-// written at once; parts of a unit that is cut go to a workspace, and a second launch, started while this one runs, joins
-// them.
+// The work is the cache's bytes, each to be read once.  A unit is a (sequence, KV head), with up to eight of its q heads; the
+// eight warps of a CTA take pages (16 rows) in turn, keep (M, l, O) in registers and merge them through shared memory.
+// Two kernels hand out the pages:
+//   clusters  a cluster of 1 to 8 CTAs per unit, whose parts meet in distributed shared memory: one launch, no workspace.  For
+//             tables that cannot hold long sequences, and for work that is small altogether.
+//   shares    the pages of all units laid end to end, every CTA taking an equal share of them, so that ragged lengths leave
+//             no SM idle and no host has to know a length.  A unit that one CTA holds whole is written at once; parts of a
+//             unit that is cut go to a workspace, and a second launch, started while this one runs, joins them.
+#include <atomic>
+
 #include "paged_attn.cuh"
 
 namespace fdms {
@@ -26,6 +30,7 @@ struct DecodeArgs {
     float* parts;                               // [ctas][2][kDecHeads][D + 2]: O, M, l
     int2* cuts;                                 // [units] first part and last CTA of a unit that is cut, (0, -1) of others
     int32_t batch, group, splits;               // splits: units per (sequence, KV head), each of up to 8 q heads
+    int32_t cluster;                            // CTAs per unit (clusters)
     float scale;
 };
 
@@ -298,14 +303,138 @@ __device__ __forceinline__ void page_prefix(const DecodeArgs& a, int32_t* s_firs
 __device__ __forceinline__ int64_t share(int64_t c, int64_t n, int64_t total) { return c * total / n; }
 __device__ __forceinline__ int owner(int64_t x, int64_t n, int64_t total) { return (int)(((x + 1) * n - 1) / total); }
 
+// The merge of a CTA's warps: every warp puts its state down, then warp h takes head h, D / 32 channels a lane.
+template <int D>
+struct MergeSmem {
+    float o[kDecWarps][kDecHeads][D];
+    float m[kDecWarps][kDecHeads], l[kDecWarps][kDecHeads];
+};
+static_assert(kDecWarps == kDecHeads, "the merge gives a head to a warp");
+
+template <int D>
+__device__ __forceinline__ void put_state(MergeSmem<D>& s, const UnitState<D>& st, int nh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float l = st.l[i];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (g == 0) { s.m[warp][2 * t + i] = st.m[i]; s.l[warp][2 * t + i] = l; }
+        if (2 * t + i < nh)
+#pragma unroll
+            for (int j = 0; j < D / 16; j += 2)
+                *(float4*)&s.o[warp][2 * t + i][(D / 8) * g + 2 * j] = make_float4(st.o[j][i], st.o[j][2 + i], st.o[j + 1][i], st.o[j + 1][2 + i]);
+    }
+}
+template <int D>
+__device__ __forceinline__ void merge_warps(const MergeSmem<D>& s, float (&acc)[D / 32], float& m, float& l) {
+    const int hd = threadIdx.x >> 5, ch = (threadIdx.x & 31) * (D / 32);
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, s.m[w][hd]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+        const float r = paged_ex2(s.m[w][hd] - ref);
+        l = fmaf(s.l[w][hd], r, l);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(s.o[w][hd][ch + i], r, acc[i]);
+    }
+}
+template <int D, bool BF16>
+__device__ __forceinline__ void write_row(const DecodeArgs& a, int seq, int hq, const float (&acc)[D / 32], float m, float l) {
+    const int lane = threadIdx.x & 31;
+    const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
+    uint16_t* out = a.out + seq * a.o_sb + (int64_t)hq * a.o_sh + lane * (D / 32);
+#pragma unroll
+    for (int i = 0; i < D / 32; i += 2) *(uint32_t*)(out + i) = pack_pair<BF16>(acc[i] * inv, acc[i + 1] * inv);
+    if (a.lse && lane == 0) a.lse[seq * a.lse_sb + (int64_t)hq * a.lse_sh] = kPagedLn2 * (m + paged_lg2(l));
+}
+
+// Clusters: unit blockIdx.x / cluster, page p of it with warp p % 8 of the cluster's CTA p / 8 % cluster.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_cluster_kernel(DecodeArgs a) {
+    __shared__ MergeSmem<D> s;
+    __shared__ float s_part[kDecHeads][D + 4];  // this CTA's part of the unit: O, M, l
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
+    const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
+    const int per_seq = a.c.heads * a.splits, seq = unit / per_seq, u = unit - seq * per_seq;
+    const int head = u / a.splits, h0 = (u % a.splits) * kDecHeads, nh = min(kDecHeads, a.group - h0);
+    const int len = paged_len(a.c, seq), pages = (int)(((int64_t)len + kCachePage - 1) / kCachePage);
+    const int first = rank * kDecWarps + warp, step = a.cluster * kDecWarps;
+    UnitState<D> st;
+    clear<D>(st);
+    if (first < pages) {
+        uint32_t qb[D / 16][2];
+        float factor[2];
+        load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
+        walk_pages<D>(a.c, st, qb, factor, seq, head, first, step, (pages - first + step - 1) / step, len);
+    }
+    put_state<D>(s, st, nh);
+    __syncthreads();
+    float acc[D / 32], m, l;
+    if (warp < nh) {
+        merge_warps<D>(s, acc, m, l);
+        if (a.cluster == 1) write_row<D, BF16>(a, seq, head * a.group + h0 + warp, acc, m, l);
+        else {
+#pragma unroll
+            for (int i = 0; i < D / 32; i += 2) *(float2*)&s_part[warp][lane * (D / 32) + i] = make_float2(acc[i], acc[i + 1]);
+            if (lane == 0) *(float2*)&s_part[warp][D] = make_float2(m, l);
+        }
+    }
+    if (a.cluster == 1) return;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp < nh && warp % a.cluster == rank) {                // heads are shared out among the cluster's CTAs
+        const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&s_part[warp][0]);
+        float pm[8], pl[8];
+        m = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            pm[r] = -INFINITY;
+            pl[r] = 0.0f;
+            if (r < a.cluster) {
+                uint32_t at;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + D * 4), "r"(r));
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(pm[r]), "=f"(pl[r]) : "r"(at) : "memory");
+            }
+            m = fmaxf(m, pm[r]);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < a.cluster) {
+                uint32_t at;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + lane * (D / 8)), "r"(r));
+                const float w = paged_ex2(pm[r] - ref);
+                l = fmaf(pl[r], w, l);
+#pragma unroll
+                for (int i = 0; i < D / 32; i += 2) {
+                    float x, y;
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x), "=f"(y) : "r"(at + 4 * i) : "memory");
+                    acc[i] = fmaf(x, w, acc[i]);
+                    acc[i + 1] = fmaf(y, w, acc[i + 1]);
+                }
+            }
+        write_row<D, BF16>(a, seq, head * a.group + h0 + warp, acc, m, l);
+    }
+    // a CTA's shared memory stays until every other has read it
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kernel(DecodeArgs a) {
     extern __shared__ int32_t s_first[];        // batch + 1
     __shared__ int32_t s_warp[kDecWarps];
-    __shared__ float s_o[kDecWarps][kDecHeads][D];
-    __shared__ float s_m[kDecWarps][kDecHeads], s_l[kDecWarps][kDecHeads];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    static_assert(kDecWarps == kDecHeads, "the merge gives a head to a warp");
+    __shared__ MergeSmem<D> s;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     pdl_trigger();
     page_prefix(a, s_first, s_warp);
     const int per_seq = a.c.heads * a.splits;
@@ -350,51 +479,19 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         UnitState<D> st;
         clear<D>(st);
         walk_pages<D>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len);
-        // merge the warps
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float l = st.l[i];
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (g == 0) { s_m[warp][2 * t + i] = st.m[i]; s_l[warp][2 * t + i] = l; }
-            if (2 * t + i < nh)
-#pragma unroll
-                for (int j = 0; j < D / 16; j += 2)
-                    *(float4*)&s_o[warp][2 * t + i][(D / 8) * g + 2 * j] =
-                        make_float4(st.o[j][i], st.o[j][2 + i], st.o[j + 1][i], st.o[j + 1][2 + i]);
-        }
+        put_state<D>(s, st, nh);
         __syncthreads();
         const bool whole = p0 == 0 && p1 == pages;
         const int slot = blockIdx.x * 2 + (at == begin ? 0 : 1);
-        constexpr int kVec = kDecHeads * D / kDecThreads;       // channels per thread: a head is a warp
-        const int hd = warp, ch = lane * kVec;
-        if (hd < nh) {
-            float mm = -INFINITY;
+        if (warp < nh) {
+            float acc[D / 32], m, l;
+            merge_warps<D>(s, acc, m, l);
+            if (whole) write_row<D, BF16>(a, seq, head * a.group + h0 + warp, acc, m, l);
+            else {
+                float* part = a.parts + ((int64_t)slot * kDecHeads + warp) * (D + 4);
 #pragma unroll
-            for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, s_m[w][hd]);
-            const float ref = mm == -INFINITY ? 0.0f : mm;
-            float ll = 0.0f, acc[kVec];
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kDecWarps; ++w) {
-                const float r = paged_ex2(s_m[w][hd] - ref);
-                ll = fmaf(s_l[w][hd], r, ll);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) acc[i] = fmaf(s_o[w][hd][ch + i], r, acc[i]);
-            }
-            if (whole) {
-                const float inv = ll > 0.0f || ll != ll ? __frcp_rn(ll) : 0.0f;
-                uint16_t* out = a.out + seq * a.o_sb + (int64_t)(head * a.group + h0 + hd) * a.o_sh + ch;
-#pragma unroll
-                for (int i = 0; i < kVec; i += 2) *(uint32_t*)(out + i) = pack_pair<BF16>(acc[i] * inv, acc[i + 1] * inv);
-                if (a.lse && lane == 0)
-                    a.lse[seq * a.lse_sb + (int64_t)(head * a.group + h0 + hd) * a.lse_sh] = kPagedLn2 * (mm + paged_lg2(ll));
-            } else {
-                float* part = a.parts + ((int64_t)slot * kDecHeads + hd) * (D + 4);
-#pragma unroll
-                for (int i = 0; i < kVec; i += 2) *(float2*)(part + ch + i) = make_float2(acc[i], acc[i + 1]);
-                if (lane == 0) *(float2*)(part + D) = make_float2(mm, ll);
+                for (int i = 0; i < D / 32; i += 2) *(float2*)(part + lane * (D / 32) + i) = make_float2(acc[i], acc[i + 1]);
+                if (lane == 0) *(float2*)(part + D) = make_float2(m, l);
             }
         }
         if (p0 == 0 && threadIdx.x == 0) {
@@ -427,7 +524,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(DecodeArgs a, in
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float ref = m == -INFINITY ? 0.0f : m;
     constexpr int kVec = D / 32;
-    float l = 0.0f, acc[kVec];
+    float l = 0.0f, acc[D / 32];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
 #pragma unroll 4
@@ -443,20 +540,21 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(DecodeArgs a, in
             acc[i + 1] = fmaf(x.y, w, acc[i + 1]);
         }
     }
-    const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
-    uint16_t* out = a.out + seq * a.o_sb + (int64_t)h * a.o_sh + lane * kVec;
-#pragma unroll
-    for (int i = 0; i < kVec; i += 2) *(uint32_t*)(out + i) = pack_pair<BF16>(acc[i] * inv, acc[i + 1] * inv);
-    if (a.lse && lane == 0) a.lse[seq * a.lse_sb + (int64_t)h * a.lse_sh] = kPagedLn2 * (m + paged_lg2(l));
+    write_row<D, BF16>(a, (int)seq, h, acc, m, l);
 }
 
 }  // namespace fdms
 
 using namespace fdms;
 
+// SM count of the current device.
 static int paged_sms() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -464,12 +562,23 @@ static int64_t decode_parts_bytes(int sms, int head_dim) {
     return (int64_t)sms * kDecCtasPerSm * 2 * kDecHeads * (head_dim + 4) * (int64_t)sizeof(float);
 }
 
-extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim) {
-    if (batch < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0) return -1;
+// CTAs per unit of the cluster kernel for sequences of up to `rows` rows, 0: the shares.  As many as one wave of the GPU
+// holds, each with a page for every warp; not where a CTA might get more than kClusterPages pages a warp, because then a long
+// sequence among short ones keeps its CTAs while the others are idle.
+constexpr int kClusterPages = 24;
+static int decode_cluster(int64_t units, int64_t rows, int sms) {
+    const int64_t pages = (rows + kCachePage - 1) / kCachePage;
+    int n = 1;
+    while (n < 8 && units * n * 2 <= (int64_t)sms * kDecCtasPerSm && pages > (int64_t)n * kDecWarps) n *= 2;
+    return pages <= (int64_t)n * kDecWarps * kClusterPages && units * n < (1ll << 31) ? n : 0;
+}
+
+extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows) {
+    if (batch < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || max_rows < 0) return -1;
     const int sms = paged_sms();
     if (sms <= 0) return -1;
-    const int group = num_q_heads / num_kv_heads;
-    return decode_parts_bytes(sms, head_dim) + (int64_t)batch * num_kv_heads * ((group + kDecHeads - 1) / kDecHeads) * (int64_t)sizeof(int2);
+    const int64_t units = batch * num_kv_heads * ((num_q_heads / num_kv_heads + kDecHeads - 1) / kDecHeads);
+    return decode_cluster(units, max_rows, sms) ? 0 : decode_parts_bytes(sms, (int)head_dim) + units * (int64_t)sizeof(int2);
 }
 
 extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream) {
@@ -488,27 +597,47 @@ extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void
     const int batch = (int)p.num_seqs;
     const int sms = paged_sms();
     FDMS_REQUIRE(sms > 0, FDMS_E_CUDA, "fdms_paged_attn_decode: cannot read the device's SM count");
-    const int64_t need = fdms_paged_attn_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim);
-    FDMS_REQUIRE(p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need, FDMS_E_WORKSPACE,
-                 "fdms_paged_attn_decode: workspace missing, unaligned or smaller than %lld bytes", (long long)need);
     a.q = (const uint16_t*)p.q;
     a.out = (uint16_t*)p.out;
     a.lse = p.lse_out;
     a.q_sb = p.q_stride[0]; a.q_sh = p.q_stride[1]; a.o_sb = p.out_stride[0]; a.o_sh = p.out_stride[1];
     a.lse_sb = p.lse_stride[0]; a.lse_sh = p.lse_stride[1];
-    a.parts = (float*)p.workspace;
-    a.cuts = (int2*)((char*)p.workspace + decode_parts_bytes(sms, head_dim));
     a.batch = batch;
     a.group = num_q_heads / num_kv_heads;
     a.splits = (a.group + kDecHeads - 1) / kDecHeads;
     a.scale = (float)p.scale;
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool bf = p.dtype == FDMS_BF16;
+    const int64_t units = (int64_t)batch * num_kv_heads * a.splits;
+    a.cluster = decode_cluster(units, p.max_blocks * p.cache.block_size, sms);
+    a.parts = nullptr;
+    a.cuts = nullptr;
+    if (a.cluster) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(units * a.cluster));
+        cfg.blockDim = dim3(kDecThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)a.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (head_dim == 64) FDMS_CUDA_OK(cudaLaunchKernelEx(&cfg, bf ? paged_decode_cluster_kernel<64, true> : paged_decode_cluster_kernel<64, false>, a));
+        else FDMS_CUDA_OK(cudaLaunchKernelEx(&cfg, bf ? paged_decode_cluster_kernel<128, true> : paged_decode_cluster_kernel<128, false>, a));
+        FDMS_CHECK_LAUNCH("paged_decode_cluster_kernel");
+        return FDMS_OK;
+    }
+    const int64_t need = decode_parts_bytes(sms, head_dim) + units * (int64_t)sizeof(int2);
+    FDMS_REQUIRE(p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need, FDMS_E_WORKSPACE,
+                 "fdms_paged_attn_decode: workspace missing, unaligned or smaller than %lld bytes", (long long)need);
+    a.parts = (float*)p.workspace;
+    a.cuts = (int2*)((char*)p.workspace + decode_parts_bytes(sms, head_dim));
     const int64_t rows_held = (int64_t)batch * p.max_blocks * (p.cache.block_size / kCachePage);
     FDMS_REQUIRE(rows_held < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_decode: the block tables hold too many rows");
     const int64_t useful = (rows_held * num_kv_heads * a.splits + 2 * kDecWarps - 1) / (2 * kDecWarps);
     const unsigned grid = (unsigned)(useful < 1 ? 1 : useful < (int64_t)sms * kDecCtasPerSm ? useful : (int64_t)sms * kDecCtasPerSm);
     const size_t smem = (size_t)(batch + 1) * sizeof(int32_t);
-    cudaStream_t st = (cudaStream_t)stream;
-    const bool bf = p.dtype == FDMS_BF16;
     const int64_t rows = (int64_t)batch * num_q_heads;
     const dim3 jgrid((unsigned)((rows + 7) / 8));
 #define FDMS_DECODE(DIM, BF)                                                                                        \

@@ -167,11 +167,11 @@ def build_paged_metadata(
     kv_lens_out = kv_lens if kv_lens_out is None else kv_lens_out
     free_count_out = free_count if free_count_out is None else free_count_out
     if cu_seqlens is None:
-        cu_seqlens = torch.empty(n + 1, dtype=_I32, device=device)
+        cu_seqlens = kv_lens.new_empty(n + 1)
     if slot_mapping is None:
-        slot_mapping = torch.empty(total_tokens, dtype=_I32, device=device)
+        slot_mapping = kv_lens.new_empty(total_tokens)
     if positions is None:
-        positions = torch.empty(total_tokens, dtype=_I64, device=device)
+        positions = kv_lens.new_empty(total_tokens, dtype=_I64)
     need = _lib.lib().fdms_paged_metadata_workspace_bytes(n, total_tokens)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch(_lib.lib().fdms_paged_metadata, _METADATA_ARGS.pack(
@@ -271,7 +271,7 @@ def _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_
         _device(dict(q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_tables=block_tables, kv_lens=kv_lens,
                      cu_seqlens_q=cu_seqlens_q))
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q)
     elif out.shape != shape or out.dtype is not q.dtype:
         raise ValueError("out must have q's shape and dtype")
     elif out.get_device() != dev:
@@ -285,8 +285,9 @@ def _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_
         lse_ptr, lse_stride = lse_out.data_ptr(), lse_out.stride()
     lib, need, ws = _lib.lib(), 0, None
     if cu_seqlens_q is None:
-        need = _on_device(dev, lib.fdms_paged_attn_decode_workspace_bytes, tokens, num_q_heads, heads, head_dim)
-        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=q.device)
+        need = _on_device(dev, lib.fdms_paged_attn_decode_workspace_bytes, tokens, num_q_heads, heads, head_dim, cols * block_size)
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch(lib.fdms_paged_attn_decode if cu_seqlens_q is None else lib.fdms_paged_attn_prefill, _ATTN_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, block_size, head_dim,
         *k_cache.stride(), *v_cache.stride(), q.data_ptr(), out.data_ptr(), lse_ptr, block_tables.data_ptr(), kv_lens.data_ptr(),

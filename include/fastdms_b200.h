@@ -515,8 +515,8 @@ int32_t fdms_linear_decode_allreduce(
  *   tokens are consecutive; no block is written by two sequences.
  * fdms_paged_attn_decode: out[b, hq] = softmax(scale * q[b, hq] K^T) V over the first kv_lens[b] rows, q [batch, q_heads,
  *   head_dim]; no rows: zeros.  lse_out (optional): natural-log log-sum-exp, -inf without rows.  batch <= 2048.
- *   workspace: fdms_paged_attn_decode_workspace_bytes(...) bytes of the current device, 16-byte aligned, any contents; calls
- *   that share one must not overlap on the GPU.
+ *   workspace: fdms_paged_attn_decode_workspace_bytes(...) bytes on the current device (max_rows = max_blocks * block_size),
+ *   16-byte aligned, any contents; calls that share one must not overlap on the GPU.
  * fdms_paged_attn_prefill: q [tokens, q_heads, head_dim], sequence s's tokens at cu_seqlens_q[s] .. cu_seqlens_q[s + 1];
  *   with n of them, token i sees rows 0 .. kv_lens[s] - n + i (none: zeros, lse -inf).  Tokens behind the last sequence
  *   are left untouched.
@@ -572,7 +572,7 @@ int32_t fdms_paged_release(
     int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
     int32_t* dev_status, void* stream);
 int32_t fdms_paged_store(const fdms_paged_store_args* args, void* stream);
-int64_t fdms_paged_attn_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
+int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows);
 int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream);
 int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, void* stream);
 

@@ -334,11 +334,21 @@ DECODE = [
     ([600], 1, 12, 64, 128, "f16", "hnd"), ([9000, 3, 0, 1200], 1, 4, 16, 64, "f16", "hnd"), ([100, 90], 1, 64, 16, 64, "bf16", "hnd")]
 
 
+def wide_table(table, bs, rows=40000):
+    """The same table with columns for long sequences, which the decode kernel for short ones does not take."""
+    wide = torch.full((table.shape[0], rows // bs), -1, dtype=torch.int32, device=table.device)
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("lens,heads,group,bs,d,dt,layout", DECODE)
-def test_decode(dev, lens, heads, group, bs, d, dt, layout):
+def test_decode(dev, lens, heads, group, bs, d, dt, layout, wide):
     from fastdms_b200.layers.paged_attention import paged_decode_attention
     rng = np.random.default_rng(sum(lens) + heads + group + d)
     (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, lens, heads, bs, d, dev, layout)
+    if wide:
+        table = wide_table(table, bs)
     q = _random_rows(rng, (len(lens), heads * group, d), dt, loud=False)
     lse = torch.full((len(lens), heads * group), 7.0, device=dev)
     got = paged_decode_attention(q.to(dev), kc, vc, ks, vs, table, i32(lens, dev), lse_out=lse)
@@ -383,14 +393,17 @@ def _magnitudes(rng, lens, heads, bs, d, dev, exps):
     return (kc, vc, ks, vs, table), (codes, scale, tab)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("exps,dt", [((-50, 0, 40), "bf16"), ((-6, 0, 6), "f16"), ((-30, -29), "bf16")])
-def test_blocks_of_very_different_magnitude(dev, exps, dt):
+def test_blocks_of_very_different_magnitude(dev, exps, dt, wide):
     """V blocks between tiny and huge: the weights stay exact enough for each (a block that matters little in the sum may
     not cost one that matters its digits)."""
     from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
     rng = np.random.default_rng(5)
     lens, heads, group, bs, d = [400], 2, 4, 16, 64
     (kc, vc, ks, vs, table), (codes, scale, tab) = _magnitudes(rng, lens, heads, bs, d, dev, exps)
+    if wide:
+        table = wide_table(table, bs)
     q = _random_rows(rng, (1, heads * group, d), dt, loud=False)
     lse, lse2 = torch.empty((1, heads * group), device=dev), torch.empty((heads * group, 1), device=dev)
     dec = paged_decode_attention(q.to(dev), kc, vc, ks, vs, table, i32(lens, dev), lse_out=lse)
@@ -428,13 +441,14 @@ def test_queries_of_very_different_magnitude(dev):
         assert (np.abs(got[0, r] - v[s.argmax()]) <= 2.0 ** -8 * np.abs(v[s.argmax()])).all()
 
 
-def test_decode_leaves_out_what_cannot_be(dev):
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_leaves_out_what_cannot_be(dev, wide):
     from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
     rng = np.random.default_rng(8)
     lens, heads, group, bs, d = [70, 40], 1, 2, 16, 64
     (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, lens, heads, bs, d, dev)
     q = _random_rows(rng, (2, group, d), "bf16", loud=False).to(dev)
-    bad = table.clone()
+    bad = wide_table(table, bs) if wide else table.clone()
     bad[0, 1], bad[0, 3] = -1, kc.shape[0]
     keep = np.r_[0:16, 32:48, 64:70]
     k, v = (O.rows_of(codes[c], scale[c], tab[0], 70, 0, bs)[keep] for c in range(2))
@@ -580,12 +594,12 @@ class Run:
     """A small server: sequences that are prefilled (in chunks), decode and end, driven through the public calls; beside it
     the same in the plain statement."""
 
-    def __init__(self, dev, seed, n=4, heads=2, group=2, bs=16, d=64, dt="bf16", pool=60):
+    def __init__(self, dev, seed, n=4, heads=2, group=2, bs=16, d=64, dt="bf16", pool=60, cols=20):
         self.dev, self.rng = dev, np.random.default_rng(seed)
         self.n, self.heads, self.group, self.bs, self.d, self.dt, self.pool = n, heads, group, bs, d, dt, pool
         self.kc, self.vc, self.ks, self.vs = make_cache(pool, heads, bs, d, dev)
         self.kv, self.count = i32([0] * n, dev), i32([pool], dev)
-        self.table = i32(np.full((n, 20), -1), dev)
+        self.table = i32(np.full((n, cols), -1), dev)
         self.free = torch.arange(pool, device=dev, dtype=torch.int32).flip(0).contiguous()
         self.codes = [codes_of(self.kc), codes_of(self.vc)]
         self.scale = [np.full((pool, heads), np.nan) for _ in range(2)]
@@ -635,10 +649,11 @@ def test_a_run_of_steps(dev, bs, d, dt):
     assert int(r.count) == r.pool and sorted(r.free.tolist()) == list(range(r.pool))
 
 
-def test_a_captured_step_replays(dev):
+@pytest.mark.parametrize("cols", [20, 1250])
+def test_a_captured_step_replays(dev, cols):
     """A decode step captured once advances the sequences at every replay; two captured graphs, replayed in turn, do not
     disturb each other's workspaces."""
-    a, b = Run(dev, 1), Run(dev, 2, n=3, bs=32, d=128, dt="f16")
+    a, b = Run(dev, 1, cols=2500), Run(dev, 2, n=3, bs=32, d=128, dt="f16", cols=cols)
     graphs = []
     for r in (a, b):
         r.step([7 * i + 3 for i in range(r.n)])
@@ -668,9 +683,10 @@ def test_a_captured_step_replays(dev):
             r.check([1] * r.n, hq, hk, hv, out, slots)
 
 
-def test_two_streams_at_once(dev):
+@pytest.mark.parametrize("cols", [20, 2500])
+def test_two_streams_at_once(dev, cols):
     """Independent steps on two streams, interleaved without any wait between them."""
-    runs = [Run(dev, 5), Run(dev, 6, d=128, dt="f16")]
+    runs = [Run(dev, 5, cols=cols), Run(dev, 6, d=128, dt="f16", cols=cols)]
     streams = [torch.cuda.Stream(dev) for _ in runs]
     for r in runs:
         r.step([300, 120, 7, 250])
@@ -698,7 +714,8 @@ def test_two_streams_at_once(dev):
         assert last[0].tolist() == got[-1][2].tolist()
 
 
-def test_decode_and_prefill_agree_with_the_same_bits_twice(dev):
+@pytest.mark.parametrize("wide", [False, True])
+def test_decode_and_prefill_agree_with_the_same_bits_twice(dev, wide):
     """The same call gives the same bits again, whatever the order in which CTAs finish."""
     from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
     g = torch.Generator(device=dev).manual_seed(3)
@@ -712,6 +729,8 @@ def test_decode_and_prefill_agree_with_the_same_bits_twice(dev):
         table[i, :m] = torch.arange(at, at + m, device=dev)
         at += m
     q = torch.randn((4, heads * group, d), device=dev, generator=g).to(torch.bfloat16)
+    if wide:
+        table = wide_table(table, bs)
     first = paged_decode_attention(q, kc, vc, ks, vs, table, i32(lens, dev))
     other = paged_prefill_attention(q, kc, vc, ks, vs, table, i32(lens, dev), i32(range(5), dev))
     for _ in range(5):

@@ -138,7 +138,7 @@ def test_c_decode_refuses(change, code, words):
     lib = _lib.lib()
     assert lib.fdms_paged_attn_decode(P._ATTN_ARGS.pack(*(ATTN | change).values()), None) == code and words in lib.fdms_last_error()
     assert lib.fdms_paged_attn_decode(None, None) == E
-    assert lib.fdms_paged_attn_decode_workspace_bytes(2, 3, 2, 64) < 0
+    assert lib.fdms_paged_attn_decode_workspace_bytes(2, 3, 2, 64, 64) < 0
 
 
 @pytest.mark.parametrize("change,code,words", BAD_ATTN + [(dict(cu=0), E, b"null pointer"), (dict(tokens=-1), E, b"negative")])
