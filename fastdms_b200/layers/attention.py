@@ -4,8 +4,12 @@ Mirrors the reference's `fastdms/layers/attention.py` for the compact path: modu
 `compact_k_cache`, `compact_v_cache`, `layer_id`; `forward(q, k, v, *, compact_append_stored,
 compact_q_rope, positions, cos_sin_cache)`; per-step inputs come from the global Context.
 Prefill attention is dense and causal (eviction only decides what is packed into the compact
-pool); it runs through torch's scaled_dot_product_attention per sequence.  The reference's dense
-paged KV branches do not exist here: compact-DMS mode allocates no dense blocks.
+pool); it runs through torch's scaled_dot_product_attention per sequence.
+
+Without compact KV, a Context that carries `block_tables`, `slot_mapping` and `context_lens` selects the dense paged
+branch (reference: attention.py:82-92, 124-151): K and V of the step are stored into the layer's `k_cache` / `v_cache`
+(e4m3 blocks with the scales `k_cache_scale` / `v_cache_scale`, `layers/paged_attention.py`) and attention reads them
+from there, prompts and single tokens alike.
 """
 from __future__ import annotations
 
@@ -15,6 +19,7 @@ from torch import nn
 
 from fastdms_b200.layers.compact_attention import (compact_decode_attention, compact_prefix_attention,
                                                    fused_store_decode_attention, store_compact_kvcache)
+from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention, store_paged_kvcache
 from fastdms_b200.utils.context import get_context
 from fastdms_b200.utils.profiler import get_profiler
 
@@ -71,6 +76,8 @@ class Attention(nn.Module):
         self.num_kv_heads = num_kv_heads
         self.compact_k_cache = self.compact_v_cache = torch.tensor([])
         self.compact_k_scale = self.compact_v_scale = None
+        self.k_cache = self.v_cache = torch.tensor([])               # dense paged cache of the layer and its block scales
+        self.k_cache_scale = self.v_cache_scale = None
         self.layer_id = -1
 
     def can_fuse_store(self) -> bool:
@@ -97,10 +104,27 @@ class Attention(nn.Module):
                 block_tables=bt, k_scale=self.compact_k_scale, v_scale=self.compact_v_scale,
                 overlap_previous_kernel=context.overlap_store_and_attention)
 
+    def _forward_paged(self, q, k, v, context, prof):
+        """Dense paged branch: stores the step's K and V, then attends over the cache."""
+        if self.k_cache.numel() == 0 or self.k_cache_scale is None or self.v_cache_scale is None:
+            raise RuntimeError("dense paged attention requires the layer's k_cache, v_cache and their scales")
+        if context.slot_mapping is None or context.context_lens is None:
+            raise RuntimeError("dense paged attention requires slot_mapping and context_lens")
+        cache = (self.k_cache, self.v_cache, self.k_cache_scale, self.v_cache_scale)
+        with prof.cuda_phase("paged_store"):
+            store_paged_kvcache(k, v, *cache, context.slot_mapping)
+        if context.is_prefill:
+            with prof.cuda_phase("paged_prefill_attn"):
+                return paged_prefill_attention(q, *cache, context.block_tables, context.context_lens, context.cu_seqlens_q, self.scale)
+        with prof.cuda_phase("paged_decode_attn"):
+            return paged_decode_attention(q, *cache, context.block_tables, context.context_lens, self.scale)
+
     def forward(self, q, k, v, *, compact_append_stored: bool = False, compact_q_rope: bool = False,
                 positions: torch.Tensor | None = None, cos_sin_cache: torch.Tensor | None = None):
         context = get_context()
         prof = get_profiler()
+        if context.block_tables is not None and not context.compact_kv_enabled:
+            return self._forward_paged(q, k, v, context, prof)
         if context.is_prefill:
             cu = context.cu_seqlens_host
             if cu is None:
