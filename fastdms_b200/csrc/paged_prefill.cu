@@ -9,8 +9,8 @@
 //   warps 12, 13     issue a tile's tensor-core products S = Q K^T and O += P V (tcgen05, accumulators in tensor memory),
 //                    one warp per tile: one for both spent more on waiting and issuing (800 cycles for each of the eight
 //                    batches of 128 keys) than the products take
-// Tensor memory holds O of both tiles (2 x D columns) and two buffers of S for each, 64 keys wide, P over the S it comes
-// from: the scores of 64 keys are computed while the 64 before them are weighed, so that the softmax, which bounds this
+// Tensor memory holds O of both tiles (2 x D columns) and for each two (D = 64: three) buffers of S, 64 keys wide, P over the
+// S it comes from: the scores of 64 keys are computed while the 64 before them are weighed, so that the softmax, which bounds this
 // kernel (one exponential per score: 16 a cycle and SM), does not wait for the products.  Two tiles per CTA halve the
 // conversions.  Every wait is bounded; when one runs out the CTA raises FDMS_DEV_WAIT_TIMEOUT, gives its tensor memory back
 // and returns.
@@ -258,6 +258,8 @@ constexpr uint32_t kSlab = kTileRows * 128;     // bytes
 template <int D>
 struct PrefillSmem {
     static constexpr uint32_t kTile = kTileRows * D * 2;        // one operand tile
+    static constexpr int kBufs = D == 64 ? 3 : 2;               // what the tensor memory has room for
+    static constexpr uint32_t kO = 2 * kBufs * kHalf;           // columns: S of tile i from i * kBufs * kHalf on, O at kO + i * D
     static constexpr uint32_t kQ = 0, kK = 2 * kTile, kV = 4 * kTile, kEnd = 6 * kTile;
     // 1 KB for the alignment of the tiles; D = 64 asks for more than half of the SM's shared memory all the same, because a
     // second CTA would wait for tensor memory that the first holds
@@ -265,7 +267,7 @@ struct PrefillSmem {
 };
 
 struct PrefillShared {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2];
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][3], p_full[2][3], pv_done[2][3];
     float4 page[kConstRing][kTileRows / kCachePage];            // ks, log2 vs, 1 / vs of the step's pages
     uint32_t tmem;
     int give_up, nan_lo, nan_hi;
@@ -278,25 +280,25 @@ __device__ __forceinline__ bool elected() {
 }
 // Scores of tile ti against the half h of the keys in stage st; the weights of tile ti times the values of that half.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, int h, PrefillShared& sh) {
+__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, PrefillShared& sh) {
     using L = PrefillSmem<D>;
     const uint64_t q = operand(base + L::kQ + ti * L::kTile, 16, 1024), k = operand(base + L::kK + st * L::kTile + h * (kHalf * 128), 16, 1024);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
         const uint32_t step = ((i >> 2) * kSlab + (i & 3) * 32) >> 4;      // addresses are in units of 16 bytes
-        mma_ss(tmem + 128 * ti + kHalf * h, q + step, k + step, instruction(kHalf, false), i > 0);
+        mma_ss(tmem + (L::kBufs * ti + buf) * kHalf, q + step, k + step, instruction(kHalf, false), i > 0);
     }
-    tc_commit(&sh.s_full[ti][h]);
+    tc_commit(&sh.s_full[ti][buf]);
     tc_commit(&sh.k_empty[st]);
 }
 template <int D>
-__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, int h, bool add, PrefillShared& sh) {
+__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, bool add, PrefillShared& sh) {
     using L = PrefillSmem<D>;
     const uint64_t v = operand(base + L::kV + st * L::kTile + h * (kHalf * 128), kSlab, 1024);
 #pragma unroll
     for (int i = 0; i < kHalf / 16; ++i)
-        mma_ts(tmem + 256 + 128 * ti, tmem + 128 * ti + kHalf * h + 8 * i, v + (i * 2048 >> 4), instruction(D, true), i > 0 || add);
-    tc_commit(&sh.pv_done[ti][h]);
+        mma_ts(tmem + L::kO + D * ti, tmem + (L::kBufs * ti + buf) * kHalf + 8 * i, v + (i * 2048 >> 4), instruction(D, true), i > 0 || add);
+    tc_commit(&sh.pv_done[ti][buf]);
     tc_commit(&sh.v_empty[st]);
 }
 
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             bar_init(&sh.v_full[i], 4);
             bar_init(&sh.k_empty[i], 2 * tiles);
             bar_init(&sh.v_empty[i], 2 * tiles);
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < 3; ++k) {
                 bar_init(&sh.s_full[i][k], 1);
                 bar_init(&sh.p_full[i][k], 4);
                 bar_init(&sh.pv_done[i][k], 1);
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;              // S of tile i at 128 i and 128 i + 64, O at 256 + 128 i
+    const uint32_t tmem = sh.tmem;
     volatile int* give_up = &sh.give_up;
 
     if (warp < kConvWarp) {
@@ -395,14 +397,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         __syncwarp();
         if (lane == 0) bar_arrive(&sh.q_full);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;                  // the warp's 32 lanes of tensor memory
-        const uint32_t o_at = tmem + lanes + 256 + 128 * ti;
+        const uint32_t o_at = tmem + lanes + L::kO + D * ti;
         float m = -INFINITY, l = 0.0f;
         bool ok = ti < tiles;
+        int buf = 0, turn = 0;                  // buffer of the half, and how often it has been used before (mod 2)
         for (int half = 0; ok && half < halves; ++half) {
-            ok = warp_wait(&sh.s_full[ti][half & 1], (half >> 1) & 1, give_up);
+            ok = warp_wait(&sh.s_full[ti][buf], turn, give_up);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t s_at = tmem + lanes + 128 * ti + kHalf * (half & 1);
+            const uint32_t s_at = tmem + lanes + (L::kBufs * ti + buf) * kHalf;
             const float4* page = &sh.page[(half >> 1) & (kConstRing - 1)][(half & 1) * (kHalf / kCachePage)];
             const int seen = (int)min(last - (int64_t)half * kHalf, (int64_t)kHalf);         // last key of the half that the row sees
             const bool cut = __any_sync(0xffffffffu, seen < kHalf - 1);
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     m = next;
                     l *= r;
                     if (half > 0) {             // the products of the half before must be complete before O is touched
-                        ok = warp_wait(&sh.pv_done[ti][(half - 1) & 1], ((half - 1) >> 1) & 1, give_up);
+                        ok = warp_wait(&sh.pv_done[ti][buf ? buf - 1 : L::kBufs - 1], buf ? turn : turn ^ 1, give_up);
                         tc_fence_after();
                         rescale_o<D>(o_at, r);
                     }
@@ -445,10 +448,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(&sh.p_full[ti][half & 1]);
+            if (lane == 0) bar_arrive(&sh.p_full[ti][buf]);
+            if (++buf == L::kBufs) { buf = 0; turn ^= 1; }
         }
         if (ti < tiles) {
-            if (halves > 0 && ok) ok = warp_wait(&sh.pv_done[ti][(halves - 1) & 1], ((halves - 1) >> 1) & 1, give_up);
+            if (halves > 0 && ok) ok = warp_wait(&sh.pv_done[ti][(halves - 1) % L::kBufs], ((halves - 1) / L::kBufs) & 1, give_up);
             tc_fence_after();
             const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
             uint16_t* out = a.out + tok * a.o_st + (int64_t)hq * a.o_sh;
@@ -610,38 +614,40 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         const int ti = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
         const uint32_t base = s_addr(tile), t0 = __shfl_sync(0xffffffffu, tmem, 0);
         bool ok = warp_wait(&sh.q_full, 0, give_up);
-        auto scores = [&](int h) {
+        auto scores = [&](int h, int buf) {
             if (elected()) {
-                if (h & 2) { if (h & 1) issue_scores<D>(base, t0, ti, 1, 1, sh); else issue_scores<D>(base, t0, ti, 1, 0, sh); }
-                else { if (h & 1) issue_scores<D>(base, t0, ti, 0, 1, sh); else issue_scores<D>(base, t0, ti, 0, 0, sh); }
+                if (h & 2) { if (h & 1) issue_scores<D>(base, t0, ti, 1, 1, buf, sh); else issue_scores<D>(base, t0, ti, 1, 0, buf, sh); }
+                else { if (h & 1) issue_scores<D>(base, t0, ti, 0, 1, buf, sh); else issue_scores<D>(base, t0, ti, 0, 0, buf, sh); }
             }
             __syncwarp();
         };
-        ok = ok && warp_wait(&sh.k_full[0], 0, give_up);
-        tc_fence_after();
-        if (ok) {
-            scores(0);
-            if (halves > 1) scores(1);
+        for (int h = 0; ok && h < L::kBufs && h < halves; ++h) {
+            ok = warp_wait(&sh.k_full[(h >> 1) & 1], 0, give_up);
+            tc_fence_after();
+            if (ok) scores(h, h);
         }
+        int buf = 0, turn = 0;
         for (int h = 0; ok && h < halves; ++h) {
-            ok = warp_wait(&sh.p_full[ti][h & 1], (h >> 1) & 1, give_up) && warp_wait(&sh.v_full[(h >> 1) & 1], (h >> 2) & 1, give_up);
+            ok = warp_wait(&sh.v_full[(h >> 1) & 1], (h >> 2) & 1, give_up) && warp_wait(&sh.p_full[ti][buf], turn, give_up);
             if (!ok) break;
             tc_fence_after();
             if (elected()) {
-                if (h & 2) { if (h & 1) issue_values<D>(base, t0, ti, 1, 1, true, sh); else issue_values<D>(base, t0, ti, 1, 0, true, sh); }
-                else { if (h & 1) issue_values<D>(base, t0, ti, 0, 1, true, sh); else issue_values<D>(base, t0, ti, 0, 0, h > 0, sh); }
+                if (h & 2) { if (h & 1) issue_values<D>(base, t0, ti, 1, 1, buf, true, sh); else issue_values<D>(base, t0, ti, 1, 0, buf, true, sh); }
+                else { if (h & 1) issue_values<D>(base, t0, ti, 0, 1, buf, true, sh); else issue_values<D>(base, t0, ti, 0, 0, buf, h > 0, sh); }
             }
             __syncwarp();
-            if (h + 2 < halves) {               // the scores of two halves on go where the weights of this one are: they must have been read
-                ok = warp_wait(&sh.pv_done[ti][h & 1], (h >> 1) & 1, give_up) && warp_wait(&sh.k_full[((h + 2) >> 1) & 1], ((h + 2) >> 2) & 1, give_up);
+            const int next = h + L::kBufs;
+            if (next < halves) {                // its scores go where the weights of this half are: they must have been read
+                ok = warp_wait(&sh.k_full[(next >> 1) & 1], (next >> 2) & 1, give_up) && warp_wait(&sh.pv_done[ti][buf], turn, give_up);
                 if (!ok) break;
                 tc_fence_after();
-                scores(h + 2);
+                scores(next, buf);
             }
+            if (++buf == L::kBufs) { buf = 0; turn ^= 1; }
         }
         // nothing of this CTA may be in flight when its memory goes
         if (ok) {
-            warp_wait(&sh.pv_done[ti][(halves - 1) & 1], ((halves - 1) >> 1) & 1, give_up);
+            warp_wait(&sh.pv_done[ti][(halves - 1) % L::kBufs], ((halves - 1) / L::kBufs) & 1, give_up);
         } else {                                // after a wait that ran out: let what was issued complete
             if (elected()) tc_commit(&sh.q_full);
             for (int i = 0; i < 100 && !bar_test(&sh.q_full, 1); ++i) __nanosleep(10000);
