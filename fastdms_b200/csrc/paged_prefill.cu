@@ -363,11 +363,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         float factor;
         {
             const uint16_t* q = a.q + tok * a.q_st + (int64_t)hq * a.q_sh;
+            uint4 w[D / 8];                     // the whole row at once: one latency
             float top = 0.0f;
-#pragma unroll 4
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) w[i] = make_uint4(0, 0, 0, 0);
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) w[i] = __ldg((const uint4*)(q + 8 * i));
+            }
+#pragma unroll
             for (int i = 0; i < D / 8; ++i) {
-                const uint4 w = live ? *(const uint4*)(q + 8 * i) : make_uint4(0, 0, 0, 0);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float e, f;
@@ -379,10 +385,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             row_power(top, up, factor);
             factor *= a.scale * kPagedLog2e;
             uint8_t* dst = tile + L::kQ + ti * L::kTile + r * 128;
-#pragma unroll 4
+#pragma unroll
             for (int i = 0; i < D / 8; ++i) {
-                const uint4 w = live ? *(const uint4*)(q + 8 * i) : make_uint4(0, 0, 0, 0);
-                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
                 uint32_t y[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
