@@ -216,56 +216,70 @@ __device__ __forceinline__ void page_values(UnitState<D>& u, const PageRegs<D>& 
     }
 }
 
-// The warp's pages first, first + step, ... (`count` of them) of a sequence's KV head, whose first `len` rows count.  32 of
-// them at a time, one per lane, are looked up in the table.
+// Table entry of page first + step * (base + lane), read ahead of everything that says whether the page exists: any column
+// of the sequence's row may be read.
+__device__ __forceinline__ int entry_ahead(const PagedCache& c, int seq, int first, int step, int base) {
+    const int64_t col = ((int64_t)first + (int64_t)step * (base + (int)(threadIdx.x & 31))) >> (c.shift - 4);
+    return col < c.max_blocks ? c.tables[seq * c.table_stride + col] : -1;
+}
+
+// The warp's pages first, first + step, ... (`count` of them) of a sequence's KV head, whose first `len` rows count.  Their
+// table entries and scales are held 32 pages at a time, one per lane: `entry` are the first 32, the next are requested while
+// these are walked.
 template <int D>
 __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u, const uint32_t (&qb)[D / 16][2], const float (&factor)[2],
-                                           int seq, int head, int first, int step, int count, int len) {
+                                           int seq, int head, int first, int step, int count, int len, int entry) {
+    if (c.num_blocks == 0 || count <= 0) return;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int ppb = c.shift - 4, in_block = (1 << ppb) - 1;
+    const int in_block = (1 << (c.shift - 4)) - 1;
     const uint32_t k_sr = (uint32_t)c.k_sr, v_sr = (uint32_t)c.v_sr;
     const uint8_t* kb = c.k + head * c.k_sh + g * c.k_sr + 16 * t;
     const uint8_t* vb = c.v + head * c.v_sh + 2 * t * c.v_sr + (D / 8) * g;
-    const int32_t* table = c.tables + seq * c.table_stride;
-    for (int base = 0; base < count; base += 32) {
-        int my_block = -1;
-        float my_ks = 0.0f, my_vs = 1.0f;
-        if (base + lane < count) {
-            my_block = table[(first + step * (base + lane)) >> ppb];
-            if (my_block < 0 || my_block >= c.num_blocks) {
-                my_block = -1;
-                if (c.status) atomicOr(c.status, FDMS_DEV_BAD_INDEX);
-            } else {
-                my_ks = c.k_scale[(int64_t)my_block * c.heads + head];
-                my_vs = c.v_scale[(int64_t)my_block * c.heads + head];
-            }
-        }
-        const float my_lvs = paged_lg2(my_vs), my_ivs = __frcp_rn(my_vs);
-        const int n = min(32, count - base);
-        PageRegs<D> pg;
-        auto block_of = [&](int i) { return __shfl_sync(0xffffffffu, my_block, i); };
-        auto row_of = [&](int i) { return (uint32_t)((first + step * (base + i)) & in_block) * kCachePage; };
-        // a page that is left out reads block 0, and none of its rows count
-        auto fetch_k = [&](int i) {
-            load_k<D>(pg, kb + (uint64_t)(uint32_t)max(block_of(i), 0) * (uint32_t)c.k_sb + row_of(i) * k_sr, k_sr);
-        };
-        auto fetch_v = [&](int i) {
-            load_v<D>(pg, vb + (uint64_t)(uint32_t)max(block_of(i), 0) * (uint32_t)c.v_sb + row_of(i) * v_sr, v_sr);
-        };
-        if (c.num_blocks == 0) return;          // nothing to read, not even block 0
-        fetch_k(0);
-        fetch_v(0);
-        for (int i = 0; i < n; ++i) {
-            const int rows = block_of(i) < 0 ? 0 : min(kCachePage, len - (first + step * (base + i)) * kCachePage);
-            float s[4];
-            page_scores<D>(pg, qb, s);
-            if (i + 1 < n) fetch_k(i + 1);
-            uint32_t b0, b1;
-            page_weights<D>(u, s, __shfl_sync(0xffffffffu, my_ks, i), __shfl_sync(0xffffffffu, my_lvs, i), __shfl_sync(0xffffffffu, my_ivs, i),
-                            factor, rows, lane, b0, b1);
-            if (rows < kCachePage) mask_v<D>(pg, rows, t);
-            page_values<D>(u, pg, b0, b1);
-            if (i + 1 < n) fetch_v(i + 1);
+    // a usable block, or -1: such a page reads block 0, and none of its rows count
+    auto block_in = [&](int e, int base) {
+        if (base + lane >= count) return -1;
+        if (e >= 0 && e < c.num_blocks) return e;
+        if (c.status) atomicOr(c.status, FDMS_DEV_BAD_INDEX);
+        return -1;
+    };
+    auto scale_of = [&](const float* s, int block) { return block >= 0 ? __ldg(s + (int64_t)block * c.heads + head) : 1.0f; };
+    int block = block_in(entry, 0), next = entry_ahead(c, seq, first, step, 32);
+    float ks = scale_of(c.k_scale, block), vs = scale_of(c.v_scale, block), next_ks = 1.0f, next_vs = 1.0f;
+    PageRegs<D> pg;
+    auto fetch_k = [&](int blk, int i) {
+        const uint32_t row = (uint32_t)((first + step * i) & in_block) * kCachePage;
+        load_k<D>(pg, kb + (uint64_t)(uint32_t)max(blk, 0) * (uint32_t)c.k_sb + row * k_sr, k_sr);
+    };
+    auto fetch_v = [&](int blk, int i) {
+        const uint32_t row = (uint32_t)((first + step * i) & in_block) * kCachePage;
+        load_v<D>(pg, vb + (uint64_t)(uint32_t)max(blk, 0) * (uint32_t)c.v_sb + row * v_sr, v_sr);
+    };
+    int blk = __shfl_sync(0xffffffffu, block, 0);
+    fetch_k(blk, 0);
+    fetch_v(blk, 0);
+    float lvs = paged_lg2(vs), ivs = __frcp_rn(vs);
+    for (int i = 0; i < count; ++i) {
+        const int j = i & 31;
+        if (j == 8) next = block_in(next, i + 24);
+        if (j == 16) { next_ks = scale_of(c.k_scale, next); next_vs = scale_of(c.v_scale, next); }
+        const int rows = blk < 0 ? 0 : min(kCachePage, len - (first + step * i) * kCachePage);
+        const bool more = i + 1 < count;
+        const int then = j == 31 ? __shfl_sync(0xffffffffu, next, 0) : __shfl_sync(0xffffffffu, block, j + 1);
+        float s[4];
+        page_scores<D>(pg, qb, s);
+        if (more) fetch_k(then, i + 1);
+        uint32_t b0, b1;
+        page_weights<D>(u, s, __shfl_sync(0xffffffffu, ks, j), __shfl_sync(0xffffffffu, lvs, j), __shfl_sync(0xffffffffu, ivs, j), factor, rows, lane, b0, b1);
+        if (rows < kCachePage) mask_v<D>(pg, rows, t);
+        page_values<D>(u, pg, b0, b1);
+        if (more) fetch_v(then, i + 1);
+        blk = then;
+        if (j == 31) {
+            block = next;
+            ks = next_ks;
+            lvs = paged_lg2(next_vs);
+            ivs = __frcp_rn(next_vs);
+            next = entry_ahead(c, seq, first, step, i + 33);
         }
     }
 }
@@ -363,16 +377,16 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
     const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
     const int per_seq = a.c.heads * a.splits, seq = unit / per_seq, u = unit - seq * per_seq;
     const int head = u / a.splits, h0 = (u % a.splits) * kDecHeads, nh = min(kDecHeads, a.group - h0);
-    const int len = paged_len(a.c, seq), pages = (int)(((int64_t)len + kCachePage - 1) / kCachePage);
     const int first = rank * kDecWarps + warp, step = a.cluster * kDecWarps;
+    // length, table entries and queries are requested together
+    const int entry = entry_ahead(a.c, seq, first, step, 0);
+    const int len = paged_len(a.c, seq), pages = (int)(((int64_t)len + kCachePage - 1) / kCachePage);
+    uint32_t qb[D / 16][2];
+    float factor[2];
+    load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
     UnitState<D> st;
     clear<D>(st);
-    if (first < pages) {
-        uint32_t qb[D / 16][2];
-        float factor[2];
-        load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
-        walk_pages<D>(a.c, st, qb, factor, seq, head, first, step, (pages - first + step - 1) / step, len);
-    }
+    walk_pages<D>(a.c, st, qb, factor, seq, head, first, step, first < pages ? (pages - first + step - 1) / step : 0, len, entry);
     put_state<D>(s, st, nh);
     __syncthreads();
     float acc[D / 32], m, l;
@@ -473,12 +487,13 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         const int p0 = (int)(at - unit_begin), p1 = (int)min((int64_t)pages, end - unit_begin);
         const int head = u / a.splits, h0 = (u % a.splits) * kDecHeads, nh = min(kDecHeads, a.group - h0);
         const int len = min(paged_len(a.c, seq), pages * kCachePage);
+        const int entry = entry_ahead(a.c, seq, p0 + warp, kDecWarps, 0);
         uint32_t qb[D / 16][2];
         float factor[2];
         load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
         UnitState<D> st;
         clear<D>(st);
-        walk_pages<D>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len);
+        walk_pages<D>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len, entry);
         put_state<D>(s, st, nh);
         __syncthreads();
         const bool whole = p0 == 0 && p1 == pages;
