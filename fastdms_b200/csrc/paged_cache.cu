@@ -327,6 +327,17 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
     }
 }
 
+// The larger of each half of two words; of a number and a NaN the number.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    if (BF16) {
+        const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+        return *(const uint32_t*)&m;
+    }
+    const __half2 m = __hmax2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&m;
+}
+
 // D: head_dim.  A lane holds 8 elements of every (32 / (D / 8))-th row of the warp's 16.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreArgs a) {
@@ -341,22 +352,19 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreA
     const int which = have && item >= a.heads ? 1 : 0, head = have ? item - which * a.heads : 0;
     const int bs = 1 << a.shift;
 
-    // runs that begin in this CTA's tokens
+    // the slots of 32 tokens, of which those of this CTA may begin a run
     const int64_t first = (int64_t)blockIdx.x * a.group;
-    int32_t my_slot = -1;
-    bool begins = false;
-    if (lane < a.group && first + lane < a.tokens) {
-        const int64_t t = first + lane;
-        my_slot = a.slots[t];
-        const int32_t prev = t > 0 ? a.slots[t - 1] : -1;
-        if (my_slot >= 0) {
-            begins = (my_slot & (bs - 1)) == 0 || prev != my_slot - 1;
-            // a slot map lists a block's tokens in order and together
-            if (my_slot >= a.num_slots || (begins && prev >= 0 && (prev >> a.shift) == (my_slot >> a.shift))) {
-                begins = false;
-                if (a.status) atomicOr(a.status, FDMS_DEV_BAD_INDEX);
-            }
-        }
+    const int32_t my_slot = first + lane < a.tokens ? __ldg(a.slots + first + lane) : -1;
+    int32_t prev = lane == 0 && first > 0 ? __ldg(a.slots + first - 1) : -1;
+    {
+        const int32_t up = __shfl_up_sync(0xffffffffu, my_slot, 1);
+        if (lane > 0) prev = up;
+    }
+    bool begins = lane < a.group && my_slot >= 0 && ((my_slot & (bs - 1)) == 0 || prev != my_slot - 1);
+    // a slot map lists a block's tokens in order and together
+    if (begins && (my_slot >= a.num_slots || (prev >= 0 && (prev >> a.shift) == (my_slot >> a.shift)))) {
+        begins = false;
+        if (a.status) atomicOr(a.status, FDMS_DEV_BAD_INDEX);
     }
     unsigned todo = __ballot_sync(0xffffffffu, begins);
     const int col = (lane % kLanes) * 8, row0 = lane / kLanes;
@@ -368,14 +376,18 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreA
         const int block = slot >> a.shift, off = slot & (bs - 1);
         float* scale = a.scale[which] + (int64_t)block * a.heads + head;
         const float old = have && off > 0 ? *scale : 0.0f;
-        int count = 1;                          // rows of the run: slots that follow one another, inside the block
-        for (int base = 1; base < bs - off; base += 32) {
-            const int i = base + lane;
-            const bool on = i < bs - off && t0 + i < a.tokens && a.slots[t0 + i] == slot + i;
-            const unsigned m = __ballot_sync(0xffffffffu, on);
-            const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-            count += run;
-            if (run < 32) break;
+        // rows of the run: slots that follow one another, inside the block
+        int count;
+        {
+            const int d = lane - src_lane;
+            const unsigned m = __ballot_sync(0xffffffffu, d > 0 && d < bs - off && my_slot == slot + d) >> src_lane >> 1;
+            count = __ffs(~m);
+            for (int base = count; base == count && base >= 32 - src_lane && base < bs - off; base += 32) {    // beyond the 32
+                const int i = base + lane;
+                const bool on = i < bs - off && t0 + i < a.tokens && a.slots[t0 + i] == slot + i;
+                const unsigned more = __ballot_sync(0xffffffffu, on);
+                count += more == 0xffffffffu ? 32 : __ffs(~more) - 1;
+            }
         }
         // the 16-row parts of the block that this warp writes
         const int lo = W > 1 ? part : off >> 4, hi = W > 1 ? part : (off + count - 1) >> 4;
@@ -390,20 +402,19 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreA
                 if (have && r >= 0 && r < count) x[j] = __ldg((const uint4*)(src + r * a.src_st[which]));
             }
         };
-        float top = 0.0f;
+        uint32_t most = 0;                      // largest magnitudes of the even and the odd elements, as they are
         for (int p = lo; p <= hi; ++p) {
             load(p);
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
                 const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float f, g;
-                    unpack2<BF16>(w[i], f, g);
-                    top = fmaxf(top, fmaxf(fabsf(f), fabsf(g)));    // a NaN does not count
-                }
+                for (int i = 0; i < 4; ++i) most = max2<BF16>(most, w[i] & 0x7fff7fffu);      // a NaN does not count
             }
         }
+        float top, odd;
+        unpack2<BF16>(most, top, odd);
+        top = fmaxf(top, odd);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (W > 1) {
