@@ -85,6 +85,7 @@ _SIGNATURES = {
     "fdms_paged_store": (I32, [c_char_p, P]),
     "fdms_paged_attn_decode_workspace_bytes": (I64, [I64, I64, I64, I64, I64]),
     "fdms_paged_attn_decode": (I32, [c_char_p, P]),
+    "fdms_paged_attn_prefill_workspace_bytes": (I64, [I64, I64, I64, I64, I64, I64]),
     "fdms_paged_attn_prefill": (I32, [c_char_p, P]),
 }
 

@@ -12,6 +12,8 @@
 // 2^-28 of the row's largest.  P is rounded to f16, 2^-12 of a weight at most; scores, M, l and the output are float32.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace fdms {
@@ -104,6 +106,17 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+
+// SM count of the current device.
+inline int paged_sms() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 // Checks of a cache that every entry makes; `idle`: the call has nothing to do, so its pointers may be null.

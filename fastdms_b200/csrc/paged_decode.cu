@@ -9,8 +9,6 @@
 //   shares    the pages of all units laid end to end, every CTA taking an equal share of them, so that ragged lengths leave
 //             no SM idle and no host has to know a length.  A unit that one CTA holds whole is written at once; parts of a
 //             unit that is cut go to a workspace, and a second launch, started while this one runs, joins them.
-#include <atomic>
-
 #include "paged_attn.cuh"
 
 namespace fdms {
@@ -561,17 +559,6 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(DecodeArgs a, in
 }  // namespace fdms
 
 using namespace fdms;
-
-// SM count of the current device.
-static int paged_sms() {
-    static std::atomic<int> known[64];
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
-    return n;
-}
 
 static int64_t decode_parts_bytes(int sms, int head_dim) {
     return (int64_t)sms * kDecCtasPerSm * 2 * kDecHeads * (head_dim + 4) * (int64_t)sizeof(float);

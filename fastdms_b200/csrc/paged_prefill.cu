@@ -2,8 +2,8 @@
 // sequence's cached rows.  Token i of a sequence with n tokens in the step and kv rows in the cache sees rows
 // 0 .. kv - n + i; a token that sees no row gets zeros and a log-sum-exp of -inf.
 //
-// A CTA takes two tiles of 128 rows ((token, q head) pairs of one KV head, the heads of a token together) and walks the
-// sequence's rows in tiles of 128 keys:
+// A CTA takes two tiles of 128 rows ((token, q head) pairs of one KV head, the heads of a token together), or one where there
+// are few, and walks the sequence's rows, or its part of them, in tiles of 128 keys:
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: scores out of tensor memory, weights P back into it as f16
 //   warps 8-11       convert the keys' K and V codes to f16 (exact) in shared memory, two stages of each
 //   warps 12, 13     issue a tile's tensor-core products S = Q K^T and O += P V (tcgen05, accumulators in tensor memory),
@@ -14,6 +14,9 @@
 // kernel (one exponential per score: 16 a cycle and SM), does not wait for the products.  Two tiles per CTA halve the
 // conversions.  Every wait is bounded; when one runs out the CTA raises FDMS_DEV_WAIT_TIMEOUT, gives its tensor memory back
 // and returns.
+//
+// Few tokens over many rows would leave most SMs idle: the rows are then cut into parts for a CTA each, whose results go to a
+// workspace and are joined by a second launch.
 #include "paged_attn.cuh"
 
 namespace fdms {
@@ -34,7 +37,9 @@ struct PrefillArgs {
     const int32_t* cu;                          // [seqs + 1]
     int64_t q_st, q_sh, o_st, o_sh, lse_sh, lse_st;
     int64_t tokens;
+    float* parts;                               // [splits][tokens][q_heads][D + 4]: O, M, l of a part of the rows
     int32_t seqs, group;
+    int32_t tiles, splits;                      // tiles of rows per CTA (1 or 2), parts that the cached rows are cut into
     float scale;
 };
 
@@ -307,18 +312,24 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     extern __shared__ uint8_t dyn[];
     __shared__ PrefillShared sh;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = kTileRows / a.group;        // tokens per tile of rows
+    if (a.splits > 1) pdl_trigger();
+    const int per = kTileRows / a.group;        // tokens per tile
     int seq;
     int64_t first, begin, count;
     // the last tiles of a sequence see the most rows: they start first
-    if (!find_tile(a, (int64_t)gridDim.x - 1 - blockIdx.x, 2 * per, seq, first, begin, count)) return;
+    if (!find_tile(a, (int64_t)gridDim.x - 1 - blockIdx.x, a.tiles * per, seq, first, begin, count)) return;
     const int head = blockIdx.y;
     const int kv = paged_len(a.c, seq);
-    const int64_t shift = (int64_t)kv - count;  // token j of the sequence's step sees rows 0 .. shift + j
-    const int64_t end = min(first + 2 * per, count);
-    const int tiles = first + per < count ? 2 : 1;
-    const int steps = (int)((max(shift + end, (int64_t)0) + kTileRows - 1) / kTileRows);
-    const int halves = (int)((max(shift + end, (int64_t)0) + kHalf - 1) / kHalf);
+    const int64_t end = min(first + a.tiles * per, count);
+    const int tiles = a.tiles > 1 && first + per < count ? 2 : 1;
+    // the CTA's part of the rows begins at row `from`; from here on rows count from there
+    const int64_t sees = max((int64_t)kv - count + end, (int64_t)0);
+    const int all = (int)((sees + kTileRows - 1) / kTileRows), part = (all + a.splits - 1) / a.splits;
+    const int from = min((int)blockIdx.z * part, all) * kTileRows;
+    const int64_t here = min(max(sees - from, (int64_t)0), (int64_t)part * kTileRows);
+    const int64_t shift = (int64_t)kv - count - from;       // token j of the sequence's step sees rows 0 .. shift + j
+    const int rows = kv - from;
+    const int steps = (int)((here + kTileRows - 1) / kTileRows), halves = (int)((here + kHalf - 1) / kHalf);
     // keys below `open` are seen by every row of the CTA
     const int64_t open = max(shift + first + 1, (int64_t)0);
     uint8_t* tile = (uint8_t*)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
@@ -461,6 +472,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             tc_fence_after();
             const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
             uint16_t* out = a.out + tok * a.o_st + (int64_t)hq * a.o_sh;
+            float* mine = a.parts + (((int64_t)blockIdx.z * a.tokens + tok) * (a.c.heads * a.group) + hq) * (D + 4);
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
@@ -470,7 +482,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     tmem_load(o_at + 16 * c, o);
                     tc_wait_ld(o);
                 }
-                if (live) {
+                if (live && a.splits > 1) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) *(uint4*)(mine + 16 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else if (live) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 8) {
                         uint32_t y[4];
@@ -481,16 +496,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     }
                 }
             }
-            if (live && a.lse) a.lse[(int64_t)hq * a.lse_sh + tok * a.lse_st] = kPagedLn2 * (m + paged_lg2(l));
+            if (live && a.splits > 1) *(float2*)(mine + D) = make_float2(m, l);
+            else if (live && a.lse) a.lse[(int64_t)hq * a.lse_sh + tok * a.lse_st] = kPagedLn2 * (m + paged_lg2(l));
             // NaN codes of V in steps that not every row sees whole were left out of the products: into the rows that see them
             const int lo = *(volatile int*)&sh.nan_lo, hi = *(volatile int*)&sh.nan_hi;
             if (live && lo <= hi)
                 for (int64_t key = (int64_t)lo * kTileRows; key < (int64_t)(hi + 1) * kTileRows && key <= last; ++key) {
-                    const int blk = a.c.tables[seq * a.c.table_stride + (key >> a.c.shift)];
+                    const int blk = a.c.tables[seq * a.c.table_stride + ((from + key) >> a.c.shift)];
                     if (blk < 0 || blk >= a.c.num_blocks) continue;
-                    const uint8_t* v = a.c.v + (int64_t)blk * a.c.v_sb + head * a.c.v_sh + (key & ((1 << a.c.shift) - 1)) * a.c.v_sr;
+                    const uint8_t* v = a.c.v + (int64_t)blk * a.c.v_sb + head * a.c.v_sh + ((from + key) & ((1 << a.c.shift) - 1)) * a.c.v_sr;
                     for (int ch = 0; ch < D; ++ch)
-                        if ((v[ch] & 0x7f) == 0x7f) out[ch] = BF16 ? 0x7fff : 0x7fff;
+                        if ((v[ch] & 0x7f) == 0x7f) {
+                            if (a.splits > 1) mine[ch] = NAN; else out[ch] = 0x7fff;        // a NaN in bf16 and in f16
+                        }
                 }
         }
     } else if (warp < kMmaWarp) {
@@ -507,7 +525,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         const int pages = (kv + kCachePage - 1) / kCachePage, ppb = a.c.shift - 4, in_block = (1 << a.c.shift) - 1;
         // block of page `lane` of a step, -1 where there is none
         auto look_up = [&](int step) {
-            const int p = step * (kTileRows / kCachePage) + lane;
+            const int p = (from + step * kTileRows) / kCachePage + lane;
             int b = -1;
             if (lane < kTileRows / kCachePage && p < pages) {
                 b = table[p >> ppb];
@@ -518,15 +536,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             }
             return b;
         };
-        auto fetch = [&](uint4 (&x)[kPer], const uint8_t* base, uint32_t sb, uint32_t sr, int step, int blocks, int rows) {
-            const bool whole = rows >= kTileRows && (__ballot_sync(0xffffffffu, blocks >= 0) & 0xff) == 0xff;
+        auto fetch = [&](uint4 (&x)[kPer], const uint8_t* base, uint32_t sb, uint32_t sr, int step, int blocks, int left) {
+            const bool whole = left >= kTileRows && (__ballot_sync(0xffffffffu, blocks >= 0) & 0xff) == 0xff;
             const uint8_t* at[kPer];
             bool use[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int row = i * kPass + row0;
                 const int blk = __shfl_sync(0xffffffffu, blocks, i * (kPass / kCachePage) + row0 / kCachePage);
-                use[i] = blk >= 0 && row < rows;
+                use[i] = blk >= 0 && row < left;
                 at[i] = base + (uint64_t)(uint32_t)blk * sb + (uint32_t)((step * kTileRows + row) & in_block) * sr;
             }
             if (whole) {
@@ -566,8 +584,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             }
         };
         scales();
-        fetch(xk, kb, k_sb, k_sr, 0, blocks, kv);
-        fetch(xv, vb, v_sb, v_sr, 0, blocks, kv);
+        fetch(xk, kb, k_sb, k_sr, 0, blocks, rows);
+        fetch(xv, vb, v_sb, v_sr, 0, blocks, rows);
         blocks = look_up(1);
         bool ok = true;
         for (int step = 0; ok && step < steps; ++step) {
@@ -583,7 +601,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (lane == 0) bar_arrive(&sh.k_full[st]);
             if (more) {
                 scales();
-                fetch(xk, kb, k_sb, k_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+                fetch(xk, kb, k_sb, k_sr, step + 1, blocks, rows - (step + 1) * kTileRows);
             }
             if (step >= 2) ok = warp_wait(&sh.v_empty[st], ((step >> 1) - 1) & 1, give_up);
             if (!ok) break;
@@ -609,7 +627,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.v_full[st]);
             if (more) {
-                fetch(xv, vb, v_sb, v_sr, step + 1, blocks, kv - (step + 1) * kTileRows);
+                fetch(xv, vb, v_sb, v_sr, step + 1, blocks, rows - (step + 1) * kTileRows);
                 blocks = look_up(step + 2);
             }
         }
@@ -666,9 +684,94 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
+// Joins the parts that the same tiles left: a CTA per (tile, KV head, eight of its rows), a warp per row.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(PrefillArgs a) {
+    const int lane = threadIdx.x & 31, per = kTileRows / a.group;
+    int seq;
+    int64_t first, begin, count;
+    pdl_wait();
+    if (!find_tile(a, (int64_t)blockIdx.x, a.tiles * per, seq, first, begin, count)) return;
+    const int hq = a.c.heads * a.group;
+    const int64_t n = min((int64_t)a.tiles * per, count - first) * a.group;
+    const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
+    if (r < n) {
+        const int64_t tok = begin + first + r / a.group;
+        const int h = blockIdx.y * a.group + r % a.group;
+        auto part = [&](int z) { return a.parts + (((int64_t)z * a.tokens + tok) * hq + h) * (D + 4); };
+        float m = lane < a.splits ? part(lane)[D] : -INFINITY, pl = lane < a.splits ? part(lane)[D + 1] : 0.0f;
+        const float pm = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // a part without a row that this one sees holds nothing
+        const unsigned held = __ballot_sync(0xffffffffu, pm != -INFINITY || pl != 0.0f);
+        const float w = pm == -INFINITY ? 0.0f : paged_ex2(pm - m);
+        float l = pl * w;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float acc[D / 32];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+        for (int z = 0; z < a.splits; ++z) {
+            const float wz = __shfl_sync(0xffffffffu, w, z);
+            if (!(held >> z & 1)) continue;
+            const float* p = part(z) + lane * (D / 32);
+#pragma unroll
+            for (int i = 0; i < D / 32; i += 2) {
+                const float2 x = *(const float2*)(p + i);
+                acc[i] = fmaf(x.x, wz, acc[i]);
+                acc[i + 1] = fmaf(x.y, wz, acc[i + 1]);
+            }
+        }
+        const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
+        uint16_t* out = a.out + tok * a.o_st + (int64_t)h * a.o_sh + lane * (D / 32);
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) *(uint32_t*)(out + i) = pack_pair<BF16>(acc[i] * inv, acc[i + 1] * inv);
+        if (a.lse && lane == 0) a.lse[(int64_t)h * a.lse_sh + tok * a.lse_st] = kPagedLn2 * (m + paged_lg2(l));
+    }
+}
+
 }  // namespace fdms
 
 using namespace fdms;
+
+// Tiles of rows per CTA and parts of the cached rows: the combination with the least time by what was measured, in half
+// microseconds: a step of 128 keys takes 4 with one tile and 5 with two, a CTA 8 besides, the join 8 and its traffic.  The
+// longest sequence that the tables can hold stands for all.
+struct PrefillPlan {
+    int64_t ctas;                               // per KV head
+    int tiles, splits;
+};
+static PrefillPlan prefill_plan(int64_t tokens, int64_t seqs, int64_t heads, int group, int64_t head_dim, int64_t max_rows, int sms) {
+    PrefillPlan best = {0, 0, 0};
+    const int per = kTileRows / group;
+    const int64_t steps = (max_rows + kTileRows - 1) / kTileRows;
+    double least = 0.0;
+    for (int tiles = 1; tiles <= 2; ++tiles)
+        for (int splits = 1; splits <= 16 && (splits == 1 || splits * 2 <= steps); ++splits) {
+            const int64_t ctas = tokens / (tiles * per) + seqs, waves = (ctas * heads * splits + sms - 1) / sms;
+            const double join = splits > 1 ? 8.0 + splits * (double)tokens * heads * group * (head_dim + 4) * 8.0 / 2.5e6 : 0.0;
+            const double time = waves * (8.0 + (double)((steps + splits - 1) / splits) * (3 + tiles)) + join;
+            if (best.tiles == 0 || time < least) {
+                best = {ctas, tiles, splits};
+                least = time;
+            }
+        }
+    return best;
+}
+
+extern "C" int64_t fdms_paged_attn_prefill_workspace_bytes(int64_t tokens, int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                           int64_t max_rows) {
+    if (tokens < 0 || num_seqs < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > kTileRows / 2 ||
+        head_dim <= 0 || max_rows < 0)
+        return -1;
+    if (tokens == 0 || num_seqs == 0) return 0;
+    const int sms = paged_sms();
+    if (sms <= 0) return -1;
+    const int splits = prefill_plan(tokens, num_seqs, num_kv_heads, (int)(num_q_heads / num_kv_heads), head_dim, max_rows, sms).splits;
+    return splits == 1 ? 0 : splits * tokens * num_q_heads * (head_dim + 4) * (int64_t)sizeof(float);
+}
 
 extern "C" int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, void* stream) {
     clear_error();
@@ -679,12 +782,19 @@ extern "C" int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, voi
     if (idle) return FDMS_OK;
     const fdms_paged_attn_args& p = *args;
     FDMS_REQUIRE(p.cu_seqlens_q, FDMS_E_ARG, "fdms_paged_attn_prefill: null pointer");
-    const int group = (int)p.num_q_heads / c.heads;
+    const int group = (int)p.num_q_heads / c.heads, sms = paged_sms();
+    FDMS_REQUIRE(sms > 0, FDMS_E_CUDA, "fdms_paged_attn_prefill: cannot read the device's SM count");
+    const PrefillPlan plan = prefill_plan(p.tokens, p.num_seqs, c.heads, group, p.cache.head_dim, p.max_blocks * p.cache.block_size, sms);
+    FDMS_REQUIRE(plan.ctas < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_prefill: too many tokens");
+    if (plan.splits > 1) {
+        const int64_t need = plan.splits * p.tokens * p.num_q_heads * (p.cache.head_dim + 4) * (int64_t)sizeof(float);
+        FDMS_REQUIRE(p.workspace && ((uintptr_t)p.workspace & 15) == 0 && p.workspace_bytes >= need, FDMS_E_WORKSPACE,
+                     "fdms_paged_attn_prefill: workspace missing, unaligned or smaller than %lld bytes", (long long)need);
+    }
     PrefillArgs a = {c, (const uint16_t*)p.q, (uint16_t*)p.out, p.lse_out, p.cu_seqlens_q, p.q_stride[0], p.q_stride[1], p.out_stride[0],
-                     p.out_stride[1], p.lse_stride[0], p.lse_stride[1], p.tokens, (int32_t)p.num_seqs, group, (float)p.scale};
-    const int64_t tiles = p.tokens / (2 * (kTileRows / group)) + p.num_seqs;
-    FDMS_REQUIRE(tiles < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_attn_prefill: too many tokens");
-    const dim3 grid((unsigned)tiles, (unsigned)c.heads);
+                     p.out_stride[1], p.lse_stride[0], p.lse_stride[1], p.tokens, (float*)p.workspace, (int32_t)p.num_seqs, group, plan.tiles,
+                     plan.splits, (float)p.scale};
+    const dim3 grid((unsigned)plan.ctas, (unsigned)c.heads, (unsigned)plan.splits), jgrid((unsigned)plan.ctas, (unsigned)c.heads, (unsigned)(plan.tiles * kTileRows / 8));
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = p.dtype == FDMS_BF16;
 #define FDMS_PREFILL(DIM, BF)                                                                                                           \
@@ -692,6 +802,8 @@ extern "C" int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, voi
         constexpr int bytes = (int)PrefillSmem<DIM>::kBytes;                                                                            \
         FDMS_CUDA_OK(cudaFuncSetAttribute(paged_prefill_kernel<DIM, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));           \
         paged_prefill_kernel<DIM, BF><<<grid, kPreThreads, bytes, st>>>(a);                                                             \
+        FDMS_CHECK_LAUNCH("paged_prefill_kernel");                                                                                      \
+        if (plan.splits > 1) FDMS_CUDA_OK(launch_chained(paged_prefill_join_kernel<DIM, BF>, jgrid, dim3(256), st, true, a));             \
     } while (0)
     if (p.cache.head_dim == 64) {
         if (bf) FDMS_PREFILL(64, true); else FDMS_PREFILL(64, false);
@@ -699,6 +811,6 @@ extern "C" int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, voi
         if (bf) FDMS_PREFILL(128, true); else FDMS_PREFILL(128, false);
     }
 #undef FDMS_PREFILL
-    FDMS_CHECK_LAUNCH("paged_prefill_kernel");
+    FDMS_CHECK_LAUNCH("paged_prefill_join_kernel");
     return FDMS_OK;
 }

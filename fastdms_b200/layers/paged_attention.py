@@ -286,8 +286,10 @@ def _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_
     lib, need, ws = _lib.lib(), 0, None
     if cu_seqlens_q is None:
         need = _on_device(dev, lib.fdms_paged_attn_decode_workspace_bytes, tokens, num_q_heads, heads, head_dim, cols * block_size)
-        if need > 0:
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        need = _on_device(dev, lib.fdms_paged_attn_prefill_workspace_bytes, tokens, seqs, num_q_heads, heads, head_dim, cols * block_size)
+    if need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch(lib.fdms_paged_attn_decode if cu_seqlens_q is None else lib.fdms_paged_attn_prefill, _ATTN_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, block_size, head_dim,
         *k_cache.stride(), *v_cache.stride(), q.data_ptr(), out.data_ptr(), lse_ptr, block_tables.data_ptr(), kv_lens.data_ptr(),

@@ -519,7 +519,7 @@ int32_t fdms_linear_decode_allreduce(
  *   16-byte aligned, any contents; calls that share one must not overlap on the GPU.
  * fdms_paged_attn_prefill: q [tokens, q_heads, head_dim], sequence s's tokens at cu_seqlens_q[s] .. cu_seqlens_q[s + 1];
  *   with n of them, token i sees rows 0 .. kv_lens[s] - n + i (none: zeros, lse -inf).  Tokens behind the last sequence
- *   are left untouched.
+ *   are left untouched.  workspace: fdms_paged_attn_prefill_workspace_bytes(...) bytes, as above.
  * Both attentions: q_heads = kv_heads times 1 to 64, bf16 / f16; a needed table entry outside [0, num_blocks) is left out
  * and raises FDMS_DEV_BAD_INDEX, as does a length beyond the table.
  * --------------------------------------------------------------------------------------------- */
@@ -574,6 +574,8 @@ int32_t fdms_paged_release(
 int32_t fdms_paged_store(const fdms_paged_store_args* args, void* stream);
 int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows);
 int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream);
+int64_t fdms_paged_attn_prefill_workspace_bytes(int64_t tokens, int64_t num_seqs, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t max_rows);
 int32_t fdms_paged_attn_prefill(const fdms_paged_attn_args* args, void* stream);
 
 #ifdef __cplusplus

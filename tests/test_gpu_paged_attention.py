@@ -477,7 +477,8 @@ PREFILL = [
     ([(5, 205), (0, 30), (130, 130), (1, 64)], 2, 4, 16, 128, "f16", "hnd"), ([(33, 300), (64, 64)], 1, 3, 64, 64, "bf16", "layers"),
     ([(200, 456)], 1, 7, 128, 128, "bf16", "hnd"), ([(40, 25), (3, 0), (20, 20)], 2, 2, 16, 64, "bf16", "hnd"),
     ([(17, 17)] * 9, 1, 5, 16, 64, "f16", "nhd"), ([(70, 150)], 1, 64, 16, 64, "bf16", "hnd"), ([(300, 1100)], 1, 1, 16, 128, "bf16", "hnd"),
-    ([(31, 31)], 1, 24, 32, 128, "f16", "hnd"), ([(129, 129), (257, 700)], 1, 2, 64, 128, "bf16", "hnd")]
+    ([(31, 31)], 1, 24, 32, 128, "f16", "hnd"), ([(129, 129), (257, 700)], 1, 2, 64, 128, "bf16", "hnd"),
+    ([(5, 4100), (2, 1)], 1, 4, 16, 128, "bf16", "hnd"), ([(1, 2500), (70, 2050)], 2, 8, 16, 64, "f16", "nhd")]
 
 
 def _prefill(dev, rng, seqs, heads, group, bs, d, dt, layout, pad=3):
@@ -498,11 +499,15 @@ def check_prefill(got, lse, q, cu, seqs, host, heads, group, bs, d, dt):
                 check_rows(got[rows, j], None if lse is None else lse[j, rows], want, dt)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("seqs,heads,group,bs,d,dt,layout", PREFILL)
-def test_prefill(dev, seqs, heads, group, bs, d, dt, layout):
+def test_prefill(dev, seqs, heads, group, bs, d, dt, layout, wide):
+    """`wide`: a table with columns for long sequences, for which the rows are cut into parts."""
     from fastdms_b200.layers.paged_attention import paged_prefill_attention
     rng = np.random.default_rng(len(seqs) + group + d + bs)
     (dv, host), cu, q = _prefill(dev, rng, seqs, heads, group, bs, d, dt, layout)
+    if wide:
+        dv = (*dv[:4], wide_table(dv[4], bs))
     out = torch.full(q.shape, 3.0, dtype=DT[dt], device=dev)
     lse = torch.full((heads * group, q.shape[0]), 7.0, device=dev)
     got = paged_prefill_attention(q.to(dev), *dv, i32([m for _, m in seqs], dev), i32(cu, dev), out=out, lse_out=lse)
@@ -523,13 +528,16 @@ def test_prefill_of_many_sequences(dev):
     check_prefill(n64(got), None, n64(q), cu, seqs, host, 1, 4, 16, 64, "bf16")
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("d", [64, 128])
-def test_prefill_does_not_see_what_is_masked(dev, d):
+def test_prefill_does_not_see_what_is_masked(dev, d, wide):
     """NaN codes and NaN queries reach exactly the rows that see them."""
     from fastdms_b200.layers.paged_attention import paged_prefill_attention
     rng = np.random.default_rng(d)
     n, heads, group, bs = 150, 1, 2, 16
     (dv, host), cu, q = _prefill(dev, rng, [(n, n)], heads, group, bs, d, "bf16", "hnd", pad=0)
+    if wide:
+        dv = (*dv[:4], wide_table(dv[4], bs))
     kc, vc, ks, vs, table = dv
     clean = n64(paged_prefill_attention(q.to(dev), *dv, i32([n], dev), i32(cu, dev)))
     v2 = vc.clone()
