@@ -9,7 +9,8 @@
 //
 // Codes are converted to f16 (exact) in registers.  A query row is brought to a power of two of its own before it goes to
 // f16 (largest element in [2^14, 2^15)), so that bf16's range does not matter: elements that lose bits there are below
-// 2^-28 of the row's largest.  P is rounded to f16, 2^-12 of a weight at most; scores, M, l and the output are float32.
+// 2^-28 of the row's largest.  P is rounded to f16, off by 2^-11 of a weight at most (for f16 outputs the
+// rest of a weight is a second f16 operand); scores, M, l and the output are float32.
 #pragma once
 
 #include <atomic>

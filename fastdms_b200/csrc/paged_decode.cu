@@ -162,9 +162,10 @@ __device__ __forceinline__ void page_scores(const PageRegs<D>& p, const uint32_t
 
 // Scores to weights, l, and P^T; `rows` of the page count.  M follows the maximum only when that is ahead by more than 2^8:
 // P stays below 256 and most pages need no maximum over the keys and rescale nothing.
-template <int D>
+// With FINE, for f16 outputs, whose own rounding is no larger than that of a weight to f16, also what that rounding left.
+template <int D, bool FINE>
 __device__ __forceinline__ void page_weights(UnitState<D>& u, float (&s)[4], float ks, float lvs, float ivs, const float (&factor)[2], int rows,
-                                             int lane, uint32_t& b0, uint32_t& b1) {
+                                             int lane, uint32_t (&b)[4]) {
     const int g = lane >> 2;
     const float f0 = ks * factor[0], f1 = ks * factor[1];
     float x[4] = {fmaf(s[0], f0, lvs), fmaf(s[1], f1, lvs), fmaf(s[2], f0, lvs), fmaf(s[3], f1, lvs)};
@@ -194,13 +195,19 @@ __device__ __forceinline__ void page_weights(UnitState<D>& u, float (&s)[4], flo
     x[3] = paged_ex2(x[3] - r1);
     u.l[0] = fmaf(x[0] + x[2], ivs, u.l[0]);
     u.l[1] = fmaf(x[1] + x[3], ivs, u.l[1]);
-    b0 = transpose_8x8(f16x2_of(x[0], x[1]));
-    b1 = transpose_8x8(f16x2_of(x[2], x[3]));
+    const uint32_t p0 = f16x2_of(x[0], x[1]), p1 = f16x2_of(x[2], x[3]);
+    b[0] = transpose_8x8(p0);
+    b[1] = transpose_8x8(p1);
+    if (FINE) {
+        const __half2 h0 = *(const __half2*)&p0, h1 = *(const __half2*)&p1;
+        b[2] = transpose_8x8(f16x2_of(x[0] - __low2float(h0), x[1] - __high2float(h0)));
+        b[3] = transpose_8x8(f16x2_of(x[2] - __low2float(h1), x[3] - __high2float(h1)));
+    }
 }
 
 // O^T of a page.
-template <int D>
-__device__ __forceinline__ void page_values(UnitState<D>& u, const PageRegs<D>& p, uint32_t b0, uint32_t b1) {
+template <int D, bool FINE>
+__device__ __forceinline__ void page_values(UnitState<D>& u, const PageRegs<D>& p, const uint32_t (&b)[4]) {
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) {
         const uint32_t k0 = v_word<D>(p, 0, w), k1 = v_word<D>(p, 1, w), k2 = v_word<D>(p, 2, w), k3 = v_word<D>(p, 3, w);
@@ -210,7 +217,10 @@ __device__ __forceinline__ void page_values(UnitState<D>& u, const PageRegs<D>& 
         e4m3x4_f16(__byte_perm(k2, k3, 0x5140), a[0][2], a[0][3]);
         e4m3x4_f16(__byte_perm(k2, k3, 0x7362), a[1][2], a[1][3]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mma_16816(u.o[2 * w + j], a[j][0], a[j][1], a[j][2], a[j][3], b0, b1);
+        for (int j = 0; j < 2; ++j) {
+            mma_16816(u.o[2 * w + j], a[j][0], a[j][1], a[j][2], a[j][3], b[0], b[1]);
+            if (FINE) mma_16816(u.o[2 * w + j], a[j][0], a[j][1], a[j][2], a[j][3], b[2], b[3]);
+        }
     }
 }
 
@@ -224,7 +234,7 @@ __device__ __forceinline__ int entry_ahead(const PagedCache& c, int seq, int fir
 // The warp's pages first, first + step, ... (`count` of them) of a sequence's KV head, whose first `len` rows count.  Their
 // table entries and scales are held 32 pages at a time, one per lane: `entry` are the first 32, the next are requested while
 // these are walked.
-template <int D>
+template <int D, bool FINE>
 __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u, const uint32_t (&qb)[D / 16][2], const float (&factor)[2],
                                            int seq, int head, int first, int step, int count, int len, int entry) {
     if (c.num_blocks == 0 || count <= 0) return;
@@ -266,10 +276,10 @@ __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u,
         float s[4];
         page_scores<D>(pg, qb, s);
         if (more) fetch_k(then, i + 1);
-        uint32_t b0, b1;
-        page_weights<D>(u, s, __shfl_sync(0xffffffffu, ks, j), __shfl_sync(0xffffffffu, lvs, j), __shfl_sync(0xffffffffu, ivs, j), factor, rows, lane, b0, b1);
+        uint32_t b[4];
+        page_weights<D, FINE>(u, s, __shfl_sync(0xffffffffu, ks, j), __shfl_sync(0xffffffffu, lvs, j), __shfl_sync(0xffffffffu, ivs, j), factor, rows, lane, b);
         if (rows < kCachePage) mask_v<D>(pg, rows, t);
-        page_values<D>(u, pg, b0, b1);
+        page_values<D, FINE>(u, pg, b);
         if (more) fetch_v(then, i + 1);
         blk = then;
         if (j == 31) {
@@ -384,7 +394,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
     load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
     UnitState<D> st;
     clear<D>(st);
-    walk_pages<D>(a.c, st, qb, factor, seq, head, first, step, first < pages ? (pages - first + step - 1) / step : 0, len, entry);
+    walk_pages<D, !BF16>(a.c, st, qb, factor, seq, head, first, step, first < pages ? (pages - first + step - 1) / step : 0, len, entry);
     put_state<D>(s, st, nh);
     __syncthreads();
     float acc[D / 32], m, l;
@@ -491,7 +501,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
         UnitState<D> st;
         clear<D>(st);
-        walk_pages<D>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len, entry);
+        walk_pages<D, !BF16>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len, entry);
         put_state<D>(s, st, nh);
         __syncthreads();
         const bool whole = p0 == 0 && p1 == pages;

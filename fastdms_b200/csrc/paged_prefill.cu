@@ -193,9 +193,10 @@ __device__ __forceinline__ void exponents(const uint32_t (&s)[32], float factor,
         for (int i = 0; i < 16; ++i) x[i] = pair(2 * i > seen ? -INFINITY : low(x[i]), 2 * i + 1 > seen ? -INFINITY : high(x[i]));
     }
 }
-// Weights of 32 scores as f16 and their sums over each of the two pages.
+// Weights of 32 scores as f16 and their sums over each of the two pages; with FINE also what the rounding to f16 left.
+template <bool FINE>
 __device__ __forceinline__ void weigh(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, float m, bool cut, int seen,
-                                      uint32_t (&p)[16], float& sum0, float& sum1) {
+                                      uint32_t (&p)[16], uint32_t (&rest)[16], float& sum0, float& sum1) {
     uint64_t x[16];
     exponents(s, factor, p0, p1, m == -INFINITY ? 0.0f : m, cut, seen, x);
 #pragma unroll
@@ -203,6 +204,11 @@ __device__ __forceinline__ void weigh(const uint32_t (&s)[32], float factor, con
         const float e = paged_ex2(low(x[i])), f = paged_ex2(high(x[i]));
         x[i] = pair(e, f);
         p[i] = f16x2_of(e, f);
+        if (FINE) {
+            const __half2 h = *(const __half2*)&p[i];
+            const uint64_t left = add2(x[i], pair(-__low2float(h), -__high2float(h)));
+            rest[i] = f16x2_of(low(left), high(left));
+        }
     }
 #pragma unroll
     for (int n = 4; n > 0; n >>= 1)
@@ -296,13 +302,17 @@ __device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int t
     tc_commit(&sh.s_full[ti][buf]);
     tc_commit(&sh.k_empty[st]);
 }
-template <int D>
+template <int D, bool FINE>
 __device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, bool add, PrefillShared& sh) {
     using L = PrefillSmem<D>;
     const uint64_t v = operand(base + L::kV + st * L::kTile + h * (kHalf * 128), kSlab, 1024);
 #pragma unroll
     for (int i = 0; i < kHalf / 16; ++i)
         mma_ts(tmem + L::kO + D * ti, tmem + (L::kBufs * ti + buf) * kHalf + 8 * i, v + (i * 2048 >> 4), instruction(D, true), i > 0 || add);
+    if (FINE)
+#pragma unroll
+        for (int i = 0; i < kHalf / 16; ++i)
+            mma_ts(tmem + L::kO + D * ti, tmem + (L::kBufs * ti + buf) * kHalf + 32 + 8 * i, v + (i * 2048 >> 4), instruction(D, true), true);
     tc_commit(&sh.pv_done[ti][buf]);
     tc_commit(&sh.v_empty[st]);
 }
@@ -334,6 +344,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
     const int64_t open = max(shift + first + 1, (int64_t)0);
     uint8_t* tile = (uint8_t*)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023);
     using L = PrefillSmem<D>;
+    // A weight in f16 is 2^-12 off on the average, as much as the rounding of an f16 output: there the rest of each weight
+    // goes through a product of its own.
+    constexpr bool kFine = !BF16;
 
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&sh.tmem)), "r"(kTmemCols) : "memory");
@@ -431,13 +444,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             uint32_t sc[2][32];
             tmem_load(s_at, sc[0]);
             tmem_load(s_at + 32, sc[1]);
+            uint32_t rest[2][16];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 tc_wait_ld(sc[c]);
                 const float4 p0 = page[2 * c], p1 = page[2 * c + 1];
                 uint32_t p[16];
                 float sum0, sum1;
-                weigh(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, sum0, sum1);
+                weigh<kFine>(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, rest[c], sum0, sum1);
                 const bool moves = m == -INFINITY || sum0 + sum1 > kMostWeight;         // rows do not follow their neighbours
                 if (__any_sync(0xffffffffu, moves)) {
                     if (c == 0) tc_wait_ld(sc[1]);
@@ -455,11 +469,23 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     }
                     tc_wait_st();
                     for (int e = 0; e < 2 * c; ++e) rescale_p(s_at + 8 * e, r);
-                    weigh(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, sum0, sum1);
+                    if (kFine && c == 1) {
+                        const __half2 h = __float2half2_rn(r);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const __half2 y = __hmul2(*(const __half2*)&rest[0][i], h);
+                            rest[0][i] = *(const uint32_t*)&y;
+                        }
+                    }
+                    weigh<kFine>(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, rest[c], sum0, sum1);
                 }
                 tmem_store(s_at + 16 * c, p);
                 l = fmaf(sum0, p0.z, l);
                 l = fmaf(sum1, p1.z, l);
+            }
+            if (kFine) {                        // over scores that are not needed any more
+                tmem_store(s_at + 32, rest[0]);
+                tmem_store(s_at + 48, rest[1]);
             }
             tc_wait_st();
             tc_fence_before();
@@ -655,8 +681,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (!ok) break;
             tc_fence_after();
             if (elected()) {
-                if (h & 2) { if (h & 1) issue_values<D>(base, t0, ti, 1, 1, buf, true, sh); else issue_values<D>(base, t0, ti, 1, 0, buf, true, sh); }
-                else { if (h & 1) issue_values<D>(base, t0, ti, 0, 1, buf, true, sh); else issue_values<D>(base, t0, ti, 0, 0, buf, h > 0, sh); }
+                if (h & 2) { if (h & 1) issue_values<D, kFine>(base, t0, ti, 1, 1, buf, true, sh); else issue_values<D, kFine>(base, t0, ti, 1, 0, buf, true, sh); }
+                else { if (h & 1) issue_values<D, kFine>(base, t0, ti, 0, 1, buf, true, sh); else issue_values<D, kFine>(base, t0, ti, 0, 0, buf, h > 0, sh); }
             }
             __syncwarp();
             const int next = h + L::kBufs;
