@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
 // memory; in small steps, where one token per block is the rule, a warp takes the whole block.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kStoreWarps = 8;
-constexpr int64_t kStoreSmall = 1024;           // tokens
+constexpr int64_t kStoreSmall = 512;            // tokens
 constexpr int kScaleExpMin = -60, kScaleExpMax = 40;
 
 struct StoreArgs {
@@ -469,8 +469,9 @@ static int32_t block_shift(int64_t block_size) {
     return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
 }
 
-// One CTA does all of a decode step in one launch.  Beyond kFusedTokens its writes are what takes time, and a second
-// launch spreads them over the GPU.
+// One CTA does all of a decode step in one launch (256 requests: 5.6 us).  Beyond kFusedTokens its writes are what takes time,
+// and a second launch spreads them over the GPU: 2 K tokens take 5.0 us with one and 5.7 with two, 8 K 8.1 and 5.7, 16 K 12
+// and 5.7; the second launch and its workspace cost 6 us of host time.
 constexpr int64_t kFusedTokens = 4 * kScanThreads * kFillTokens;
 static bool metadata_fused(int64_t num_seqs, int64_t total_tokens) { return num_seqs <= kFusedRequests && total_tokens <= kFusedTokens; }
 
@@ -552,18 +553,20 @@ extern "C" int32_t fdms_paged_store(const fdms_paged_store_args* args, void* str
     const uintptr_t act = (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)(2 * (p.k_stride[0] | p.k_stride[1] | p.v_stride[0] | p.v_stride[1]));
     FDMS_REQUIRE((act & 15) == 0 && p.k_stride[2] == 1 && p.v_stride[2] == 1, FDMS_E_ARG,
                  "fdms_paged_store: key and value must be contiguous in their last dimension and aligned to 16 bytes in the others");
-    // Small steps: a warp per (run, head); large ones: one per 16 rows of it.
+    // Small steps: a warp per (run, head); large ones: one per 16 rows of it.  256 tokens for as many blocks of 64 take 4.9 us
+    // with the first and 12.9 with the second, 8000 prompt tokens 15.9 and 14.7.
     const int W = p.tokens <= kStoreSmall ? 1 : (int)c.block_size / 16, per_cta = kStoreWarps / W;
-    // Tokens per CTA: few runs begin in a prompt's tokens, one at every token of a decode batch.  1024 CTAs keep the GPU
-    // busy either way; more than a block's worth of tokens per CTA would only make them unequal.
+    const int64_t columns = (2 * c.kv_heads + per_cta - 1) / per_cta;
+    // Tokens per CTA: a run begins at every token of a decode batch, but only once in a block of a prompt, and a CTA without one
+    // is not free: at most 32 tokens, a block's worth, until the CTAs are two rounds of what the GPU holds.
     int group = 1;
-    while (group < 16 && p.tokens > (int64_t)group * 1024) group *= 2;
+    while (group < (c.block_size > 16 ? 32 : 16) && (p.tokens + group - 1) / group * columns > 1184) group *= 2;
     StoreArgs a = {{(const uint16_t*)p.k, (const uint16_t*)p.v}, {p.k_stride[0], p.v_stride[0]}, {p.k_stride[1], p.v_stride[1]}, {c.k, c.v},
                    {c.k_stride[0], c.v_stride[0]}, {c.k_stride[1], c.v_stride[1]}, {c.k_stride[2], c.v_stride[2]}, {c.k_scale, c.v_scale},
                    p.slot_mapping, p.dev_status, p.tokens, c.num_blocks << shift, (int32_t)c.kv_heads, shift, group, W};
     const int64_t ctas = (p.tokens + group - 1) / group;
     FDMS_REQUIRE(ctas < (1ll << 31), FDMS_E_CAPACITY, "fdms_paged_store: too many tokens");
-    const dim3 grid((unsigned)ctas, (unsigned)((2 * c.kv_heads + per_cta - 1) / per_cta));
+    const dim3 grid((unsigned)ctas, (unsigned)columns);
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = p.act_dtype == FDMS_BF16;
     if (c.head_dim == 64) {

@@ -575,14 +575,16 @@ static int64_t decode_parts_bytes(int sms, int head_dim) {
 }
 
 // CTAs per unit of the cluster kernel for sequences of up to `rows` rows, 0: the shares.  As many as one wave of the GPU
-// holds, each with a page for every warp; not where a CTA might get more than kClusterPages pages a warp, because then a long
-// sequence among short ones keeps its CTAs while the others are idle.
-constexpr int kClusterPages = 24;
+// holds, each with a page for every warp.  Where a CTA might get more pages a warp than the limit, a long sequence among short
+// ones keeps its CTAs while the others are idle, and where the clusters do not fill the GPU that happens sooner.  Measured
+// (head_dim 128, 8 KV heads, clusters / shares, us): 8 x 1000 rows 8.2 / 14.1, 100 ragged up to 4000 90 / 126, 3 up to 30000
+// 37 / 49, 64 up to 16384 255 / 216; one sequence of 8000 11.5 / 18.6, 24000 24.0 / 22.2, 48000 52 / 31.
+constexpr int kClusterPages = 64, kClusterPagesFew = 24;
 static int decode_cluster(int64_t units, int64_t rows, int sms) {
     const int64_t pages = (rows + kCachePage - 1) / kCachePage;
     int n = 1;
     while (n < 8 && units * n * 2 <= (int64_t)sms * kDecCtasPerSm && pages > (int64_t)n * kDecWarps) n *= 2;
-    return pages <= (int64_t)n * kDecWarps * kClusterPages && units * n < (1ll << 31) ? n : 0;
+    return pages <= (int64_t)n * kDecWarps * (units * n >= sms ? kClusterPages : kClusterPagesFew) && units * n < (1ll << 31) ? n : 0;
 }
 
 extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows) {

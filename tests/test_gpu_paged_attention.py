@@ -334,7 +334,7 @@ DECODE = [
     ([600], 1, 12, 64, 128, "f16", "hnd"), ([9000, 3, 0, 1200], 1, 4, 16, 64, "f16", "hnd"), ([100, 90], 1, 64, 16, 64, "bf16", "hnd")]
 
 
-def wide_table(table, bs, rows=40000):
+def wide_table(table, bs, rows=70000):
     """The same table with columns for long sequences, which the decode kernel for short ones does not take."""
     wide = torch.full((table.shape[0], rows // bs), -1, dtype=torch.int32, device=table.device)
     wide[:, :table.shape[1]] = table
