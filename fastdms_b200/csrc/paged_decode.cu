@@ -4,12 +4,16 @@
 // The work is the cache's bytes, each to be read once.  A unit is a (sequence, KV head), with up to eight of its q heads; the
 // eight warps of a CTA take pages (16 rows) in turn, keep (M, l, O) in registers and merge them through shared memory.
 // Two kernels hand out the pages:
-//   clusters  a cluster of 1 to 8 CTAs per unit, whose parts meet in distributed shared memory: one launch, no workspace.  For
+//   clusters  a cluster of 1 to 16 CTAs per unit, whose parts meet in distributed shared memory: one launch, no workspace.  For
 //             tables that cannot hold long sequences, and for work that is small altogether.
 //   shares    the pages of all units laid end to end, every CTA taking an equal share of them, so that ragged lengths leave
 //             no SM idle and no host has to know a length.  A unit that one CTA holds whole is written at once; parts of a
 //             unit that is cut go to a workspace, and a second launch, started while this one runs, joins them.
 #include "paged_attn.cuh"
+
+#include <algorithm>
+#include <climits>
+#include <mutex>
 
 namespace fdms {
 
@@ -18,6 +22,7 @@ constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecHeads = 8;                    // q heads of a KV head that one unit takes
 constexpr int kDecMaxBatch = 2048;              // prefix sums of the pages live in shared memory
 constexpr int kDecCtasPerSm = 2;
+constexpr int kClusterSizes = 5, kMaxCluster = 1 << (kClusterSizes - 1), kMaxDevices = 64;
 
 struct DecodeArgs {
     PagedCache c;
@@ -302,14 +307,22 @@ __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u,
     }
 }
 
-// Pages before sequence b for all b (and in total), in shared memory; by all threads of the CTA.
-__device__ __forceinline__ void page_prefix(const DecodeArgs& a, int32_t* s_first, int32_t* s_warp) {
+// What a unit costs its CTA before its first page and after its last, in pages: loads that wait for one another and the merge of
+// the warps.  The shares count it, so that short sequences among long ones do not pile up in one CTA: from
+// memory, 24 / 8 / 0 pages, 64 sequences ragged up to 16384 188 / 207 / 213 us, 3 up to 30000 30.5 / 44 / 54; 48 pages was slower again
+// for many short sequences (300 up to 2000 rows 151 against 142).
+constexpr int kUnitPages = 24;
+
+// The weight (a unit's pages and kUnitPages, 0 without rows) of the sequences before b for all b, and in total, in shared memory; by
+// all threads of the CTA.
+__device__ __forceinline__ void weight_prefix(const DecodeArgs& a, int32_t* s_first, int32_t* s_warp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int32_t before = 0;
     for (int base = 0; base < a.batch; base += kDecThreads) {
         const int b = base + threadIdx.x;
         const int pages = b < a.batch ? (int)(((int64_t)paged_len(a.c, b) + kCachePage - 1) / kCachePage) : 0;
-        int sum = pages;
+        const int weight = pages ? pages + kUnitPages : 0;
+        int sum = weight;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, sum, o);
@@ -323,7 +336,7 @@ __device__ __forceinline__ void page_prefix(const DecodeArgs& a, int32_t* s_firs
             if (w < warp) add += s_warp[w];
             total += s_warp[w];
         }
-        if (b < a.batch) s_first[b] = add + sum - pages;
+        if (b < a.batch) s_first[b] = add + sum - weight;
         before += total;
         __syncthreads();
     }
@@ -331,7 +344,7 @@ __device__ __forceinline__ void page_prefix(const DecodeArgs& a, int32_t* s_firs
     __syncthreads();
 }
 
-// The share of CTA `c` of `n` in `total` pages begins at share(c); page x belongs to CTA owner(x).
+// The share of CTA `c` of `n` in a weight of `total` begins at share(c); place x belongs to CTA owner(x).
 __device__ __forceinline__ int64_t share(int64_t c, int64_t n, int64_t total) { return c * total / n; }
 __device__ __forceinline__ int owner(int64_t x, int64_t n, int64_t total) { return (int)(((x + 1) * n - 1) / total); }
 
@@ -422,10 +435,10 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp < nh && warp % a.cluster == rank) {                // heads are shared out among the cluster's CTAs
         const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&s_part[warp][0]);
-        float pm[8], pl[8];
+        float pm[kMaxCluster], pl[kMaxCluster];
         m = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+        for (int r = 0; r < kMaxCluster; ++r) {
             pm[r] = -INFINITY;
             pl[r] = 0.0f;
             if (r < a.cluster) {
@@ -440,7 +453,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < kMaxCluster; ++r)
             if (r < a.cluster) {
                 uint32_t at;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + lane * (D / 8)), "r"(r));
@@ -468,11 +481,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
     __shared__ MergeSmem<D> s;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     pdl_trigger();
-    page_prefix(a, s_first, s_warp);
+    weight_prefix(a, s_first, s_warp);
     const int per_seq = a.c.heads * a.splits;
     const int64_t total = (int64_t)s_first[a.batch] * per_seq;
     // fewer CTAs than the grid has where there are not two pages for each warp
-    const int64_t ctas = min((int64_t)gridDim.x, max((int64_t)1, (total + 2 * kDecWarps - 1) / (2 * kDecWarps)));
+    const int64_t ctas = min((int64_t)gridDim.x, max((int64_t)1, total / (2 * kDecWarps + kUnitPages)));
     if (blockIdx.x == 0) {                      // sequences without rows: zeros
         for (int b = warp; b < a.batch; b += kDecWarps) {
             if (s_first[b + 1] != s_first[b]) continue;
@@ -486,7 +499,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
     }
     if (blockIdx.x >= ctas) return;
     const int64_t begin = share(blockIdx.x, ctas, total), end = share((int64_t)blockIdx.x + 1, ctas, total);
-    int seq = 0;                                // last sequence whose pages begin at or before `begin`, and has any
+    int seq = 0;                                // last sequence that begins at or before `begin`, and has any weight
     {
         int lo = 0, hi = a.batch;
         while (lo < hi) {
@@ -498,11 +511,15 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
     int64_t at = begin;
     while (at < end) {
         while ((int64_t)s_first[seq + 1] * per_seq <= at) ++seq;
-        const int pages = s_first[seq + 1] - s_first[seq];
+        const int weight = s_first[seq + 1] - s_first[seq], pages = weight - kUnitPages;
         const int64_t seq_begin = (int64_t)s_first[seq] * per_seq;
-        const int u = (int)((at - seq_begin) / pages);          // unit of the sequence
-        const int64_t unit_begin = seq_begin + (int64_t)u * pages;
-        const int p0 = (int)(at - unit_begin), p1 = (int)min((int64_t)pages, end - unit_begin);
+        const int u = (int)((at - seq_begin) / weight);         // unit of the sequence
+        const int64_t unit_begin = seq_begin + (int64_t)u * weight, unit_end = unit_begin + weight;
+        const int64_t from = at;
+        at = min(unit_end, end);
+        // page p lies at unit_begin + kUnitPages + p; a share that ends before the first page leaves the unit to the next CTA
+        const int p0 = (int)max((int64_t)0, from - unit_begin - kUnitPages), p1 = (int)(at - unit_begin) - kUnitPages;
+        if (p1 <= 0) break;
         const int head = u / a.splits, h0 = (u % a.splits) * kDecHeads, nh = min(kDecHeads, a.group - h0);
         const int len = min(paged_len(a.c, seq), pages * kCachePage);
         const int entry = entry_ahead(a.c, seq, p0 + warp, kDecWarps, 0);
@@ -515,7 +532,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         put_state<D>(s, st, nh);
         __syncthreads();
         const bool whole = p0 == 0 && p1 == pages;
-        const int slot = blockIdx.x * 2 + (at == begin ? 0 : 1);
+        const int slot = blockIdx.x * 2 + (from == begin ? 0 : 1);
         if (warp < nh) {
             float acc[D / 32], m, l;
             merge_warps<D>(s, acc, m, l);
@@ -528,11 +545,10 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
             }
         }
         if (p0 == 0 && threadIdx.x == 0) {
-            const int2 cut = whole ? make_int2(0, -1) : make_int2(slot, owner(unit_begin + pages - 1, ctas, total));
+            const int2 cut = whole ? make_int2(0, -1) : make_int2(slot, owner(unit_end - 1, ctas, total));
             a.cuts[(int64_t)seq * per_seq + u] = cut;
         }
         __syncthreads();
-        at = unit_begin + p1;
     }
 }
 
@@ -584,17 +600,71 @@ static int64_t decode_parts_bytes(int sms, int head_dim) {
     return (int64_t)sms * kDecCtasPerSm * 2 * kDecHeads * (head_dim + 4) * (int64_t)sizeof(float);
 }
 
+using ClusterKernel = void (*)(DecodeArgs);
+static ClusterKernel cluster_kernel(int head_dim, bool bf16) {
+    return head_dim == 64 ? (bf16 ? paged_decode_cluster_kernel<64, true> : paged_decode_cluster_kernel<64, false>)
+                          : (bf16 ? paged_decode_cluster_kernel<128, true> : paged_decode_cluster_kernel<128, false>);
+}
+static void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, int64_t ctas, int cluster, cudaStream_t stream) {
+    cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kDecThreads);
+    cfg.stream = stream;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+}
+// How many clusters of 2^i CTAs the current device holds at once, the least over the kernel's forms; 0 where it takes none.  The
+// SMs of a partition that do not make up a cluster stay empty, so that wide clusters hold fewer CTAs than the SMs would.
+struct ClusterRoom {
+    int held[kClusterSizes];
+};
+static ClusterRoom read_cluster_room() {
+    ClusterRoom room;
+    for (int i = 0; i < kClusterSizes; ++i) {
+        room.held[i] = INT_MAX;
+        for (int form = 0; form < 4; ++form) {
+            ClusterKernel kern = cluster_kernel(form & 1 ? 64 : 128, (form & 2) != 0);
+            cudaLaunchConfig_t cfg;
+            cudaLaunchAttribute attr;
+            cluster_config(cfg, attr, 1 << i, 1 << i, nullptr);
+            int n = 0;
+            if ((i > 3 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+                cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            room.held[i] = std::min(room.held[i], n);
+        }
+    }
+    return room;
+}
+static const ClusterRoom& cluster_room() {
+    static ClusterRoom rooms[kMaxDevices];
+    static std::once_flag once[kMaxDevices];
+    static const ClusterRoom none = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return none;
+    std::call_once(once[dev], [dev] { rooms[dev] = read_cluster_room(); });
+    return rooms[dev];
+}
+
 // CTAs per unit of the cluster kernel for sequences of up to `rows` rows, 0: the shares.  As many as one wave of the GPU
-// holds, each with a page for every warp.  Where a CTA might get more pages a warp than the limit, a long sequence among short
-// ones keeps its CTAs while the others are idle, and where the clusters do not fill the GPU that happens sooner.  Measured
-// (head_dim 128, 8 KV heads, clusters / shares, us): 8 x 1000 rows 8.2 / 14.1, 100 ragged up to 4000 90 / 126, 3 up to 30000
-// 37 / 49, 64 up to 16384 255 / 216; one sequence of 8000 11.5 / 18.6, 24000 24.0 / 22.2, 48000 52 / 31.
-constexpr int kClusterPages = 64, kClusterPagesFew = 24;
+// holds, each with a page for every warp.  The clusters save the join and the walk over all lengths, but a long sequence among
+// short ones keeps its CTAs while others are idle, the more so the fewer waves follow; so the pages that a warp may get are
+// limited, by the waves.  Measured (head_dim 128, 8 KV heads, from memory, clusters / shares, us): one sequence of 2000 rows 7.7 / 12.4,
+// 8000 11.2 / 14.2, 24000 23.8 / 25.9, 48000 39.0 / 34.8; 5 ragged up to 8000 24.5 / 19.2, 16 up to 3000 21.4 / 20.1 (all of 3000
+// 24.4 / 29.0), 64 up to 1000 24.5 / 27.0, 64 up to 3000 53.7 / 49.2, 100 up to 4000 89 / 88, 600 up to 1000 156 / 172.
+constexpr int kClusterPages = 12, kClusterWaves = 4;
 static int decode_cluster(int64_t units, int64_t rows, int sms) {
-    const int64_t pages = (rows + kCachePage - 1) / kCachePage;
+    const int64_t pages = (rows + kCachePage - 1) / kCachePage, wave = (int64_t)sms * kDecCtasPerSm;
+    const ClusterRoom& room = cluster_room();
     int n = 1;
-    while (n < 8 && units * n * 2 <= (int64_t)sms * kDecCtasPerSm && pages > (int64_t)n * kDecWarps) n *= 2;
-    return pages <= (int64_t)n * kDecWarps * (units * n >= sms ? kClusterPages : kClusterPagesFew) && units * n < (1ll << 31) ? n : 0;
+    for (int i = 1; i < kClusterSizes && units <= room.held[i] && pages > (int64_t)n * kDecWarps; ++i) n *= 2;
+    const int64_t work = std::min(std::max(units * n, wave), wave * kClusterWaves);
+    return pages * wave <= work * n * kDecWarps * kClusterPages && units * n < (1ll << 31) ? n : 0;
 }
 
 extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows) {
@@ -637,18 +707,10 @@ extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void
     a.parts = nullptr;
     a.cuts = nullptr;
     if (a.cluster) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(units * a.cluster));
-        cfg.blockDim = dim3(kDecThreads);
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)a.cluster;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (head_dim == 64) FDMS_CUDA_OK(cudaLaunchKernelEx(&cfg, bf ? paged_decode_cluster_kernel<64, true> : paged_decode_cluster_kernel<64, false>, a));
-        else FDMS_CUDA_OK(cudaLaunchKernelEx(&cfg, bf ? paged_decode_cluster_kernel<128, true> : paged_decode_cluster_kernel<128, false>, a));
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr;
+        cluster_config(cfg, attr, units * a.cluster, a.cluster, st);
+        FDMS_CUDA_OK(cudaLaunchKernelEx(&cfg, cluster_kernel(head_dim, bf), a));
         FDMS_CHECK_LAUNCH("paged_decode_cluster_kernel");
         return FDMS_OK;
     }

@@ -331,7 +331,11 @@ DECODE = [
     ([0], 2, 2, 16, 128, "bf16", "hnd"), ([0, 0, 0], 1, 4, 32, 64, "bf16", "hnd"),
     ([201], 8, 4, 16, 128, "f16", "hnd"), ([300, 1, 33, 512], 2, 7, 32, 128, "bf16", "layers"), ([777], 1, 3, 64, 64, "bf16", "nhd"),
     ([129, 128, 127, 1], 4, 5, 128, 128, "f16", "hnd"), ([64] * 40, 2, 2, 16, 64, "bf16", "hnd"), ([2500, 40], 1, 16, 16, 64, "bf16", "hnd"),
-    ([600], 1, 12, 64, 128, "f16", "hnd"), ([9000, 3, 0, 1200], 1, 4, 16, 64, "f16", "hnd"), ([100, 90], 1, 64, 16, 64, "bf16", "hnd")]
+    ([600], 1, 12, 64, 128, "f16", "hnd"), ([9000, 3, 0, 1200], 1, 4, 16, 64, "f16", "hnd"), ([100, 90], 1, 64, 16, 64, "bf16", "hnd"),
+    # the widest clusters; and, from wide tables, sequences of which many begin and end in one share, next to one that fills many
+    ([15000], 2, 3, 16, 128, "bf16", "hnd"), ([15001, 1], 1, 8, 32, 64, "f16", "nhd"),
+    ([1] * 30 + [15000, 0] + [40] * 9 + [390, 0, 380, 400, 0], 2, 2, 16, 128, "bf16", "hnd"),
+    ([3000, 2] * 10, 2, 4, 64, 64, "f16", "hnd")]
 
 
 def wide_table(table, bs, rows=70000):
