@@ -656,15 +656,17 @@ static const ClusterRoom& cluster_room() {
 // short ones keeps its CTAs while others are idle, the more so the fewer waves follow; so the pages that a warp may get are
 // limited, by the waves.  Measured (head_dim 128, 8 KV heads, from memory, clusters / shares, us): one sequence of 2000 rows 7.7 / 12.4,
 // 8000 11.2 / 14.2, 24000 23.8 / 25.9, 48000 39.0 / 34.8; 5 ragged up to 8000 24.5 / 19.2, 16 up to 3000 21.4 / 20.1 (all of 3000
-// 24.4 / 29.0), 64 up to 1000 24.5 / 27.0, 64 up to 3000 53.7 / 49.2, 100 up to 4000 89 / 88, 600 up to 1000 156 / 172.
-constexpr int kClusterPages = 12, kClusterWaves = 4;
-static int decode_cluster(int64_t units, int64_t rows, int sms) {
+// 24.4 / 29.0), 64 up to 1000 24.5 / 27.0, 64 up to 3000 53.7 / 49.2, 100 up to 4000 89 / 88, 600 up to 1000 156 / 172.  At head_dim 64 a
+// page is half the work: 8 of 8192 20.0 / 23.4, 8 ragged up to 8192 18.2 / 18.4 and up to 10000 21.1 / 19.6, 2 of 24000 25.7 / 21.9.
+constexpr int kClusterWaves = 4;
+static int decode_cluster(int64_t units, int64_t rows, int64_t head_dim, int sms) {
+    const int64_t most = head_dim == 64 ? 20 : 12;      // pages of a warp in a wave
     const int64_t pages = (rows + kCachePage - 1) / kCachePage, wave = (int64_t)sms * kDecCtasPerSm;
     const ClusterRoom& room = cluster_room();
     int n = 1;
     for (int i = 1; i < kClusterSizes && units <= room.held[i] && pages > (int64_t)n * kDecWarps; ++i) n *= 2;
     const int64_t work = std::min(std::max(units * n, wave), wave * kClusterWaves);
-    return pages * wave <= work * n * kDecWarps * kClusterPages && units * n < (1ll << 31) ? n : 0;
+    return pages * wave <= work * n * kDecWarps * most && units * n < (1ll << 31) ? n : 0;
 }
 
 extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows) {
@@ -672,7 +674,7 @@ extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t
     const int sms = paged_sms();
     if (sms <= 0) return -1;
     const int64_t units = batch * num_kv_heads * ((num_q_heads / num_kv_heads + kDecHeads - 1) / kDecHeads);
-    return decode_cluster(units, max_rows, sms) ? 0 : decode_parts_bytes(sms, (int)head_dim) + units * (int64_t)sizeof(int2);
+    return decode_cluster(units, max_rows, head_dim, sms) ? 0 : decode_parts_bytes(sms, (int)head_dim) + units * (int64_t)sizeof(int2);
 }
 
 extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream) {
@@ -703,7 +705,7 @@ extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = p.dtype == FDMS_BF16;
     const int64_t units = (int64_t)batch * num_kv_heads * a.splits;
-    a.cluster = decode_cluster(units, p.max_blocks * p.cache.block_size, sms);
+    a.cluster = decode_cluster(units, p.max_blocks * p.cache.block_size, head_dim, sms);
     a.parts = nullptr;
     a.cuts = nullptr;
     if (a.cluster) {
