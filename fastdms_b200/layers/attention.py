@@ -110,6 +110,8 @@ class Attention(nn.Module):
             raise RuntimeError("dense paged attention requires the layer's k_cache, v_cache and their scales")
         if context.slot_mapping is None or context.context_lens is None:
             raise RuntimeError("dense paged attention requires slot_mapping and context_lens")
+        if context.is_prefill and context.cu_seqlens_q is None:
+            raise RuntimeError("dense paged prefill requires cu_seqlens_q")
         cache = (self.k_cache, self.v_cache, self.k_cache_scale, self.v_cache_scale)
         with prof.cuda_phase("paged_store"):
             store_paged_kvcache(k, v, *cache, context.slot_mapping)

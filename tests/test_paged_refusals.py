@@ -157,6 +157,25 @@ def test_c_release_refuses():
     assert lib.fdms_paged_release(*(rel | dict(listed=0)).values()) == _lib.FDMS_OK and lib.fdms_last_error() == b""
 
 
+def test_layer_refuses_incomplete_contexts():
+    from fastdms_b200.layers.attention import Attention
+    from fastdms_b200.utils.context import reset_context, set_context
+    layer = Attention(4, 64, 0.125, 2)
+    q, k = torch.zeros((3, 4, 64), dtype=torch.bfloat16), torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+    step = dict(block_tables=torch.zeros((1, 2), dtype=torch.int32), slot_mapping=ints(0, 1, 2), context_lens=ints(3), cu_seqlens_q=ints(0, 3))
+    try:
+        set_context(True, **step)
+        with pytest.raises(RuntimeError, match="k_cache"):
+            layer(q, k, k)
+        layer.k_cache, layer.v_cache, layer.k_cache_scale, layer.v_cache_scale = cache()
+        for missing in ("slot_mapping", "context_lens", "cu_seqlens_q"):
+            set_context(True, **(step | {missing: None}))
+            with pytest.raises(RuntimeError, match=missing):
+                layer(q, k, k)
+    finally:
+        reset_context()
+
+
 def test_plain_statement():
     """The oracle's codes are torch's: every value that is one, values around every border, ties."""
     v = O.VALUES[np.isfinite(O.VALUES)]
