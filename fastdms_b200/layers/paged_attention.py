@@ -167,9 +167,6 @@ def build_paged_metadata(
     device = kv_lens.device
     kv_lens_out = kv_lens if kv_lens_out is None else kv_lens_out
     free_count_out = free_count if free_count_out is None else free_count_out
-    new_ptr, kv_out_ptr = new_lens.data_ptr(), kv_lens_out.data_ptr()
-    if new_ptr == kv_out_ptr and n > 0:
-        raise ValueError("the advanced kv_lens would overwrite new_lens")
     if cu_seqlens is None:
         cu_seqlens = kv_lens.new_empty(n + 1)
     if slot_mapping is None:
@@ -179,7 +176,7 @@ def build_paged_metadata(
     need = _lib.lib().fdms_paged_metadata_workspace_bytes(n, total_tokens)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch(_lib.lib().fdms_paged_metadata, _METADATA_ARGS.pack(
-        new_ptr, kv_lens.data_ptr(), kv_out_ptr, block_tables.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(),
+        new_lens.data_ptr(), kv_lens.data_ptr(), kv_lens_out.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(),
         free_count_out.data_ptr(), cu_seqlens.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), ws.data_ptr() if need else 0,
         _lib.status_word(device).data_ptr(), n, cols, stride, block_size, free_blocks.numel(), total_tokens, need), dev)
     return cu_seqlens, slot_mapping, positions
