@@ -3,14 +3,18 @@
 //
 // With x_j = scale * log2(e) * ks_j * (q . kcode_j) the output of a row is sum_j 2^x_j vs_j vcode_j / sum_j 2^x_j.  The
 // scales never touch the codes: ks_j multiplies a score, and vs_j is a power of two that goes into the exponent,
-//   M = max_j (x_j + log2 vs_j),  P_j = 2^(x_j + log2 vs_j - M) <= 1,  out = sum_j P_j vcode_j / l,  l = sum_j P_j / vs_j,
+//   P_j = 2^(x_j + log2 vs_j - M),  out = sum_j P_j vcode_j / l,  l = sum_j P_j / vs_j,
 // so that P is always fit for 16 bits whatever the blocks' magnitudes are, and a block with small values does not
 // disturb one with large ones.  Scales lie in [2^-60, 2^40] (what the store writes), which keeps l inside float32.
+// M is set so that the weights so far lie well above 1 (decode: the largest at 2^11; prefill: the sum of 32 at 2^7 to 2^8) and
+// follows them only when one might leave f16: P stays at or below 2^15 in decode, below 61440 in prefill.  So far above
+// 1, because f16 has no finer step than 2^-24: what rounds to zero lies below 2^-32 of the weights it stands beside, and the quiet
+// keys of a long row count behind a loud one.
 //
 // Codes are converted to f16 (exact) in registers.  A query row is brought to a power of two of its own before it goes to
 // f16 (largest element in [2^14, 2^15)), so that bf16's range does not matter: elements that lose bits there are below
-// 2^-28 of the row's largest.  P is rounded to f16, off by 2^-11 of a weight at most (for f16 outputs the
-// rest of a weight is a second f16 operand); scores, M, l and the output are float32.
+// 2^-28 of the row's largest.  P is rounded to f16, off by 2^-11 of a weight or by 2^-25 at most (for f16 outputs the
+// rest of a weight is a second f16 operand: 2^-22 or 2^-25); scores, M, l and the output are float32.
 #pragma once
 
 #include <atomic>

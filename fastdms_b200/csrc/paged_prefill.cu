@@ -183,7 +183,11 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[8]
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), FDMS_W8(r, 0) : "memory");
 }
 
-constexpr float kMostWeight = 16384.0f;         // a sum of weights below this keeps each inside f16
+constexpr float kMostWeight = 61440.0f;         // a sum of weights below this keeps each inside f16
+// log2 of what the sum of 32 weights is brought to, or up to a half below, when M is set.  Higher keeps more of the weights that f16
+// cannot hold and leaves less room until M has to move again: 2048 tokens over 16384 rows take 568 us with 7 and 571 with 8, 7 ragged
+// prompts 352 and 352 (head_dim 64), 392 and 394 (128).
+constexpr float kSetWeight = 8.0f;
 
 // Exponents of 32 scores: x = s * factor * ks + log2 vs - ref, keys behind `seen` masked.
 __device__ __forceinline__ void exponents(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, float ref, bool cut, int seen,
@@ -224,16 +228,19 @@ __device__ __forceinline__ void weigh(const uint32_t (&s)[32], float factor, con
     sum0 = low(x[0]) + high(x[0]);
     sum1 = low(x[8]) + high(x[8]);
 }
-__device__ __forceinline__ float largest(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, bool cut, int seen) {
+// The rare paths of the softmax, kept out of its loop: the largest exponent of 32 scores; a row of O, or a page of P, times a power
+// of two.
+__device__ __noinline__ float largest(uint32_t at, float factor, const float4* page, int seen) {
+    uint32_t s[32];
     uint64_t x[16];
-    exponents(s, factor, p0, p1, 0.0f, cut, seen, x);
+    tmem_load(at, s);
+    tc_wait_ld(s);
+    exponents(s, factor, page[0], page[1], 0.0f, true, seen, x);
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(low(x[i]), high(x[i])));
     return top;
 }
-
-// The rare path of the softmax, kept out of its loop: a row of O, or a page of P, times a power of two.
 template <int D>
 __device__ __noinline__ void rescale_o(uint32_t at, float r) {
     for (int c = 0; c < D / 16; ++c) {
@@ -245,16 +252,17 @@ __device__ __noinline__ void rescale_o(uint32_t at, float r) {
         tmem_store(at + 16 * c, o);
     }
 }
+// The factor may lie below what f16 holds while the product does not.
+__device__ __forceinline__ uint32_t f16x2_times(uint32_t x, float r) {
+    const __half2 h = *(const __half2*)&x;
+    return f16x2_of(__low2float(h) * r, __high2float(h) * r);
+}
 __device__ __noinline__ void rescale_p(uint32_t at, float r) {
     uint32_t p[8];
     tmem_load(at, p);
     tc_wait_ld(p);
-    const __half2 h = __float2half2_rn(r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const __half2 y = __hmul2(*(__half2*)&p[i], h);
-        p[i] = *(const uint32_t*)&y;
-    }
+    for (int i = 0; i < 8; ++i) p[i] = f16x2_times(p[i], r);
     tmem_store(at, p);
 }
 
@@ -442,9 +450,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             const float4* page = &sh.page[(half >> 1) & (kConstRing - 1)][(half & 1) * (kHalf / kCachePage)];
             const int seen = (int)min(last - (int64_t)half * kHalf, (int64_t)kHalf);         // last key of the half that the row sees
             const bool cut = __any_sync(0xffffffffu, seen < kHalf - 1);
-            // 32 keys at a time.  P takes the columns of scores that have been read.  M follows the maximum only when a
-            // weight might leave f16 (the sum of 32 tells) and is a whole number: O, l and the earlier weights of the half then
-            // follow by an exact factor.  Most keys need no maximum at all.
+            // 32 keys at a time.  P takes the columns of scores that have been read.  M follows the weights only when one
+            // might leave f16 (the sum of 32 tells, and says where M goes) and is a whole number: O, l and the earlier weights of
+            // the half then follow by an exact factor.  Most keys need no maximum at all.
             uint32_t sc[2][32];
             tmem_load(s_at, sc[0]);
             tmem_load(s_at + 32, sc[1]);
@@ -459,10 +467,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                 const bool moves = m == -INFINITY || sum0 + sum1 > kMostWeight;         // rows do not follow their neighbours
                 if (__any_sync(0xffffffffu, moves)) {
                     if (c == 0) tc_wait_ld(sc[1]);
-                    tmem_load(s_at + 32 * c, sc[c]);
-                    tc_wait_ld(sc[c]);
-                    const float top = largest(sc[c], factor, p0, p1, cut, seen - 32 * c);
-                    const float next = moves ? fmaxf(m, ceilf(top)) : m;
+                    const float sum = sum0 + sum1;
+                    const bool known = sum > 0x1p-100f && sum < 0x1p100f;       // else the maximum has to say
+                    float to = (m == -INFINITY ? 0.0f : m) + (float)((int)(__float_as_uint(sum) >> 23) - 126);
+                    if (__any_sync(0xffffffffu, moves && !known)) {
+                        const float top = largest(s_at + 32 * c, factor, page + 2 * c, seen - 32 * c);
+                        if (!known) to = ceilf(top);
+                    }
+                    const float next = moves ? fmaxf(m, to - kSetWeight) : m;
                     const float r = next == m ? 1.0f : paged_ex2(m - next);
                     m = next;
                     l *= r;
@@ -474,13 +486,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     tc_wait_st();
                     for (int e = 0; e < 2 * c; ++e) rescale_p(s_at + 8 * e, r);
                     if (kFine && c == 1) {
-                        const __half2 h = __float2half2_rn(r);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const __half2 y = __hmul2(*(const __half2*)&rest[0][i], h);
-                            rest[0][i] = *(const uint32_t*)&y;
-                        }
+                        for (int i = 0; i < 16; ++i) rest[0][i] = f16x2_times(rest[0][i], r);
                     }
+                    tmem_load(s_at + 32 * c, sc[c]);
+                    tc_wait_ld(sc[c]);
                     weigh<kFine>(sc[c], factor, p0, p1, m, cut, seen - 32 * c, p, rest[c], sum0, sum1);
                 }
                 tmem_store(s_at + 16 * c, p);
