@@ -53,3 +53,29 @@ def test_many_quiet_keys_behind_a_loud_one(dev, form, rows, seqs, dt, wide):
     for r in (got[0, :1], got[seqs - 1, 1:]):
         check_rows(n64(r), n64(lse)[0, :1], want, dt)
     assert (got == got[0, 0]).all()
+
+
+@pytest.mark.parametrize("jump", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("form", ["prefill", "decode"])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_weights_whose_roundings_add_up(dev, form, dt, wide, jump):
+    """Two kinds of keys with V of 1 and -1, all of a kind with the same weight: the roundings of a kind do not cancel while the
+    output nearly does, so that an f16 output shows whether a weight's rest has come along.  With `jump` a key in the
+    second 32 of a step's half is louder by 2^8 or so, and what is there of the first 32 follows M down."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
+    d, rows, heads = 64, 200, 32
+    k, v = np.zeros((rows, d)), np.ones((rows, d))
+    k[::2, 0], k[1::2, 0], v[1::2] = 1.0, 0.9375, -1.0
+    if jump:
+        k[104, 0], v[104] = 2.5, 0.0
+    kc, vc, ks, vs, table = one_sequence(dev, k, v)
+    if wide:
+        table = wide_table(table, 16)
+    q = torch.zeros((1, heads, d), dtype=DT[dt])
+    q[0, :, 0] = torch.linspace(3.5, 4.5, heads)
+    if form == "decode":
+        got = paged_decode_attention(q.to(dev), kc, vc, ks, vs, table, i32([rows], dev), 1.0)
+    else:
+        got = paged_prefill_attention(q.to(dev), kc, vc, ks, vs, table, i32([rows], dev), i32([0, 1], dev), 1.0)
+    check_rows(n64(got)[0], None, O.attention_tight(n64(q)[0], k, v, np.ones(rows), [rows - 1] * heads, 1.0, dt == "f16", terms=1), dt)
