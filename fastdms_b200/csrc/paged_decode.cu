@@ -31,14 +31,24 @@ struct DecodeArgs {
     PagedCache c;
     const uint16_t* q;
     uint16_t* out;
-    float* lse;                                 // optional [batch, q_heads]
+    float* lse;                                 // optional [tokens, q_heads]
+    const int32_t* cu;                          // [batch + 1] where each sequence's token lies, or null: token b is sequence b's
     int64_t q_sb, q_sh, o_sb, o_sh, lse_sb, lse_sh;
-    float* parts;                               // [ctas][2][kDecHeads][D + 2]: O, M, l
+    float* parts;                               // [ctas][2][kDecHeads][D + 4]: O, M, l
     int2* cuts;                                 // [units] first part and last CTA of a unit that is cut, (0, -1) of others
-    int32_t batch, group, splits;               // splits: units per (sequence, KV head), each of up to 8 q heads
+    int32_t batch, tokens, group, splits;       // splits: units per (sequence, KV head), each of up to 8 q heads
     int32_t cluster;                            // CTAs per unit (clusters)
     float scale;
 };
+
+// Row of q and out that holds sequence b's token; -1 where it has none in this step, or not exactly one.
+__device__ __forceinline__ int token_of(const DecodeArgs& a, int b) {
+    if (!a.cu) return b;
+    const int at = a.cu[b], end = a.cu[b + 1];
+    if (at >= 0 && at < a.tokens && end == at + 1) return at;
+    if (end != at && a.c.status) atomicOr(a.c.status, FDMS_DEV_BAD_INDEX);
+    return -1;
+}
 
 // One 16-row page as matrix operands; lane (g, t) = (lane / 4, lane % 4).  Both products run transposed, the page's codes
 // being the 16-row operand and up to 8 q heads the 8 columns, so that no row of a fragment is idle:
@@ -318,14 +328,14 @@ __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u,
 // for many short sequences (300 up to 2000 rows 151 against 142).
 constexpr int kUnitPages = 24;
 
-// The weight (a unit's pages and kUnitPages, 0 without rows) of the sequences before b for all b, and in total, in shared memory; by
+// The weight (a unit's pages and kUnitPages, 0 without rows or without a token) of the sequences before b for all b, and in total, in shared memory; by
 // all threads of the CTA.
 __device__ __forceinline__ void weight_prefix(const DecodeArgs& a, int32_t* s_first, int32_t* s_warp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int32_t before = 0;
     for (int base = 0; base < a.batch; base += kDecThreads) {
         const int b = base + threadIdx.x;
-        const int pages = b < a.batch ? (int)(((int64_t)paged_len(a.c, b) + kCachePage - 1) / kCachePage) : 0;
+        const int pages = b < a.batch && token_of(a, b) >= 0 ? (int)(((int64_t)paged_len(a.c, b) + kCachePage - 1) / kCachePage) : 0;
         const int weight = pages ? pages + kUnitPages : 0;
         int sum = weight;
 #pragma unroll
@@ -395,13 +405,13 @@ __device__ __forceinline__ void merge_warps(const MergeSmem<D>& s, float (&acc)[
     }
 }
 template <int D, bool BF16>
-__device__ __forceinline__ void write_row(const DecodeArgs& a, int seq, int hq, const float (&acc)[D / 32], float m, float l) {
+__device__ __forceinline__ void write_row(const DecodeArgs& a, int tok, int hq, const float (&acc)[D / 32], float m, float l) {
     const int lane = threadIdx.x & 31;
     const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
-    uint16_t* out = a.out + seq * a.o_sb + (int64_t)hq * a.o_sh + lane * (D / 32);
+    uint16_t* out = a.out + tok * a.o_sb + (int64_t)hq * a.o_sh + lane * (D / 32);
 #pragma unroll
     for (int i = 0; i < D / 32; i += 2) *(uint32_t*)(out + i) = pack_pair<BF16>(acc[i] * inv, acc[i + 1] * inv);
-    if (a.lse && lane == 0) a.lse[seq * a.lse_sb + (int64_t)hq * a.lse_sh] = kPagedLn2 * (m + paged_lg2(l));
+    if (a.lse && lane == 0) a.lse[tok * a.lse_sb + (int64_t)hq * a.lse_sh] = kPagedLn2 * (m + paged_lg2(l));
 }
 
 // Clusters: unit blockIdx.x / cluster, page p of it with warp p % 8 of the cluster's CTA p / 8 % cluster.
@@ -416,10 +426,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
     const int first = rank * kDecWarps + warp, step = a.cluster * kDecWarps;
     // length, table entries and queries are requested together
     const int entry = entry_ahead(a.c, seq, first, step, 0);
+    const int tok = token_of(a, seq);
+    if (tok < 0) return;                        // the whole cluster
     const int len = paged_len(a.c, seq), pages = (int)(((int64_t)len + kCachePage - 1) / kCachePage);
     uint32_t qb[D / 16][2];
     float factor[2];
-    load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
+    load_q<D, BF16>(a.q + tok * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
     UnitState<D> st;
     clear<D>(st);
     walk_pages<D, !BF16>(a.c, st, qb, factor, seq, head, first, step, first < pages ? (pages - first + step - 1) / step : 0, len, entry);
@@ -428,7 +440,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
     float acc[D / 32], m, l;
     if (warp < nh) {
         merge_warps<D>(s, acc, m, l);
-        if (a.cluster == 1) write_row<D, BF16>(a, seq, head * a.group + h0 + warp, acc, m, l);
+        if (a.cluster == 1) write_row<D, BF16>(a, tok, head * a.group + h0 + warp, acc, m, l);
         else {
 #pragma unroll
             for (int i = 0; i < D / 32; i += 2) *(float2*)&s_part[warp][lane * (D / 32) + i] = make_float2(acc[i], acc[i + 1]);
@@ -472,7 +484,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_clust
                     acc[i + 1] = fmaf(y, w, acc[i + 1]);
                 }
             }
-        write_row<D, BF16>(a, seq, head * a.group + h0 + warp, acc, m, l);
+        write_row<D, BF16>(a, tok, head * a.group + h0 + warp, acc, m, l);
     }
     // a CTA's shared memory stays until every other has read it
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -494,11 +506,11 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
     if (blockIdx.x == 0) {                      // sequences without rows: zeros
         for (int b = warp; b < a.batch; b += kDecWarps) {
             if (s_first[b + 1] != s_first[b]) continue;
-            const int hq = a.c.heads * a.group;
-            for (int i = lane; i < hq * (D / 8); i += 32)
-                *(uint4*)(a.out + b * a.o_sb + (i / (D / 8)) * a.o_sh + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+            const int hq = a.c.heads * a.group, tok = token_of(a, b);
+            for (int i = lane; i < hq * (D / 8) && tok >= 0; i += 32)
+                *(uint4*)(a.out + tok * a.o_sb + (i / (D / 8)) * a.o_sh + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
             if (a.lse)
-                for (int i = lane; i < hq; i += 32) a.lse[b * a.lse_sb + i * a.lse_sh] = -INFINITY;
+                for (int i = lane; i < hq && tok >= 0; i += 32) a.lse[tok * a.lse_sb + i * a.lse_sh] = -INFINITY;
             for (int i = lane; i < per_seq; i += 32) a.cuts[(int64_t)b * per_seq + i] = make_int2(0, -1);
         }
     }
@@ -526,11 +538,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         const int p0 = (int)max((int64_t)0, from - unit_begin - kUnitPages), p1 = (int)(at - unit_begin) - kUnitPages;
         if (p1 <= 0) break;
         const int head = u / a.splits, h0 = (u % a.splits) * kDecHeads, nh = min(kDecHeads, a.group - h0);
+        const int tok = max(token_of(a, seq), 0);       // a sequence with weight has one
         const int len = min(paged_len(a.c, seq), pages * kCachePage);
         const int entry = entry_ahead(a.c, seq, p0 + warp, kDecWarps, 0);
         uint32_t qb[D / 16][2];
         float factor[2];
-        load_q<D, BF16>(a.q + seq * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
+        load_q<D, BF16>(a.q + tok * a.q_sb + (int64_t)(head * a.group + h0 + min(g, nh - 1)) * a.q_sh, a.scale, qb, factor, lane);
         UnitState<D> st;
         clear<D>(st);
         walk_pages<D, !BF16>(a.c, st, qb, factor, seq, head, p0 + warp, kDecWarps, p1 - p0 > warp ? (p1 - p0 - warp + kDecWarps - 1) / kDecWarps : 0, len, entry);
@@ -541,7 +554,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtasPerSm) paged_decode_kerne
         if (warp < nh) {
             float acc[D / 32], m, l;
             merge_warps<D>(s, acc, m, l);
-            if (whole) write_row<D, BF16>(a, seq, head * a.group + h0 + warp, acc, m, l);
+            if (whole) write_row<D, BF16>(a, tok, head * a.group + h0 + warp, acc, m, l);
             else {
                 float* part = a.parts + ((int64_t)slot * kDecHeads + warp) * (D + 4);
 #pragma unroll
@@ -594,7 +607,7 @@ __global__ void __launch_bounds__(256) paged_decode_join_kernel(DecodeArgs a, in
             acc[i + 1] = fmaf(x.y, w, acc[i + 1]);
         }
     }
-    write_row<D, BF16>(a, (int)seq, h, acc, m, l);
+    write_row<D, BF16>(a, max(token_of(a, (int)seq), 0), h, acc, m, l);
 }
 
 }  // namespace fdms
@@ -685,13 +698,13 @@ extern "C" int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t
 extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void* stream) {
     clear_error();
     DecodeArgs a;
-    const bool idle = args && args->num_seqs == 0;
+    const bool idle = args && (args->num_seqs == 0 || (args->cu_seqlens_q && args->tokens == 0));
     const int32_t rc = paged_attn_check("fdms_paged_attn_decode", args, a.c, idle);
     if (rc != FDMS_OK) return rc;
     const fdms_paged_attn_args& p = *args;
     const int num_q_heads = (int)p.num_q_heads, num_kv_heads = a.c.heads, head_dim = (int)p.cache.head_dim;
-    FDMS_REQUIRE(p.tokens == p.num_seqs, FDMS_E_ARG, "fdms_paged_attn_decode: one token per sequence, got %lld for %lld", (long long)p.tokens,
-                 (long long)p.num_seqs);
+    FDMS_REQUIRE(p.tokens == p.num_seqs || (p.cu_seqlens_q && p.tokens < p.num_seqs), FDMS_E_ARG,
+                 "fdms_paged_attn_decode: one token per sequence, got %lld for %lld", (long long)p.tokens, (long long)p.num_seqs);
     FDMS_REQUIRE(p.num_seqs <= kDecMaxBatch, FDMS_E_CAPACITY, "fdms_paged_attn_decode: at most %d sequences a call, got %lld", kDecMaxBatch,
                  (long long)p.num_seqs);
     if (idle) return FDMS_OK;
@@ -701,6 +714,8 @@ extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void
     a.q = (const uint16_t*)p.q;
     a.out = (uint16_t*)p.out;
     a.lse = p.lse_out;
+    a.cu = p.cu_seqlens_q;
+    a.tokens = (int)p.tokens;
     a.q_sb = p.q_stride[0]; a.q_sh = p.q_stride[1]; a.o_sb = p.out_stride[0]; a.o_sh = p.out_stride[1];
     a.lse_sb = p.lse_stride[0]; a.lse_sh = p.lse_stride[1];
     a.batch = batch;

@@ -9,7 +9,8 @@ pool); it runs through torch's scaled_dot_product_attention per sequence.
 Without compact KV, a Context that carries `block_tables`, `slot_mapping` and `context_lens` selects the dense paged
 branch (reference: attention.py:82-92, 124-151): K and V of the step are stored into the layer's `k_cache` / `v_cache`
 (e4m3 blocks with the scales `k_cache_scale` / `v_cache_scale`, `layers/paged_attention.py`) and attention reads them
-from there, prompts and single tokens alike.
+from there, prompts and single tokens alike.  Without `cu_seqlens_q` a decode step has one token for every row of
+`block_tables`; with it some may have none.
 """
 from __future__ import annotations
 
@@ -119,7 +120,8 @@ class Attention(nn.Module):
             with prof.cuda_phase("paged_prefill_attn"):
                 return paged_prefill_attention(q, *cache, context.block_tables, context.context_lens, context.cu_seqlens_q, self.scale)
         with prof.cuda_phase("paged_decode_attn"):
-            return paged_decode_attention(q, *cache, context.block_tables, context.context_lens, self.scale)
+            return paged_decode_attention(q, *cache, context.block_tables, context.context_lens, self.scale,
+                                          cu_seqlens_q=context.cu_seqlens_q)
 
     def forward(self, q, k, v, *, compact_append_stored: bool = False, compact_q_rope: bool = False,
                 positions: torch.Tensor | None = None, cos_sin_cache: torch.Tensor | None = None):

@@ -13,8 +13,11 @@ A step, for prompts and for single tokens alike:
 
     cu_seqlens, slots, positions = build_paged_metadata(new_lens, kv_lens, block_tables, free_blocks, free_count, ...)
     per layer:  store_paged_kvcache(k, v, ..., slots)
-                paged_prefill_attention(q, ..., cu_seqlens)   or, one token per sequence, paged_decode_attention(q, ...)
+                paged_prefill_attention(q, ..., cu_seqlens)   or, with a token per sequence at most,
+                paged_decode_attention(q, ..., cu_seqlens_q=cu_seqlens)
     release_paged_blocks(...)   for sequences that ended
+
+The tokens of a step lie one after the other, sequence by sequence, without gaps for sequences that have none.
 
 Every call enqueues on the current stream of its tensors' device and can be captured into a CUDA graph.  There is no CPU
 path: tensors must live on a CUDA device.
@@ -253,8 +256,8 @@ def store_paged_kvcache(
         _lib.status_word(k_cache.device).data_ptr(), shape[0], dtype, *key.stride(), *value.stride()), dev)
 
 
-def _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, lse_shape):
-    """Both attentions: with `cu_seqlens_q` the prefill, without it one token per sequence."""
+def _attention(decode, q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, lse_shape):
+    """Both attentions."""
     blocks, heads, block_size, head_dim = _cache_shape(k_cache, v_cache, k_scale, v_scale)
     shape = q.shape
     if shape[2] != head_dim:
@@ -285,13 +288,13 @@ def _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_
             _device(dict(q=q, lse_out=lse_out))
         lse_ptr, lse_stride = lse_out.data_ptr(), lse_out.stride()
     lib, need, ws = _lib.lib(), 0, None
-    if cu_seqlens_q is None:
-        need = _on_device(dev, lib.fdms_paged_attn_decode_workspace_bytes, tokens, num_q_heads, heads, head_dim, cols * block_size)
+    if decode:
+        need = _on_device(dev, lib.fdms_paged_attn_decode_workspace_bytes, seqs, num_q_heads, heads, head_dim, cols * block_size)
     else:
         need = _on_device(dev, lib.fdms_paged_attn_prefill_workspace_bytes, tokens, seqs, num_q_heads, heads, head_dim, cols * block_size)
     if need > 0:
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _launch(lib.fdms_paged_attn_decode if cu_seqlens_q is None else lib.fdms_paged_attn_prefill, _ATTN_ARGS.pack(
+    _launch(lib.fdms_paged_attn_decode if decode else lib.fdms_paged_attn_prefill, _ATTN_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, block_size, head_dim,
         *k_cache.stride(), *v_cache.stride(), q.data_ptr(), out.data_ptr(), lse_ptr, block_tables.data_ptr(), kv_lens.data_ptr(),
         0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if ws is None else ws.data_ptr(), _lib.status_word(q.device).data_ptr(),
@@ -310,6 +313,7 @@ def paged_decode_attention(
     kv_lens: torch.Tensor,
     scale: float | None = None,
     *,
+    cu_seqlens_q: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
     lse_out: torch.Tensor | None = None,
 ) -> torch.Tensor:
@@ -317,16 +321,26 @@ def paged_decode_attention(
     each sequence, the token's own row among them; q head h reads KV head h // (q_heads // kv_heads).  bfloat16 or float16
     queries, head_dim 64 or 128, at most 2048 sequences.  `scale` defaults to head_dim ** -0.5.  A sequence without rows gets
     zeros.  `lse_out` (float32 `[batch, q_heads]`) receives the natural-log log-sum-exp of the scaled scores.  Table
-    entries that are needed and name no block of the cache are left out and raise the device status bit for bad indices."""
+    entries that are needed and name no block of the cache are left out and raise the device status bit for bad indices.
+
+    Without `cu_seqlens_q` row b of q is sequence b's token: every sequence has exactly one in the step.  A step in which some
+    sequences have none (`new_lens` of 0: released, or waiting) passes the `cu_seqlens` of `build_paged_metadata` (int32
+    `[sequences + 1]`): q, out and `lse_out` are then `[tokens, ...]`, no more tokens than sequences, and sequence b's token is
+    row `cu_seqlens_q[b]`.  A sequence without a token takes no part; one with several neither, and raises the device status bit
+    for bad indices.  Rows that are no sequence's token (a padded step) are left as they were in `out` and `lse_out`."""
     shape = q.shape
     if len(shape) != 3:
         raise ValueError(f"expected q as [batch, q_heads, head_dim], got {tuple(shape)}")
-    batch = shape[0]
-    if kv_lens.numel() != batch:
-        raise ValueError(f"expected kv_lens as contiguous int32 [{batch}], got {tuple(kv_lens.shape)} {kv_lens.dtype}")
+    batch = kv_lens.numel()
+    if cu_seqlens_q is not None:
+        _int_vector(cu_seqlens_q, "cu_seqlens_q", batch + 1)
+        if shape[0] > batch:
+            raise ValueError(f"expected at most {batch} tokens, one per sequence, got {shape[0]}")
+    elif batch != shape[0]:
+        raise ValueError(f"expected kv_lens as contiguous int32 [{shape[0]}], got {tuple(kv_lens.shape)} {kv_lens.dtype}")
     if batch > MAX_DECODE_BATCH:
         raise RuntimeError(f"at most {MAX_DECODE_BATCH} sequences a call, got {batch}")
-    return _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, None, scale, out, lse_out, shape[:2])
+    return _attention(True, q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, shape[:2])
 
 
 def paged_prefill_attention(
@@ -352,4 +366,4 @@ def paged_prefill_attention(
     if len(shape) != 3:
         raise ValueError(f"expected q as [tokens, q_heads, head_dim], got {tuple(shape)}")
     _int_vector(cu_seqlens_q, "cu_seqlens_q", kv_lens.numel() + 1)
-    return _attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, (shape[1], shape[0]))
+    return _attention(False, q, k_cache, v_cache, k_scale, v_scale, block_tables, kv_lens, cu_seqlens_q, scale, out, lse_out, (shape[1], shape[0]))

@@ -514,7 +514,10 @@ int32_t fdms_linear_decode_allreduce(
  *   written, not below the scale of a block that holds earlier rows, whose codes then move to the new scale.  A sequence's
  *   tokens are consecutive; no block is written by two sequences.
  * fdms_paged_attn_decode: out[b, hq] = softmax(scale * q[b, hq] K^T) V over the first kv_lens[b] rows, q [batch, q_heads,
- *   head_dim]; no rows: zeros.  lse_out (optional): natural-log log-sum-exp, -inf without rows.  batch <= 2048.
+ *   head_dim]; no rows: zeros.  lse_out (optional): natural-log log-sum-exp, -inf without rows.  batch <= 2048.  With
+ *   cu_seqlens_q (or NULL) sequence b's token is row cu_seqlens_q[b] of q, out and lse_out, [tokens <= batch, ...], as
+ *   fdms_paged_metadata lays a step's tokens out; a sequence without a token takes no part, one with several neither and raises FDMS_DEV_BAD_INDEX,
+ *   and rows that are no sequence's token are left untouched.
  *   workspace: fdms_paged_attn_decode_workspace_bytes(...) bytes on the current device (max_rows = max_blocks * block_size),
  *   16-byte aligned, any contents; calls that share one must not overlap on the GPU.
  * fdms_paged_attn_prefill: q [tokens, q_heads, head_dim], sequence s's tokens at cu_seqlens_q[s] .. cu_seqlens_q[s + 1];
@@ -560,7 +563,7 @@ typedef struct fdms_paged_attn_args {
     int32_t *dev_status;
     int64_t tokens, num_seqs, num_q_heads, dtype, max_blocks, bt_stride, workspace_bytes;
     int64_t q_stride[3], out_stride[3]; /* token, head, channel (1), in elements */
-    int64_t lse_stride[2];              /* decode: sequence, head; prefill: head, token */
+    int64_t lse_stride[2];              /* decode: token, head; prefill: head, token */
     double scale;
 } fdms_paged_attn_args;
 

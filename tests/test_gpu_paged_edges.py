@@ -79,3 +79,110 @@ def test_weights_whose_roundings_add_up(dev, form, dt, wide, jump):
     else:
         got = paged_prefill_attention(q.to(dev), kc, vc, ks, vs, table, i32([rows], dev), i32([0, 1], dev), 1.0)
     check_rows(n64(got)[0], None, O.attention_tight(n64(q)[0], k, v, np.ones(rows), [rows - 1] * heads, 1.0, dt == "f16", terms=1), dt)
+
+
+# ---- rows that sit a step out --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("d,dt,spare", [(64, "bf16", 0), (128, "f16", 2)])
+def test_decode_finds_the_token_of_a_sequence(dev, d, dt, spare, wide):
+    """Sequences without a token between others, one of them empty; `spare` rows of q are nobody's."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention
+    rng = np.random.default_rng(d)
+    heads, group, bs = 2, 4, 16
+    lens, new = [40, 333, 0, 7, 90, 0, 1], [1, 0, 1, 1, 0, 0, 1]
+    (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, lens, heads, bs, d, dev)
+    if wide:
+        table = wide_table(table, bs)
+    tokens = sum(new) + spare
+    q = _random_rows(rng, (tokens, heads * group, d), dt, loud=False)
+    out, lse = torch.full(q.shape, 3.0, dtype=DT[dt], device=dev), torch.full((tokens, heads * group), 7.0, device=dev)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    got = paged_decode_attention(q.to(dev), kc, vc, ks, vs, table, i32(lens, dev), cu_seqlens_q=i32(cu, dev), out=out, lse_out=lse)
+    assert (got[sum(new):] == 3.0).all() and (lse[sum(new):] == 7.0).all()
+    for b, m in enumerate(lens):
+        if not new[b]:
+            continue
+        for h in range(heads):
+            k, v = (O.rows_of(codes[c], scale[c], tab[b], m, h, bs) for c in range(2))
+            r = slice(h * group, (h + 1) * group)
+            check_rows(n64(got)[cu[b], r], n64(lse)[cu[b], r], O.attention(n64(q)[cu[b], r], k, v, [m - 1] * group, d ** -0.5), dt)
+    # the same bits as the sequences of the tokens by themselves
+    have = torch.tensor([b for b in range(len(lens)) if new[b]], device=dev)
+    alone = paged_decode_attention(q[:sum(new)].to(dev), kc, vc, ks, vs, table[have].contiguous(), i32(np.asarray(lens)[have.cpu()], dev))
+    half = torch.finfo(DT[dt]).eps
+    assert ((got[:sum(new)].float() - alone.float()).abs() <= half * alone.float().abs() + half * float(vs.nan_to_num().max())).all()
+    # several tokens, or one beyond q: left out, and said
+    for broken in ([0, 2, 2, 3, 4, 4, 4, 4], [0, 1, 1, 2, 3, 3, 3, tokens + 1], [-1, 0, 0, 0, 0, 0, 0, 0]):
+        out = torch.full(q.shape, 3.0, dtype=DT[dt], device=dev)
+        paged_decode_attention(q.to(dev), kc, vc, ks, vs, table, i32(lens, dev), cu_seqlens_q=i32(broken, dev), out=out)
+        assert raised(dev)
+        held = [a for a, b in zip(broken, broken[1:]) if a >= 0 and b == a + 1 and a < tokens]
+        assert all((out[t] == 3.0).all() == (t not in held) for t in range(tokens))
+    nobody = paged_decode_attention(q[:0].to(dev), kc, vc, ks, vs, table, i32(lens, dev), cu_seqlens_q=i32([0] * 8, dev))
+    assert nobody.shape[0] == 0
+
+
+@pytest.mark.parametrize("cols", [20, 2500])
+def test_a_captured_step_with_rows_that_have_ended(dev, cols):
+    """A decode step of four rows, captured once: rows are released, sit steps out and come back between its replays."""
+    from fastdms_b200.layers import paged_attention as P
+    r = Run(dev, 9, cols=cols)
+    r.step([30, 5, 44, 17])
+    q, k, v = (x.to(dev) for x in r.inputs(r.n))
+    new = i32([1] * r.n, dev)
+
+    def call():
+        cu, slots, _ = P.build_paged_metadata(new, r.kv, r.table, r.free, r.count, block_size=r.bs, total_tokens=r.n)
+        P.store_paged_kvcache(k, v, r.kc, r.vc, r.ks, r.vs, slots)
+        return P.paged_decode_attention(q, r.kc, r.vc, r.ks, r.vs, r.table, r.kv, cu_seqlens_q=cu), slots
+
+    state = [x.clone() for x in (r.kv, r.count, r.table, r.kc, r.vc, r.ks, r.vs)]
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream(dev).wait_stream(side)
+    for x, y in zip((r.kv, r.count, r.table, r.kc, r.vc, r.ks, r.vs), state):
+        x.copy_(y)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, slots = call()
+
+    def replay(step):
+        new.copy_(i32(step, dev))
+        ins = r.inputs(r.n)
+        for x, y in zip((q, k, v), ins):
+            x.copy_(y)
+        g.replay()
+        torch.cuda.synchronize(dev)
+        r.check(step, *ins, out, slots)
+
+    replay([1, 1, 1, 1])
+    P.release_paged_blocks(r.kv, r.table, r.free, r.count, block_size=r.bs, rows=i32([1], dev))
+    for _ in range(18):
+        replay([1, 0, 1, 1])
+    replay([0, 0, 0, 1])
+    replay([0, 1, 1, 0])                         # the released row starts again, others wait
+    replay([0, 0, 0, 0])
+    replay([1, 1, 1, 1])
+
+
+def test_layer_decodes_with_rows_that_sit_out(dev):
+    """`Attention` gives its decode the offsets of the context."""
+    from fastdms_b200.layers import paged_attention as P
+    from fastdms_b200.layers.attention import Attention
+    from fastdms_b200.utils.context import reset_context, set_context
+    r = Run(dev, 10)
+    r.step([30, 5, 44, 17])
+    layer = Attention(r.heads * r.group, r.d, r.d ** -0.5, r.heads)
+    layer.k_cache, layer.v_cache, layer.k_cache_scale, layer.v_cache_scale = r.kc, r.vc, r.ks, r.vs
+    for new in ([1, 0, 1, 1], [0, 1, 0, 0], [1, 1, 1, 1]):
+        q, k, v = r.inputs(sum(new))
+        cu, slots, _ = P.build_paged_metadata(i32(new, dev), r.kv, r.table, r.free, r.count, block_size=r.bs, total_tokens=sum(new))
+        try:
+            set_context(False, cu_seqlens_q=cu, slot_mapping=slots, context_lens=r.kv, block_tables=r.table)
+            out = layer(q.to(dev), k.to(dev), v.to(dev))
+        finally:
+            reset_context()
+        r.check(new, q, k, v, out, slots)

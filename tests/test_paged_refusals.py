@@ -184,3 +184,16 @@ def test_plain_statement():
     x = torch.from_numpy(x).float().clamp(-448, 448)
     assert np.array_equal(O.encode(x.double().numpy()), x.to(torch.float8_e4m3fn).view(torch.uint8).numpy())
     assert O.scale_of(448.0) == 1.0 and O.scale_of(448.1) == 2.0 and O.scale_of(224.0) == 0.5 and O.scale_of(0.0) == 2.0 ** -60 and O.scale_of(1e30) == 2.0 ** 40
+
+
+def test_decode_refuses_offsets():
+    q, kv, table = torch.zeros((2, 4, 64), dtype=torch.bfloat16), ints(3, 4), torch.zeros((2, 2), dtype=torch.int32)
+    for cu, match in ((ints(0, 1), "cu_seqlens_q"), (torch.tensor([0, 1, 2]), "cu_seqlens_q"), (ints(0, 9, 1, 9, 2)[::2], "cu_seqlens_q")):
+        with pytest.raises(ValueError, match=match):
+            P.paged_decode_attention(q, *cache(), table, kv, cu_seqlens_q=cu)
+    with pytest.raises(ValueError, match="at most 1 tokens"):
+        P.paged_decode_attention(q, *cache(), table[:1], kv[:1], cu_seqlens_q=ints(0, 1))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.paged_decode_attention(q[:1], *cache(), table, kv, cu_seqlens_q=ints(0, 0, 1))
+    lib = _lib.lib()
+    assert lib.fdms_paged_attn_decode(P._ATTN_ARGS.pack(*(ATTN | dict(tokens=1, cu=0)).values()), None) == E and b"one token per sequence" in lib.fdms_last_error()
