@@ -82,6 +82,7 @@ _SIGNATURES = {
     "fdms_paged_metadata_workspace_bytes": (I64, [I64, I64]),
     "fdms_paged_metadata": (I32, [c_char_p, P]),
     "fdms_paged_release": (I32, [P, I32, P, I32, P, I64, I32, I32, P, I64, P, P, P]),
+    "fdms_paged_release_pool": (I32, [P, I32, P, I32, P, I64, I32, I32, P, I64, I64, P, P, P]),
     "fdms_paged_store": (I32, [c_char_p, P]),
     "fdms_paged_attn_decode_workspace_bytes": (I64, [I64, I64, I64, I64, I64]),
     "fdms_paged_attn_decode": (I32, [c_char_p, P]),

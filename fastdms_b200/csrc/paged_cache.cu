@@ -204,7 +204,7 @@ constexpr int kReleaseRows = 4096;
 
 __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
     const int32_t* rows, int n, int32_t* kv_lens, int num_rows, int32_t* tables, int64_t table_stride, int max_blocks,
-    int shift, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count, int32_t* status) {
+    int shift, int32_t* free_blocks, int64_t free_capacity, int64_t num_blocks, int32_t* free_count, int32_t* status) {
     __shared__ int32_t s_row[kReleaseRows];     // row of each entry, -1 where it is out of range or listed before
     __shared__ int32_t s_held[kReleaseRows];    // usable blocks of the entry, then their place on the stack
     __shared__ int32_t s_end;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
             const int cols = (int)min((len + (1 << shift) - 1) >> shift, (int64_t)max_blocks);
             for (int c = lane; c < cols; c += 32) {
                 const int b = tables[(int64_t)r * table_stride + c];
-                if (b >= 0 && b < free_capacity) ++held; else bad = true;
+                if (b >= 0 && b < num_blocks) ++held; else bad = true;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) held += __shfl_xor_sync(0xffffffffu, held, o);
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(
                 b = tables[(int64_t)r * table_stride + c];
                 tables[(int64_t)r * table_stride + c] = -1;
             }
-            const bool use = b >= 0 && b < free_capacity;
+            const bool use = b >= 0 && b < num_blocks;
             const unsigned m = __ballot_sync(0xffffffffu, use);
             const int64_t to = at + __popc(m & ((1u << lane) - 1));
             if (use && to < free_capacity) free_blocks[to] = b;
@@ -521,25 +521,33 @@ extern "C" int32_t fdms_paged_metadata(const fdms_paged_metadata_args* args, voi
     return FDMS_OK;
 }
 
-extern "C" int32_t fdms_paged_release(
+extern "C" int32_t fdms_paged_release_pool(
     const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
-    int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
+    int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int64_t num_blocks, int32_t* free_count,
     int32_t* dev_status, void* stream) {
     clear_error();
     FDMS_REQUIRE(free_count && (free_blocks || free_capacity == 0) && ((kv_lens && (block_tables || max_blocks == 0)) || num_rows == 0), FDMS_E_ARG,
                  "fdms_paged_release: null pointer");
     const int32_t shift = block_shift(block_size);
     FDMS_REQUIRE(shift > 0, FDMS_E_ARG, "fdms_paged_release: block_size must be 16, 32, 64 or 128, got %d", block_size);
-    FDMS_REQUIRE(num_listed >= 0 && num_rows >= 0 && max_blocks >= 0 && free_capacity >= 0 && bt_stride >= max_blocks, FDMS_E_ARG,
+    FDMS_REQUIRE(num_listed >= 0 && num_rows >= 0 && max_blocks >= 0 && free_capacity >= 0 && num_blocks >= 0 && bt_stride >= max_blocks, FDMS_E_ARG,
                  "fdms_paged_release: negative size, or rows of the block table overlap");
     FDMS_REQUIRE(rows || num_listed <= num_rows, FDMS_E_ARG, "fdms_paged_release: more rows than the block table has");
-    FDMS_REQUIRE(num_listed <= kReleaseRows && free_capacity <= (0x7fffffffll >> shift), FDMS_E_CAPACITY,
+    FDMS_REQUIRE(num_listed <= kReleaseRows && free_capacity <= (0x7fffffffll >> shift) && num_blocks <= (0x7fffffffll >> shift), FDMS_E_CAPACITY,
                  "fdms_paged_release: at most %d rows a call, and slot numbers must fit in 31 bits", kReleaseRows);
     if (num_listed == 0) return FDMS_OK;
-    paged_release_kernel<<<1, kReleaseThreads, 0, (cudaStream_t)stream>>>(rows, num_listed, kv_lens, num_rows, block_tables, bt_stride,
-                                                                         max_blocks, shift, free_blocks, free_capacity, free_count, dev_status);
+    paged_release_kernel<<<1, kReleaseThreads, 0, (cudaStream_t)stream>>>(rows, num_listed, kv_lens, num_rows, block_tables, bt_stride, max_blocks,
+                                                                         shift, free_blocks, free_capacity, num_blocks, free_count, dev_status);
     FDMS_CHECK_LAUNCH("paged_release_kernel");
     return FDMS_OK;
+}
+
+extern "C" int32_t fdms_paged_release(
+    const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
+    int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
+    int32_t* dev_status, void* stream) {
+    return fdms_paged_release_pool(rows, num_listed, kv_lens, num_rows, block_tables, bt_stride, max_blocks, block_size, free_blocks, free_capacity,
+                                   free_capacity, free_count, dev_status, stream);
 }
 
 extern "C" int32_t fdms_paged_store(const fdms_paged_store_args* args, void* stream) {

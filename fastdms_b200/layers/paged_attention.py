@@ -141,7 +141,8 @@ def build_paged_metadata(
     `positions` (int64 `[total_tokens]`); buffers given for them are
     filled, and overlap no other argument.  `total_tokens` may exceed the sum of `new_lens`
     (a padded batch): the slots behind it are -1, which the store skips, and the positions 0.  Each sequence has a row of its
-    own; free block ids are distinct."""
+    own; free block ids are distinct, and blocks of the cache (`release_paged_blocks` has to know how many those are where the
+    stack does not hold them all)."""
     n = kv_lens.numel()
     _int_vector(kv_lens, "kv_lens")
     _int_vector(new_lens, "new_lens", n)
@@ -193,10 +194,15 @@ def release_paged_blocks(
     *,
     block_size: int,
     rows: torch.Tensor | None = None,
+    num_blocks: int | None = None,
 ) -> None:
     """Gives the blocks of the listed rows (int32 indices of `kv_lens` and `block_tables`; all rows without a list) back to
     the stack and empties the rows: table entries -1, length 0.  A row that is listed twice is released once and, like one
-    out of range or a block id outside the pool, raises the device status bit for bad indices."""
+    out of range or a block id outside the pool, raises the device status bit for bad indices.
+
+    `num_blocks` is the number of blocks of the cache, whose ids lie below it; without it `free_blocks` has room for all of them.
+    A stack that holds only some (a block kept for padding, a range of a shared pool) needs it: ids at or beyond
+    `free_blocks.numel()` would be taken for none of the pool's, and their blocks lost."""
     n = kv_lens.numel()
     _int_vector(kv_lens, "kv_lens")
     _int_vector(free_blocks, "free_blocks")
@@ -205,13 +211,16 @@ def release_paged_blocks(
     _check_block_size(block_size)
     if rows is not None:
         _int_vector(rows, "rows")
+    num_blocks = free_blocks.numel() if num_blocks is None else int(num_blocks)
+    if num_blocks < 0:
+        raise ValueError(f"num_blocks must not be negative, got {num_blocks}")
     dev = _device(dict(kv_lens=kv_lens, block_tables=block_tables, free_blocks=free_blocks, free_count=free_count, rows=rows))
     status = _lib.status_word(kv_lens.device)
     with torch.cuda.device(dev):
-        rc = _lib.lib().fdms_paged_release(
+        rc = _lib.lib().fdms_paged_release_pool(
             _lib.ptr(rows) if rows is not None and rows.numel() else None, n if rows is None else rows.numel(), kv_lens.data_ptr(), n,
-            block_tables.data_ptr(), stride, cols, block_size, free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(),
-            status.data_ptr(), _lib.stream_ptr(kv_lens.device))
+            block_tables.data_ptr(), stride, cols, block_size, free_blocks.data_ptr(), free_blocks.numel(), num_blocks,
+            free_count.data_ptr(), status.data_ptr(), _lib.stream_ptr(kv_lens.device))
     _lib.check(rc)
 
 

@@ -507,8 +507,10 @@ int32_t fdms_linear_decode_allreduce(
  *   (tokens behind the last: -1 and 0).  kv_lens_out / free_count_out may be kv_lens / free_count.  A negative length, one
  *   beyond max_blocks * block_size, or more tokens than total_tokens is not served and raises FDMS_DEV_BAD_INDEX.
  *   workspace: fdms_paged_metadata_workspace_bytes(...) bytes, 8-byte aligned, any contents.
- * fdms_paged_release: the blocks of rows[0 .. num_listed) (NULL: rows 0 .. num_listed) return to the stack; their
- *   table entries become -1 and their lengths 0.  At most 4096 rows; a row listed twice is released once.
+ * fdms_paged_release_pool: the blocks of rows[0 .. num_listed) (NULL: rows 0 .. num_listed) return to the stack; their
+ *   table entries become -1 and their lengths 0.  At most 4096 rows; a row listed twice is released once.  Ids are
+ *   0 .. num_blocks - 1 (others are dropped and raise FDMS_DEV_BAD_INDEX), which need not be the stack's capacity: a stack may hold
+ *   some of the pool's blocks only.  fdms_paged_release: a stack with room for the whole pool, num_blocks = free_capacity.
  * fdms_paged_store: k, v [tokens, kv_heads, head_dim] (bf16 / f16, strides in elements, 16-byte aligned) into the rows of
  *   slot_mapping (negative: skipped).  Per block and head: the scale is the least 2^k with |x| <= 448 * 2^k over the rows
  *   written, not below the scale of a block that holds earlier rows, whose codes then move to the new scale.  A sequence's
@@ -573,6 +575,10 @@ int32_t fdms_paged_metadata(const fdms_paged_metadata_args* args, void* stream);
 int32_t fdms_paged_release(
     const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
     int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int32_t* free_count,
+    int32_t* dev_status, void* stream);
+int32_t fdms_paged_release_pool(
+    const int32_t* rows, int32_t num_listed, int32_t* kv_lens, int32_t num_rows, int32_t* block_tables, int64_t bt_stride,
+    int32_t max_blocks, int32_t block_size, int32_t* free_blocks, int64_t free_capacity, int64_t num_blocks, int32_t* free_count,
     int32_t* dev_status, void* stream);
 int32_t fdms_paged_store(const fdms_paged_store_args* args, void* stream);
 int64_t fdms_paged_attn_decode_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows);

@@ -186,3 +186,25 @@ def test_layer_decodes_with_rows_that_sit_out(dev):
         finally:
             reset_context()
         r.check(new, q, k, v, out, slots)
+
+
+# ---- pools whose stack does not hold every block -------------------------------------------------------------------
+
+@pytest.mark.parametrize("first,blocks", [(1, 12), (20, 31)])
+def test_release_into_a_stack_of_part_of_the_pool(dev, first, blocks):
+    """Blocks below `first` are kept for something else, so that ids reach beyond the stack's length."""
+    from fastdms_b200.layers.paged_attention import build_paged_metadata, release_paged_blocks
+    n = blocks - first
+    free, count = torch.arange(first, blocks, dtype=torch.int32, device=dev), i32([n], dev)
+    kv, table = i32([0, 0, 0], dev), i32(np.full((3, 8), -1), dev)
+    for _ in range(3):
+        build_paged_metadata(i32([40, 16, 70], dev), kv, table, free, count, block_size=16, total_tokens=126)
+        assert int(count) == n - 9 and kv.tolist() == [40, 16, 70]
+        release_paged_blocks(kv, table, free, count, block_size=16, rows=i32([2, 0], dev), num_blocks=blocks)
+        release_paged_blocks(kv, table, free, count, block_size=16, num_blocks=blocks)
+        assert int(count) == n and sorted(free.tolist()) == list(range(first, blocks)) and (table == -1).all()
+    # an id beyond the pool is no block of it
+    kv, table = i32([40], dev), i32([[first, blocks, first + 1]], dev)
+    count = i32([n - 2], dev)
+    release_paged_blocks(kv, table, free, count, block_size=16, num_blocks=blocks)
+    assert raised(dev) and int(count) == n and free[n - 2:].tolist() == [first + 1, first]

@@ -197,3 +197,15 @@ def test_decode_refuses_offsets():
         P.paged_decode_attention(q[:1], *cache(), table, kv, cu_seqlens_q=ints(0, 0, 1))
     lib = _lib.lib()
     assert lib.fdms_paged_attn_decode(P._ATTN_ARGS.pack(*(ATTN | dict(tokens=1, cu=0)).values()), None) == E and b"one token per sequence" in lib.fdms_last_error()
+
+
+def test_release_refuses_the_number_of_blocks():
+    kv, table, free, count = ints(1, 2), torch.zeros((2, 4), dtype=torch.int32), ints(0, 1), ints(2)
+    with pytest.raises(ValueError, match="num_blocks"):
+        P.release_paged_blocks(kv, table, free, count, block_size=16, num_blocks=-1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.release_paged_blocks(kv, table, free, count, block_size=16, num_blocks=9)
+    lib = _lib.lib()
+    rel = dict(rows=PTR, listed=2, kv=PTR, n=2, bt=PTR, stride=4, cols=4, bs=16, free=PTR, capacity=8, blocks=9, count=PTR, status=None, stream=None)
+    for change, code, words in [(dict(blocks=-1), E, b"negative"), (dict(blocks=1 << 28), C, b"31 bits"), (dict(listed=5000), C, b"rows a call")]:
+        assert lib.fdms_paged_release_pool(*(rel | change).values()) == code and words in lib.fdms_last_error()
