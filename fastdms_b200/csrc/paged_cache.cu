@@ -341,6 +341,22 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     return *(const uint32_t*)&m;
 }
 
+// The nearest slot before the lane's token that is not negative, -1 if there is none; the lanes hold the slots of tokens first + lane,
+// `prev` the slot before each.  By the whole warp.
+__device__ __noinline__ int32_t slot_before(const int32_t* slots, int64_t first, int32_t my_slot, int32_t prev) {
+    const int lane = threadIdx.x & 31;
+    const unsigned below = __ballot_sync(0xffffffffu, my_slot >= 0) & ((1u << lane) - 1);
+    const int32_t near = __shfl_sync(0xffffffffu, my_slot, below ? 31 - __clz(below) : 0);
+    int32_t before = __shfl_sync(0xffffffffu, prev, 0);
+    for (int64_t end = first - 1; before < 0 && end > 0; end -= 32) {
+        const int64_t t = end - 32 + lane;
+        const int32_t x = t >= 0 ? __ldg(slots + t) : -1;
+        const unsigned m = __ballot_sync(0xffffffffu, x >= 0);
+        if (m) before = __shfl_sync(0xffffffffu, x, 31 - __clz(m));
+    }
+    return below ? near : before;
+}
+
 // D: head_dim.  A lane holds 8 elements of every (32 / (D / 8))-th row of the warp's 16.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreArgs a) {
@@ -364,7 +380,9 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) paged_store_kernel(StoreA
         if (lane > 0) prev = up;
     }
     bool begins = lane < a.group && my_slot >= 0 && ((my_slot & (bs - 1)) == 0 || prev != my_slot - 1);
-    // a slot map lists a block's tokens in order and together
+    // A slot map lists a block's tokens in order and together: two runs in one block would move its scale and its codes side by
+    // side.  So what a token begins a run after is the nearest one before it that is not skipped, however far back.
+    if (__any_sync(0xffffffffu, begins && prev < 0)) prev = slot_before(a.slots, first, my_slot, prev);
     if (begins && (my_slot >= a.num_slots || (prev >= 0 && (prev >> a.shift) == (my_slot >> a.shift)))) {
         begins = false;
         if (a.status) atomicOr(a.status, FDMS_DEV_BAD_INDEX);

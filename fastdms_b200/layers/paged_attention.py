@@ -242,9 +242,9 @@ def store_paged_kvcache(
     even; values beyond 448 * 2^40 are held at it, a NaN stays one and does not count for the scale.  Rows behind the last
     one written are left as they were.
 
-    A sequence's tokens are consecutive, as `build_paged_metadata` lays them out, and no block is written by two sequences.
-    A slot beyond the cache, or next to a token of its own block that it does not follow, is skipped and raises the device
-    status bit for bad indices."""
+    The tokens of a block are consecutive, as `build_paged_metadata` lays them out, without skipped ones between them, and no
+    block is written by two sequences.  A slot beyond the cache, or in the block of the nearest earlier token that is not
+    skipped without following it directly, is skipped and raises the device status bit for bad indices."""
     blocks, heads, block_size, head_dim = _cache_shape(k_cache, v_cache, k_scale, v_scale)
     shape = key.shape
     if len(shape) != 3 or value.shape != shape:

@@ -513,8 +513,9 @@ int32_t fdms_linear_decode_allreduce(
  *   some of the pool's blocks only.  fdms_paged_release: a stack with room for the whole pool, num_blocks = free_capacity.
  * fdms_paged_store: k, v [tokens, kv_heads, head_dim] (bf16 / f16, strides in elements, 16-byte aligned) into the rows of
  *   slot_mapping (negative: skipped).  Per block and head: the scale is the least 2^k with |x| <= 448 * 2^k over the rows
- *   written, not below the scale of a block that holds earlier rows, whose codes then move to the new scale.  A sequence's
- *   tokens are consecutive; no block is written by two sequences.
+ *   written, not below the scale of a block that holds earlier rows, whose codes then move to the new scale.  The
+ *   tokens of a block are consecutive, no skipped ones between them; no block is written by two sequences.  A slot beyond the cache,
+ *   or in the block of the nearest earlier slot that is not negative without following it, is skipped and raises FDMS_DEV_BAD_INDEX.
  * fdms_paged_attn_decode: out[b, hq] = softmax(scale * q[b, hq] K^T) V over the first kv_lens[b] rows, q [batch, q_heads,
  *   head_dim]; no rows: zeros.  lse_out (optional): natural-log log-sum-exp, -inf without rows.  batch <= 2048.  With
  *   cu_seqlens_q (or NULL) sequence b's token is row cu_seqlens_q[b] of q, out and lse_out, [tokens <= batch, ...], as

@@ -208,3 +208,34 @@ def test_release_into_a_stack_of_part_of_the_pool(dev, first, blocks):
     count = i32([n - 2], dev)
     release_paged_blocks(kv, table, free, count, block_size=16, num_blocks=blocks)
     assert raised(dev) and int(count) == n and free[n - 2:].tolist() == [first + 1, first]
+
+
+# ---- slot maps with gaps -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("gap", [1, 2, 31, 32, 33, 700])
+@pytest.mark.parametrize("tokens", [0, 3000])
+def test_store_skips_what_returns_to_a_block_after_a_gap(dev, gap, tokens):
+    """A block's tokens with skipped ones between them would be two runs in one block, at the same time: the later one is left out
+    and said.  Sequences on both sides of such a gap are stored.  `tokens`: a prompt before, with which the kernel takes several
+    tokens per CTA and a warp per 16 rows."""
+    from fastdms_b200.layers.paged_attention import store_paged_kvcache
+    rng = np.random.default_rng(gap + tokens)
+    heads, d, bs = 2, 64, 32
+    blocks = 8 + -(-tokens // bs)
+    prompt = [8 * bs + i for i in range(tokens)]
+    skip = [-1] * gap
+    for after, lost in (([6, 7], 2), ([5, 6, 7], 3), ([0, 1], 2), ([bs + 3, bs + 4], 0), ([2 * bs, 2 * bs + 1], 0)):
+        slots = prompt + [3, 4] + skip + after + [-1] + [3 * bs + 9]
+        kc, vc, ks, vs = make_cache(blocks, heads, bs, d, dev, fill=0x30)
+        ks.fill_(1.0), vs.fill_(2.0 ** -3)
+        want = [codes_of(kc), codes_of(vc), np.full((blocks, heads), 1.0), np.full((blocks, heads), 2.0 ** -3)]
+        k, v = _random_rows(rng, (len(slots), heads, d), "bf16"), _random_rows(rng, (len(slots), heads, d), "bf16")
+        k[-2 - lost:] *= 16                                                  # louder: the scale would move
+        store_paged_kvcache(k.to(dev), v.to(dev), kc, vc, ks, vs, i32(slots, dev))
+        assert raised(dev) == (lost > 0)
+        kept = list(slots)
+        for i in range(lost):
+            kept[tokens + 2 + gap + i] = -1
+        O.store(n64(k), want[0], want[2], kept, bs)
+        O.store(n64(v), want[1], want[3], kept, bs)
+        check_store(kc, vc, ks, vs, want)
