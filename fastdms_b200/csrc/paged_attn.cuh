@@ -71,6 +71,10 @@ __device__ __forceinline__ int paged_len(const PagedCache& c, int b) {
     return len;
 }
 
+// A block's V scale as the weights can carry it.  The store writes 2^-60 and more; a block that nothing was stored into may hold 0,
+// whose logarithm no sum of exponents survives: it counts as 2^-60.  What is negative or NaN gives NaN.
+__device__ __forceinline__ float paged_v_scale(float vs) { return vs >= 0.0f ? fmaxf(vs, 0x1p-60f) : vs; }
+
 // Power of two that brings a row with largest magnitude `top` to [2^14, 2^15), and its inverse.
 __device__ __forceinline__ void row_power(float top, float& up, float& down) {
     const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;      // -127 for zero and subnormals, 128 for inf

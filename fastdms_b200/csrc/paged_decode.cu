@@ -271,6 +271,12 @@ __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u,
         return -1;
     };
     auto scale_of = [&](const float* s, int block) { return block >= 0 ? __ldg(s + (int64_t)block * c.heads + head) : 1.0f; };
+    float lvs, ivs;
+    auto take_vs = [&](float x) {
+        x = paged_v_scale(x);
+        lvs = paged_lg2(x);
+        ivs = __frcp_rn(x);
+    };
     int block = block_in(entry, 0), next = entry_ahead(c, seq, first, step, 32);
     float ks = scale_of(c.k_scale, block), vs = scale_of(c.v_scale, block), next_ks = 1.0f, next_vs = 1.0f;
     // Pages in registers: two at D = 64, where one is only 2 KB (8 x 8192 rows from memory 22.3 -> 19.4 us, 64 ragged up to 16384
@@ -292,7 +298,7 @@ __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u,
             load_k<D>(pg[d], page_at(kb, k_sb, k_sr, blk, d), k_sr);
             load_v<D>(pg[d], page_at(vb, v_sb, v_sr, blk, d), v_sr);
         }
-    float lvs = paged_lg2(vs), ivs = __frcp_rn(vs);
+    take_vs(vs);
     for (int i0 = 0; i0 < count; i0 += kDepth) {
 #pragma unroll
         for (int d = 0; d < kDepth; ++d) {
@@ -314,8 +320,7 @@ __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u,
             if (j == 31) {
                 block = next;
                 ks = next_ks;
-                lvs = paged_lg2(next_vs);
-                ivs = __frcp_rn(next_vs);
+                take_vs(next_vs);
                 next = entry_ahead(c, seq, first, step, i + 33);
             }
         }

@@ -614,11 +614,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         const uint32_t k_sb = (uint32_t)a.c.k_sb, k_sr = (uint32_t)a.c.k_sr, v_sb = (uint32_t)a.c.v_sb, v_sr = (uint32_t)a.c.v_sr;
         // one step ahead: the codes and scales of the next step; two ahead: its blocks
         uint4 xk[kPer], xv[kPer];
-        float ks = 0.0f, vs = 0.0f;             // 0: a page that is left out, every score -inf
+        float ks = 0.0f, vs = 0.0f;
+        bool held = false;                      // a page that is left out has every score -inf
         int blocks = look_up(0);
         auto scales = [&]() {
-            ks = vs = 0.0f;
-            if (warp == kConvWarp && blocks >= 0) {
+            held = blocks >= 0;
+            if (warp == kConvWarp && held) {
                 ks = __ldg(a.c.k_scale + (int64_t)blocks * a.c.heads + head);
                 vs = __ldg(a.c.v_scale + (int64_t)blocks * a.c.heads + head);
             }
@@ -635,7 +636,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (!ok) break;
             put(L::kK + st * L::kTile, xk);
             if (warp == kConvWarp && lane < kTileRows / kCachePage)
-                sh.page[step & (kConstRing - 1)][lane] = vs > 0.0f ? make_float4(ks, paged_lg2(vs), __frcp_rn(vs), 0.0f) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+                sh.page[step & (kConstRing - 1)][lane] = held ? make_float4(ks, paged_lg2(paged_v_scale(vs)), __frcp_rn(paged_v_scale(vs)), 0.0f)
+                                                              : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.k_full[st]);

@@ -239,3 +239,41 @@ def test_store_skips_what_returns_to_a_block_after_a_gap(dev, gap, tokens):
         O.store(n64(k), want[0], want[2], kept, bs)
         O.store(n64(v), want[1], want[3], kept, bs)
         check_store(kc, vc, ks, vs, want)
+
+
+# ---- scales that the store did not write ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("d,dt", [(64, "bf16"), (128, "f16")])
+def test_scales_of_zero_and_nan(dev, d, dt, wide):
+    """A block whose V scale is 0 holds values of 0, which count in the softmax, whatever its codes are; one of NaN makes NaN of the
+    rows that see it.  Decode and prefill say the same."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
+    rng = np.random.default_rng(d)
+    heads, group, bs, rows = 2, 4, 16, 300
+    (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, [rows], heads, bs, d, dev, loud=False)
+    if wide:
+        table = wide_table(table, bs)
+    q = _random_rows(rng, (1, heads * group, d), dt, loud=False)
+
+    def both(t, head, lens=rows):
+        args = (q.to(dev), kc, vc, ks, t, table, i32([lens], dev))
+        got = [paged_decode_attention(*args), paged_prefill_attention(*args, i32([0, 1], dev))]
+        return [n64(x)[0, head * group:(head + 1) * group] for x in got]
+
+    for zeros in ([0], [3, 4, 9], list(range(19))):
+        now = scale[1].copy()
+        now[tab[0, zeros], 1] = 0.0
+        t = torch.from_numpy(now).float().to(dev)
+        k, v = (O.rows_of(codes[c], s, tab[0], rows, 1, bs) for c, s in ((0, scale[0]), (1, now)))
+        r = slice(group, 2 * group)
+        # a code of 448 at a scale of 2^-60 in place of 0
+        out, lse, tol, ltol = O.attention(n64(q)[0, r], k, v, [rows - 1] * group, d ** -0.5)
+        for got in both(t, 1):
+            check_rows(got, None, (out, lse, tol + 448 * 2.0 ** -60, ltol), dt)
+    t = vs.clone()
+    t[int(tab[0, 5]), 0] = float("nan")
+    for got, other in zip(both(t, 0), both(t, 1)):
+        assert np.isnan(got).all() and np.isfinite(other).all()
+    for got in both(t, 0, 80):                   # its rows lie behind the last
+        assert np.isfinite(got).all()
