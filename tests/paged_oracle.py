@@ -132,7 +132,7 @@ def attention_tight(q, k, v, vs, last, scale, f16, terms=None):
     scales of the keys' blocks; `terms`: products of a score that are not zero.
 
     A weight is an f16 value, or for f16 outputs two of them: 2^-11 or 2^-22 of it, or 2^-25 where f16 has no finer steps (three
-    times: the value, the rest, a change of M).  The weights 2^(x + log2 vs - M) of a row sum to 2^7 at least (prefill; 2^11 in
+    times: the value, the rest, a change of M).  The weights 2^(x + log2 vs - M) of a row sum to 2^7 at least (prefill; 2^8 in
     decode), so that 3 * 2^-25 is 3 * 2^-32 of the sum of w_j vs_j at most; a key's term is that times v_j / vs_j."""
     n, d = q.shape
     out, lse = np.zeros((n, d)), np.full(n, -np.inf)
