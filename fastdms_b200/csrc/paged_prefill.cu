@@ -31,6 +31,7 @@ constexpr int kPreThreads = 14 * 32;
 constexpr int kConvWarp = 8, kMmaWarp = 12;
 constexpr int kConstRing = 4;                   // steps whose page constants are held: the softmax may lag two behind
 constexpr uint64_t kPreWaitNs = 1000000000;     // a wait gives up after a second
+constexpr int kDrainPolls = 10000000;            // of 100 ns: the wait for what was issued gives up after a second too
 constexpr uint32_t kTmemCols = 512;
 
 struct PrefillArgs {
@@ -290,7 +291,7 @@ struct PrefillSmem {
 };
 
 struct PrefillShared {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][3], p_full[2][3], pv_done[2][3];
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][3], p_full[2][3], pv_done[2][3], drain[2];
     float4 page[kConstRing][kTileRows / kCachePage];            // ks, log2 vs, 1 / vs of the step's pages
     uint32_t tmem;
     int give_up, nan_lo, nan_hi;
@@ -301,9 +302,10 @@ __device__ __forceinline__ bool elected() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
 }
-// Scores of tile ti against the half h of the keys in stage st; the weights of tile ti times the values of that half.
+// Scores of tile ti against the half h of the keys in stage st; the weights of tile ti times the values of that half.  `again`: the stage
+// will be filled again, and that waits for the products; an arrival that nobody waits for might come after the CTA's end.
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, PrefillShared& sh) {
+__device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, bool again, PrefillShared& sh) {
     using L = PrefillSmem<D>;
     const uint64_t q = operand(base + L::kQ + ti * L::kTile, 16, 1024), k = operand(base + L::kK + st * L::kTile + h * (kHalf * 128), 16, 1024);
 #pragma unroll
@@ -312,10 +314,10 @@ __device__ __forceinline__ void issue_scores(uint32_t base, uint32_t tmem, int t
         mma_ss(tmem + (L::kBufs * ti + buf) * kHalf, q + step, k + step, instruction(kHalf, false), i > 0);
     }
     tc_commit(&sh.s_full[ti][buf]);
-    tc_commit(&sh.k_empty[st]);
+    if (again) tc_commit(&sh.k_empty[st]);
 }
 template <int D, bool FINE>
-__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, bool add, PrefillShared& sh) {
+__device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int ti, int st, int h, int buf, bool add, bool again, PrefillShared& sh) {
     using L = PrefillSmem<D>;
     const uint64_t v = operand(base + L::kV + st * L::kTile + h * (kHalf * 128), kSlab, 1024);
 #pragma unroll
@@ -326,7 +328,7 @@ __device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int t
         for (int i = 0; i < kHalf / 16; ++i)
             mma_ts(tmem + L::kO + D * ti, tmem + (L::kBufs * ti + buf) * kHalf + 32 + 8 * i, v + (i * 2048 >> 4), instruction(D, true), true);
     tc_commit(&sh.pv_done[ti][buf]);
-    tc_commit(&sh.v_empty[st]);
+    if (again) tc_commit(&sh.v_empty[st]);
 }
 
 template <int D, bool BF16>
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             bar_init(&sh.v_full[i], 4);
             bar_init(&sh.k_empty[i], 2 * tiles);
             bar_init(&sh.v_empty[i], 2 * tiles);
+            bar_init(&sh.drain[i], 1);
             for (int k = 0; k < 3; ++k) {
                 bar_init(&sh.s_full[i][k], 1);
                 bar_init(&sh.p_full[i][k], 4);
@@ -680,9 +683,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
         const uint32_t base = s_addr(tile), t0 = __shfl_sync(0xffffffffu, tmem, 0);
         bool ok = warp_wait(&sh.q_full, 0, give_up);
         auto scores = [&](int h, int buf) {
+            const bool again = (h >> 1) + 2 < steps;
             if (elected()) {
-                if (h & 2) { if (h & 1) issue_scores<D>(base, t0, ti, 1, 1, buf, sh); else issue_scores<D>(base, t0, ti, 1, 0, buf, sh); }
-                else { if (h & 1) issue_scores<D>(base, t0, ti, 0, 1, buf, sh); else issue_scores<D>(base, t0, ti, 0, 0, buf, sh); }
+                if (h & 2) { if (h & 1) issue_scores<D>(base, t0, ti, 1, 1, buf, again, sh); else issue_scores<D>(base, t0, ti, 1, 0, buf, again, sh); }
+                else { if (h & 1) issue_scores<D>(base, t0, ti, 0, 1, buf, again, sh); else issue_scores<D>(base, t0, ti, 0, 0, buf, again, sh); }
             }
             __syncwarp();
         };
@@ -696,9 +700,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             ok = warp_wait(&sh.v_full[(h >> 1) & 1], (h >> 2) & 1, give_up) && warp_wait(&sh.p_full[ti][buf], turn, give_up);
             if (!ok) break;
             tc_fence_after();
+            const bool again = (h >> 1) + 2 < steps;
             if (elected()) {
-                if (h & 2) { if (h & 1) issue_values<D, kFine>(base, t0, ti, 1, 1, buf, true, sh); else issue_values<D, kFine>(base, t0, ti, 1, 0, buf, true, sh); }
-                else { if (h & 1) issue_values<D, kFine>(base, t0, ti, 0, 1, buf, true, sh); else issue_values<D, kFine>(base, t0, ti, 0, 0, buf, h > 0, sh); }
+                if (h & 2) {
+                    if (h & 1) issue_values<D, kFine>(base, t0, ti, 1, 1, buf, true, again, sh);
+                    else issue_values<D, kFine>(base, t0, ti, 1, 0, buf, true, again, sh);
+                } else {
+                    if (h & 1) issue_values<D, kFine>(base, t0, ti, 0, 1, buf, true, again, sh);
+                    else issue_values<D, kFine>(base, t0, ti, 0, 0, buf, h > 0, again, sh);
+                }
             }
             __syncwarp();
             const int next = h + L::kBufs;
@@ -710,13 +720,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             }
             if (++buf == L::kBufs) { buf = 0; turn ^= 1; }
         }
-        // nothing of this CTA may be in flight when its memory goes
-        if (ok) {
-            warp_wait(&sh.pv_done[ti][(halves - 1) % L::kBufs], ((halves - 1) / L::kBufs) & 1, give_up);
-        } else {                                // after a wait that ran out: let what was issued complete
-            if (elected()) tc_commit(&sh.q_full);
-            for (int i = 0; i < 100 && !bar_test(&sh.q_full, 1); ++i) __nanosleep(10000);
-        }
+        // nothing of this CTA may be in flight when its memory goes, after a wait that ran out neither
+        if (elected()) tc_commit(&sh.drain[ti]);
+        for (int i = 0; i < kDrainPolls && !bar_test(&sh.drain[ti], 0); ++i) __nanosleep(100);
     }
     __syncwarp();
     tc_fence_before();

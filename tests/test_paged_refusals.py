@@ -1,6 +1,9 @@
 """What the paged cache's calls refuse, on the CPU: nothing here launches a kernel."""
 from __future__ import annotations
 
+import re
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -209,3 +212,17 @@ def test_release_refuses_the_number_of_blocks():
     rel = dict(rows=PTR, listed=2, kv=PTR, n=2, bt=PTR, stride=4, cols=4, bs=16, free=PTR, capacity=8, blocks=9, count=PTR, status=None, stream=None)
     for change, code, words in [(dict(blocks=-1), E, b"negative"), (dict(blocks=1 << 28), C, b"31 bits"), (dict(listed=5000), C, b"rows a call")]:
         assert lib.fdms_paged_release_pool(*(rel | change).values()) == code and words in lib.fdms_last_error()
+
+
+def test_prefill_drains_on_a_barrier_of_its_own():
+    """Before the prefill kernel gives its tensor memory back it waits for the products that it issued, also after a wait that ran
+    out.  An mbarrier completes a phase with as many arrivals as it was initialised with, and a commit is one: the barrier of
+    that wait must take one arrival, from that commit alone, and be waited for in its first phase."""
+    src = (Path(__file__).resolve().parent.parent / "fastdms_b200" / "csrc" / "paged_prefill.cu").read_text()
+    tail = src[src.index("nothing of this CTA may be in flight"):src.index("tcgen05.dealloc")]
+    commits = re.findall(r"tc_commit\(&sh\.(\w+)", tail)
+    waits = re.findall(r"bar_\w+\(&sh\.(\w+)(?:\[\w+\])?, (\d)", tail)
+    assert len(commits) == 1 and waits == [(commits[0], "0")]
+    counts = re.findall(rf"bar_init\(&sh\.{commits[0]}(?:\[\w+\])?, (\w+)\)", src)
+    assert counts == ["1"]
+    assert len(re.findall(rf"sh\.{commits[0]}\b", src)) == 3                  # its start, the commit and the wait
