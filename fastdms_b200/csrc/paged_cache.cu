@@ -515,6 +515,10 @@ extern "C" int32_t fdms_paged_metadata(const fdms_paged_metadata_args* args, voi
                  "fdms_paged_metadata: negative size, or rows of the block table overlap");
     FDMS_REQUIRE((((uintptr_t)p.slot_mapping | (uintptr_t)p.positions) & 15) == 0, FDMS_E_ARG,
                  "fdms_paged_metadata: slot_mapping and positions must be 16-byte aligned");
+    // The scan reads the lengths of kScanThreads requests and then writes theirs: what it writes must not lie ahead of what it reads.
+    auto ahead = [&](const int32_t* in) { return (const int32_t*)p.kv_lens_out > in && p.kv_lens_out < in + p.num_seqs; };
+    FDMS_REQUIRE(p.num_seqs <= kScanThreads || (!ahead(p.new_lens) && !ahead(p.kv_lens)), FDMS_E_ARG,
+                 "fdms_paged_metadata: kv_lens_out begins inside new_lens or kv_lens, behind their first element");
     FDMS_REQUIRE(p.total_tokens < 0x7fffffff && p.num_seqs < 0x7fffffff && p.free_capacity <= (0x7fffffff >> shift) && p.max_blocks <= (0x7fffffff >> shift),
                  FDMS_E_CAPACITY, "fdms_paged_metadata: token and slot numbers must fit in 31 bits");
     const MetaArgs a = {p.new_lens, p.kv_lens, p.kv_lens_out, p.block_tables, p.bt_stride, p.free_blocks, p.free_capacity, p.free_count,

@@ -136,7 +136,8 @@ def build_paged_metadata(
     the lengths).  A negative length, one beyond the table's columns, or more tokens than `total_tokens` are not served
     either and raise the device status bit for bad indices.
 
-    `kv_lens` and `free_count` are advanced in place, or left alone where `kv_lens_out` / `free_count_out` are given.
+    `kv_lens` and `free_count` are advanced in place, or left alone where `kv_lens_out` / `free_count_out` are given
+    (`kv_lens_out` may be `new_lens`; otherwise they overlap no other argument).
     Returns `cu_seqlens` (int32 `[n + 1]`), `slot_mapping` (int32 `[total_tokens]`, block * block_size + row) and
     `positions` (int64 `[total_tokens]`); buffers given for them are
     filled, and overlap no other argument.  `total_tokens` may exceed the sum of `new_lens`

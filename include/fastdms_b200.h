@@ -504,7 +504,8 @@ int32_t fdms_linear_decode_allreduce(
  *   free_blocks[0 .. free_count) (the top is the end) into its row of the table, in the order of the sequences; where the
  *   stack runs out a sequence and the later ones that need blocks are not served: slots -1, length and table as before.
  *   cu_seqlens [num_seqs + 1] = prefix sums of new_lens; slot_mapping and positions [total_tokens], 16-byte aligned
- *   (tokens behind the last: -1 and 0).  kv_lens_out / free_count_out may be kv_lens / free_count.  A negative length, one
+ *   (tokens behind the last: -1 and 0).  kv_lens_out / free_count_out may be kv_lens / free_count (kv_lens_out new_lens
+ *   too, but not a later part of either).  A negative length, one
  *   beyond max_blocks * block_size, or more tokens than total_tokens is not served and raises FDMS_DEV_BAD_INDEX.
  *   workspace: fdms_paged_metadata_workspace_bytes(...) bytes, 8-byte aligned, any contents.
  * fdms_paged_release_pool: the blocks of rows[0 .. num_listed) (NULL: rows 0 .. num_listed) return to the stack; their

@@ -226,3 +226,14 @@ def test_prefill_drains_on_a_barrier_of_its_own():
     counts = re.findall(rf"bar_init\(&sh\.{commits[0]}(?:\[\w+\])?, (\w+)\)", src)
     assert counts == ["1"]
     assert len(re.findall(rf"sh\.{commits[0]}\b", src)) == 3                  # its start, the commit and the wait
+
+
+def test_c_metadata_refuses_lengths_over_later_ones():
+    """Beyond one round of the scan, a length written ahead of those still to be read would change them."""
+    lib, n = _lib.lib(), 3000
+    far = dict(n=n, new=PTR, kv=PTR + 4 * n, total=1 << 20, ws=PTR, ws_bytes=0)        # refused at the latest for its workspace
+    for out, code, words in [(PTR + 4, E, b"kv_lens_out"), (PTR + 4 * n - 4, E, b"kv_lens_out"), (PTR + 4 * n + 4, E, b"kv_lens_out"),
+                             (PTR, W, b"workspace"), (PTR + 4 * n, W, b"workspace"), (PTR + 8 * n, W, b"workspace")]:
+        assert lib.fdms_paged_metadata(P._METADATA_ARGS.pack(*(METADATA | far | dict(kv_out=out)).values()), None) == code and words in lib.fdms_last_error()
+    near = far | dict(n=1024, kv=PTR + 4 * n, kv_out=PTR + 4)                # one round reads all lengths before it writes any
+    assert lib.fdms_paged_metadata(P._METADATA_ARGS.pack(*(METADATA | near).values()), None) == W
