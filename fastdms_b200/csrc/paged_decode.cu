@@ -748,9 +748,9 @@ extern "C" int32_t fdms_paged_attn_decode(const fdms_paged_attn_args* args, void
                  "fdms_paged_attn_decode: workspace missing, unaligned or smaller than %lld bytes", (long long)need);
     a.parts = (float*)p.workspace;
     a.cuts = (int2*)((char*)p.workspace + decode_parts_bytes(sms, head_dim));
-    const int64_t rows_held = (int64_t)batch * p.max_blocks * (p.cache.block_size / kCachePage);
-    FDMS_REQUIRE(rows_held < (1ll << 30), FDMS_E_CAPACITY, "fdms_paged_attn_decode: the block tables hold too many rows");
-    const int64_t useful = (rows_held * num_kv_heads * a.splits + 2 * kDecWarps - 1) / (2 * kDecWarps);
+    const int64_t pages_held = (int64_t)batch * p.max_blocks * (p.cache.block_size / kCachePage);
+    FDMS_REQUIRE(pages_held + (int64_t)batch * kUnitPages <= 0x7fffffff, FDMS_E_CAPACITY, "fdms_paged_attn_decode: the block tables hold too many rows");
+    const int64_t useful = (pages_held * num_kv_heads * a.splits + 2 * kDecWarps - 1) / (2 * kDecWarps);
     const unsigned grid = (unsigned)(useful < 1 ? 1 : useful < (int64_t)sms * kDecCtasPerSm ? useful : (int64_t)sms * kDecCtasPerSm);
     const size_t smem = (size_t)(batch + 1) * sizeof(int32_t);
     const int64_t rows = (int64_t)batch * num_q_heads;

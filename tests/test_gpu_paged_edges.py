@@ -277,3 +277,30 @@ def test_scales_of_zero_and_nan(dev, d, dt, wide):
         assert np.isnan(got).all() and np.isfinite(other).all()
     for got in both(t, 0, 80):                   # its rows lie behind the last
         assert np.isfinite(got).all()
+
+
+# ---- sizes ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("pages", [(1 << 30) + 5, (1 << 31) - 1 - 2048 * 24])
+def test_decode_of_tables_for_very_many_rows(dev, pages):
+    """The pages that the tables may hold are counted in 31 bits: 2048 sequences of which two hold rows, all with the same wide row."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention
+    rng = np.random.default_rng(3)
+    seqs, bs, d, rows = 2048, 16, 64, 900
+    (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, [rows], 1, bs, d, dev)
+    cols = pages // seqs
+    wide = torch.full((1, cols), -1, dtype=torch.int32, device=dev)
+    wide[:, :table.shape[1]] = table
+    lens = [0] * seqs
+    lens[3], lens[2047] = rows, 70
+    q = _random_rows(rng, (seqs, 2, d), "bf16", loud=False)
+    got = n64(paged_decode_attention(q.to(dev), kc, vc, ks, vs, wide.expand(seqs, cols), i32(lens, dev)))
+    for b in (3, 2047):
+        k, v = (O.rows_of(codes[c], scale[c], tab[0], lens[b], 0, bs) for c in range(2))
+        check_rows(got[b], None, O.attention(n64(q)[b], k, v, [lens[b] - 1] * 2, d ** -0.5), "bf16")
+    got[[3, 2047]] = 0
+    assert (got == 0).all()
+    with pytest.raises(RuntimeError, match="too many rows"):
+        cols = ((1 << 31) - 1) // seqs + 1
+        wide = torch.full((1, cols), -1, dtype=torch.int32, device=dev)
+        paged_decode_attention(q.to(dev), kc, vc, ks, vs, wide.expand(seqs, cols), i32([0] * seqs, dev))
