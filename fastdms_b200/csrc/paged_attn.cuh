@@ -78,7 +78,7 @@ __device__ __forceinline__ float paged_v_scale(float vs) { return vs >= 0.0f ? f
 // Power of two that brings a row with largest magnitude `top` to [2^14, 2^15), and its inverse.
 __device__ __forceinline__ void row_power(float top, float& up, float& down) {
     const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;      // -127 for zero and subnormals, 128 for inf
-    const int k = min(max(14 - e, -100), 100);
+    const int k = min(14 - e, 126);             // both powers are normal numbers for every e
     up = __uint_as_float((uint32_t)(127 + k) << 23);
     down = __uint_as_float((uint32_t)(127 - k) << 23);
 }

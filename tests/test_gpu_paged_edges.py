@@ -304,3 +304,27 @@ def test_decode_of_tables_for_very_many_rows(dev, pages):
         cols = ((1 << 31) - 1) // seqs + 1
         wide = torch.full((1, cols), -1, dtype=torch.int32, device=dev)
         paged_decode_attention(q.to(dev), kc, vc, ks, vs, wide.expand(seqs, cols), i32([0] * seqs, dev))
+
+
+# ---- queries -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("power", [122, 114, 100, -100, -125])
+def test_queries_at_the_ends_of_bfloat16(dev, power, wide):
+    """Queries near bf16's largest and smallest numbers, with a scale that brings the scores back."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
+    rng = np.random.default_rng(power + 200)
+    heads, group, bs, d, rows = 1, 8, 16, 64, 90
+    (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, [rows], heads, bs, d, dev, loud=False)
+    if wide:
+        table = wide_table(table, bs)
+    x = np.clip(rng.standard_normal((1, heads * group, d)), -1.9, 1.9)
+    q = torch.from_numpy(x * 2.0 ** power).to(torch.bfloat16)
+    small = q.abs().double() < 2.0 ** -126                                   # what bf16 holds as a subnormal counts as 0
+    q = torch.where(small, torch.zeros_like(q), q)
+    back = 2.0 ** (-3 - power)
+    args = (q.to(dev), kc, vc, ks, vs, table, i32([rows], dev))
+    k, v = (O.rows_of(codes[c], scale[c], tab[0], rows, 0, bs) for c in range(2))
+    want = O.attention(n64(q)[0], k, v, [rows - 1] * group, back)
+    for got in (paged_decode_attention(*args, back), paged_prefill_attention(*args, i32([0, 1], dev), back)):
+        check_rows(n64(got)[0], None, want, "bf16")
