@@ -259,7 +259,11 @@ __device__ __forceinline__ int entry_ahead(const PagedCache& c, int seq, int fir
 template <int D, bool FINE>
 __device__ __forceinline__ void walk_pages(const PagedCache& c, UnitState<D>& u, const uint32_t (&qb)[D / 16][2], const float (&factor)[2],
                                            int seq, int head, int first, int step, int count, int len, int entry) {
-    if (c.num_blocks == 0 || count <= 0) return;
+    if (count <= 0) return;
+    if (c.num_blocks == 0) {                    // a needed page that no block is
+        if (c.status) atomicOr(c.status, FDMS_DEV_BAD_INDEX);
+        return;
+    }
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int in_block = (1 << (c.shift - 4)) - 1;
     const uint32_t k_sr = (uint32_t)c.k_sr, v_sr = (uint32_t)c.v_sr;

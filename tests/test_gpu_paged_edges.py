@@ -328,3 +328,19 @@ def test_queries_at_the_ends_of_bfloat16(dev, power, wide):
     want = O.attention(n64(q)[0], k, v, [rows - 1] * group, back)
     for got in (paged_decode_attention(*args, back), paged_prefill_attention(*args, i32([0, 1], dev), back)):
         check_rows(n64(got)[0], None, want, "bf16")
+
+
+# ---- caches --------------------------------------------------------------------------------------------------------
+
+def test_a_cache_without_blocks(dev):
+    """Rows that no block can hold are left out and said, by both forms; without rows nothing is wrong."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
+    cache = make_cache(0, 1, 16, 64, dev)
+    q = torch.ones((2, 4, 64), dtype=torch.bfloat16, device=dev)
+    for cols in (2, 5000):
+        table = torch.zeros((2, cols), dtype=torch.int32, device=dev)
+        for lens in ([0, 0], [3, 0]):
+            assert (paged_decode_attention(q, *cache, table, i32(lens, dev)) == 0).all()
+            assert raised(dev) == any(lens)
+            assert (paged_prefill_attention(q, *cache, table, i32(lens, dev), i32([0, 1, 2], dev)) == 0).all()
+            assert raised(dev) == any(lens)
