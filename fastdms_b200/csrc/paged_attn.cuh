@@ -140,6 +140,7 @@ inline int32_t paged_cache_check(const char* name, const fdms_paged_cache& c, in
     if (idle || c.num_blocks == 0) return FDMS_OK;
     FDMS_REQUIRE(c.k && c.v && c.k_scale && c.v_scale, FDMS_E_ARG, "%s: null pointer", name);
     const int64_t strides = c.k_stride[0] | c.k_stride[1] | c.k_stride[2] | c.v_stride[0] | c.v_stride[1] | c.v_stride[2];
+    FDMS_REQUIRE(strides >= 0, FDMS_E_ARG, "%s: negative stride of the cache", name);
     FDMS_REQUIRE((((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)strides) & 15) == 0 && c.k_stride[3] == 1 && c.v_stride[3] == 1, FDMS_E_ARG,
                  "%s: the cache must be contiguous in its last dimension and aligned to 16 bytes in the others", name);
     return FDMS_OK;

@@ -534,7 +534,7 @@ typedef struct fdms_paged_cache {
     uint8_t *k, *v;                     /* e4m3 [num_blocks, kv_heads, block_size, head_dim] */
     float *k_scale, *v_scale;           /* [num_blocks, kv_heads], contiguous */
     int64_t num_blocks, kv_heads, block_size, head_dim;
-    int64_t k_stride[4], v_stride[4];   /* block, head, row (multiples of 16), channel (1), in bytes */
+    int64_t k_stride[4], v_stride[4];   /* block, head, row (multiples of 16, not negative), channel (1), in bytes */
 } fdms_paged_cache;
 
 typedef struct fdms_paged_metadata_args {

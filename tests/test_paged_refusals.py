@@ -237,3 +237,12 @@ def test_c_metadata_refuses_lengths_over_later_ones():
         assert lib.fdms_paged_metadata(P._METADATA_ARGS.pack(*(METADATA | far | dict(kv_out=out)).values()), None) == code and words in lib.fdms_last_error()
     near = far | dict(n=1024, kv=PTR + 4 * n, kv_out=PTR + 4)                # one round reads all lengths before it writes any
     assert lib.fdms_paged_metadata(P._METADATA_ARGS.pack(*(METADATA | near).values()), None) == W
+
+
+@pytest.mark.parametrize("name", ["k0", "k1", "k2", "v0", "v1", "v2"])
+def test_c_calls_refuse_negative_strides(name):
+    """Block and row strides are taken as unsigned 32-bit numbers: a negative one would read far behind the cache."""
+    lib, bad = _lib.lib(), {name: -2048}
+    for fn, args in ((lib.fdms_paged_store, P._STORE_ARGS.pack(*(STORE | bad).values())), (lib.fdms_paged_attn_decode, P._ATTN_ARGS.pack(*(ATTN | bad).values())),
+                     (lib.fdms_paged_attn_prefill, P._ATTN_ARGS.pack(*(ATTN | bad).values()))):
+        assert fn(args, None) == E and b"negative stride" in lib.fdms_last_error()
