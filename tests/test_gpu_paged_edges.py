@@ -7,8 +7,8 @@ import pytest
 import torch
 
 import paged_oracle as O
-from test_gpu_paged_attention import (DT, Run, _random_rows, _status_clean, build_case, check_rows, check_store, codes_of, dev, i32, make_cache,  # noqa: F401
-                                      n64, raised, wide_table)
+from test_gpu_paged_attention import (DT, Run, _random_rows, _status_clean, build_case, check_prefill, check_rows, check_store, codes_of,  # noqa: F401
+                                      dev, i32, make_cache, n64, raised, wide_table)
 
 pytestmark = pytest.mark.gpu
 
@@ -344,3 +344,54 @@ def test_a_cache_without_blocks(dev):
             assert raised(dev) == any(lens)
             assert (paged_prefill_attention(q, *cache, table, i32(lens, dev), i32([0, 1, 2], dev)) == 0).all()
             assert raised(dev) == any(lens)
+
+
+# ---- prefill beside itself -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cols", [20, 2500])
+def test_prefill_on_two_streams_and_captured(dev, cols):
+    """Prompt steps of two servers on two streams without any wait between them, eager and from graphs; with wide tables the rows are
+    cut into parts, whose workspaces must not meet."""
+    runs = [Run(dev, 21, cols=cols, pool=90), Run(dev, 22, d=128, dt="f16", cols=cols, pool=90)]
+    streams = [torch.cuda.Stream(dev) for _ in runs]
+    step = [9, 0, 40, 3]
+    for r in runs:
+        r.step([60, 120, 7, 100])
+    jobs = []
+    for r, s in zip(runs, streams):
+        ins = [r.inputs(sum(step)) for _ in range(3)]
+        jobs.append((r, s, i32(step, dev), ins, [tuple(x.to(dev) for x in t) for t in ins], []))
+    torch.cuda.synchronize(dev)
+    for i in range(3):
+        for r, s, new, ins, on, got in jobs:
+            with torch.cuda.stream(s):
+                got.append(r.call(new, *on[i], False))
+                got[-1] += tuple(x.clone() for x in (r.kv, r.table))
+    torch.cuda.synchronize(dev)
+    for r, s, new, ins, on, got in jobs:
+        cu = np.concatenate([[0], np.cumsum(step)])
+        for (q, k, v), (out, slots, kv, table) in zip(ins, got):
+            for c, x in ((0, k), (1, v)):
+                O.store(n64(x), r.codes[c], r.scale[c], slots.cpu().tolist(), r.bs)
+            check_prefill(n64(out), None, n64(q), cu, [(a, int(m)) for a, m in zip(step, kv.tolist())], (r.codes, r.scale, table.cpu().numpy()),
+                          r.heads, r.group, r.bs, r.d, r.dt)
+    graphs = []
+    for r, s, new, ins, on, got in jobs:
+        g, live = torch.cuda.CUDAGraph(), [x.clone() for x in on[0]]
+        with torch.cuda.graph(g, stream=s):
+            out, slots = r.call(new, *live, False)
+        graphs.append((r, s, g, new, live, out, slots))
+    for _ in range(2):
+        fed = []
+        for r, s, g, new, live, out, slots in graphs:
+            ins = r.inputs(sum(step))
+            for x, y in zip(live, ins):
+                x.copy_(y)
+            fed.append(ins)
+        torch.cuda.synchronize(dev)
+        for r, s, g, new, live, out, slots in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize(dev)
+        for (r, s, g, new, live, out, slots), ins in zip(graphs, fed):
+            r.check(step, *ins, out, slots)
