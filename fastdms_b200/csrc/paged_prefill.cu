@@ -638,9 +638,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (step >= 2) ok = warp_wait(&sh.k_empty[st], ((step >> 1) - 1) & 1, give_up);
             if (!ok) break;
             put(L::kK + st * L::kTile, xk);
-            if (warp == kConvWarp && lane < kTileRows / kCachePage)
-                sh.page[step & (kConstRing - 1)][lane] = held ? make_float4(ks, paged_lg2(paged_v_scale(vs)), __frcp_rn(paged_v_scale(vs)), 0.0f)
+            if (warp == kConvWarp && lane < kTileRows / kCachePage) {
+                const float v = paged_v_scale(vs);          // a NaN is in the scores; 1 / vs also meets rows that do not see the page
+                sh.page[step & (kConstRing - 1)][lane] = held ? make_float4(ks, paged_lg2(v), v == v ? __frcp_rn(v) : 1.0f, 0.0f)
                                                               : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+            }
             fence_async_shared();
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.k_full[st]);

@@ -277,6 +277,12 @@ def test_scales_of_zero_and_nan(dev, d, dt, wide):
         assert np.isnan(got).all() and np.isfinite(other).all()
     for got in both(t, 0, 80):                   # its rows lie behind the last
         assert np.isfinite(got).all()
+    # a prompt: the rows before the block's do not see it
+    n, first = 250, int(5 * bs)
+    q = _random_rows(rng, (n, heads * group, d), dt, loud=False)
+    for at in (table, table[:, :-(-rows // bs)]):
+        clean, got = (n64(paged_prefill_attention(q.to(dev), kc, vc, ks, x, at, i32([n], dev), i32([0, n], dev))) for x in (vs, t))
+        assert np.isnan(got[first:, :group]).all() and np.array_equal(got[:first], clean[:first]) and np.array_equal(got[:, group:], clean[:, group:])
 
 
 # ---- sizes ---------------------------------------------------------------------------------------------------------
