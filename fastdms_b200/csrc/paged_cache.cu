@@ -348,11 +348,18 @@ __device__ __noinline__ int32_t slot_before(const int32_t* slots, int64_t first,
     const unsigned below = __ballot_sync(0xffffffffu, my_slot >= 0) & ((1u << lane) - 1);
     const int32_t near = __shfl_sync(0xffffffffu, my_slot, below ? 31 - __clz(below) : 0);
     int32_t before = __shfl_sync(0xffffffffu, prev, 0);
-    for (int64_t end = first - 1; before < 0 && end > 0; end -= 32) {
-        const int64_t t = end - 32 + lane;
-        const int32_t x = t >= 0 ? __ldg(slots + t) : -1;
-        const unsigned m = __ballot_sync(0xffffffffu, x >= 0);
-        if (m) before = __shfl_sync(0xffffffffu, x, 31 - __clz(m));
+    for (int64_t end = first - 1; before < 0 && end > 0; end -= 256) {
+        int32_t x[8];                           // 256 slots, the nearest first
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t t = end - 32 * (i + 1) + lane;
+            x[i] = t >= 0 ? __ldg(slots + t) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned m = __ballot_sync(0xffffffffu, x[i] >= 0);
+            if (m && before < 0) before = __shfl_sync(0xffffffffu, x[i], 31 - __clz(m));
+        }
     }
     return below ? near : before;
 }

@@ -212,7 +212,7 @@ def test_release_into_a_stack_of_part_of_the_pool(dev, first, blocks):
 
 # ---- slot maps with gaps -------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("gap", [1, 2, 31, 32, 33, 700])
+@pytest.mark.parametrize("gap", [1, 2, 31, 32, 33, 255, 257, 700])
 @pytest.mark.parametrize("tokens", [0, 3000])
 def test_store_skips_what_returns_to_a_block_after_a_gap(dev, gap, tokens):
     """A block's tokens with skipped ones between them would be two runs in one block, at the same time: the later one is left out
