@@ -6,8 +6,8 @@
 // earlier ones moves the earlier codes to the larger scale, which is an exponent shift (exact down to e4m3's
 // subnormals).
 //
-// Measured: tables of a decode step of 256 requests 5.6 us, of 64 prompts of up to 32768 tokens (a million slots) 8.5 us; a store
-// of 256 tokens into as many blocks 5 us (8 KV heads of 128), of 16 K prompt tokens 20 us: 101.6 MB read and written, 5.1 TB/s.
+// Measured: tables of a decode step of 256 requests 5.7 us, of 64 prompts of up to 32768 tokens (a million slots) 8.5 us; a store
+// of 256 tokens into as many blocks 5 us (8 KV heads of 128), of 16 K prompt tokens 21 us: 101.6 MB read and written, 4.8 TB/s.
 #include "paged_attn.cuh"
 
 namespace fdms {
@@ -497,7 +497,7 @@ static int32_t block_shift(int64_t block_size) {
     return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
 }
 
-// One CTA does all of a decode step in one launch (256 requests: 5.6 us).  Beyond kFusedTokens its writes are what takes time,
+// One CTA does all of a decode step in one launch (256 requests: 5.7 us).  Beyond kFusedTokens its writes are what takes time,
 // and a second launch spreads them over the GPU: 2 K tokens take 5.0 us with one and 5.7 with two, 8 K 8.1 and 5.7, 16 K 12
 // and 5.7; the second launch and its workspace cost 6 us of host time.
 constexpr int64_t kFusedTokens = 4 * kScanThreads * kFillTokens;

@@ -9,9 +9,9 @@
 //   shares    the pages of all units laid end to end, every CTA taking an equal share of them, so that ragged lengths leave
 //             no SM idle and no host has to know a length.  A unit that one CTA holds whole is written at once; parts of a
 //             unit that is cut go to a workspace, and a second launch, started while this one runs, joins them.
-// Measured from memory (bf16, 32 q heads on 8 KV heads): 64 sequences ragged up to 16384 rows at head_dim 128 read their 1.08 GB in
-// 188 us (5.7 TB/s); 8 x 8192 rows at head_dim 64 their 67 MB in 20.0 us (3.4 TB/s), of which about 5 are launch, merge and join;
-// one sequence of 200 rows takes 5.7 us, a chain of latencies.
+// Measured from memory (32 q heads on 8 KV heads): 64 sequences ragged up to 16384 rows at head_dim 128 read their 1.08 GB in
+// 190 us (5.7 TB/s) in bf16 and 199 in f16; 8 sequences at head_dim 64 take about 6 us and then read at 4.9 TB/s (8192 rows: 67 MB in
+// 20 us, f16 21); one sequence of 200 rows takes 5.7 us, a chain of latencies.
 #include "paged_attn.cuh"
 
 #include <algorithm>

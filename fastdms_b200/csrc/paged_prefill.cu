@@ -10,14 +10,16 @@
 //                    one warp per tile: one for both spent more on waiting and issuing (800 cycles for each of the eight
 //                    batches of 128 keys) than the products take
 // Tensor memory holds O of both tiles (2 x D columns) and for each two (D = 64: three) buffers of S, 64 keys wide, P over the
-// S it comes from: the scores of 64 keys are computed while the 64 before them are weighed, so that the softmax, which bounds this
-// kernel (one exponential per score: 16 a cycle and SM), does not wait for the products.  Two tiles per CTA halve the
-// conversions.  Every wait is bounded; when one runs out the CTA raises FDMS_DEV_WAIT_TIMEOUT, gives its tensor memory back
-// and returns.
+// S it comes from: the scores of 64 keys are computed while the 64 before them are weighed, so that the softmax does not wait for
+// their product.  Two tiles per CTA halve the conversions.  Every wait is bounded; when one runs out the CTA raises
+// FDMS_DEV_WAIT_TIMEOUT, lets what it issued complete, gives its tensor memory back and returns.
 //
-// Measured (bf16, 32 q heads on 8 KV heads, a B200): 2048 tokens over 16384 rows at head_dim 128 take 610 us, 845 TFLOP/s; of the
-// SMs' active time the tensor pipe works 45 %, the unit of the exponential 45 %, and the 256 equal CTAs on 148 SMs leave a
-// seventh of the second wave idle.  7 ragged prompts of up to 3001 tokens at head_dim 64 take 350 us.
+// Measured (32 q heads on 8 KV heads, a B200): 2048 tokens over 16384 rows at head_dim 128 take 571 us in bf16 (902 TFLOP/s) and 795 in
+// f16, whose weights take a second product; 7 ragged prompts of up to 3001 tokens at head_dim 64 353 and 440 us.  No unit bounds
+// it: of the SMs' active time the tensor pipe works 48 %, the unit of the exponential 49 %, and an instruction issues in 46 % of the
+// cycles.  A step of 128 keys takes about 2.4 us at both head sizes, where its exponentials need 1.1: each softmax warp goes through
+// load, weights, store and arrival in turn, and the two of a scheduler do not fill each other's waits.  256 equal CTAs on 148 SMs
+// run in two waves and leave 14 % of them idle.
 //
 // Few tokens over many rows would leave most SMs idle: the rows are then cut into parts for a CTA each, whose results go to a
 // workspace and are joined by a second launch.
@@ -31,7 +33,7 @@ constexpr int kPreThreads = 14 * 32;
 constexpr int kConvWarp = 8, kMmaWarp = 12;
 constexpr int kConstRing = 4;                   // steps whose page constants are held: the softmax may lag two behind
 constexpr uint64_t kPreWaitNs = 1000000000;     // a wait gives up after a second
-constexpr int kDrainPolls = 10000000;            // of 100 ns: the wait for what was issued gives up after a second too
+constexpr int kDrainPolls = 10000000;           // of 100 ns: the wait for what was issued gives up after a second too
 constexpr uint32_t kTmemCols = 512;
 
 struct PrefillArgs {

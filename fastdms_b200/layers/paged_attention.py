@@ -31,9 +31,7 @@ import torch
 from fastdms_b200 import _lib
 
 BLOCK_SIZES = (16, 32, 64, 128)
-HEAD_DIMS = (64, 128)
 MAX_DECODE_BATCH = 2048
-MAX_RELEASE_ROWS = 4096
 
 # The argument blocks of include/fastdms_b200.h; every member is 8 bytes wide.
 _METADATA_ARGS = Struct("12P7q")
