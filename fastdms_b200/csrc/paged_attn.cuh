@@ -6,9 +6,9 @@
 //   P_j = 2^(x_j + log2 vs_j - M),  out = sum_j P_j vcode_j / l,  l = sum_j P_j / vs_j,
 // so that P is always fit for 16 bits whatever the blocks' magnitudes are, and a block with small values does not
 // disturb one with large ones.  Scales lie in [2^-60, 2^40] (what the store writes), which keeps l inside float32.
-// M is set so that the weights so far lie well above 1 (decode: the largest at 2^8; prefill: the sum of 32 at 2^7 to 2^8) and
+// M is set so that the weights so far lie well above 1 (decode: the largest at 2^7; prefill: the sum of 32 at 2^6 to 2^7) and
 // follows them only when one might leave f16: P stays at or below 2^15 in decode, below 61440 in prefill.  So far above
-// 1, because f16 has no finer step than 2^-24: what rounds to zero lies below 2^-32 of the weights it stands beside, and the quiet
+// 1, because f16 has no finer step than 2^-24: what rounds to zero lies below 2^-31 of the weights it stands beside, and the quiet
 // keys of a long row count behind a loud one.
 //
 // Codes are converted to f16 (exact) in registers.  A query row is brought to a power of two of its own before it goes to

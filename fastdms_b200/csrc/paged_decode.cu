@@ -178,11 +178,13 @@ __device__ __forceinline__ void page_scores(const PageRegs<D>& p, const uint32_t
     }
 }
 
-// log2 of the largest weight when M is set, and how far one may grow until M moves.  With 11 and 4 more of the quiet weights count, and
-// 64 sequences ragged up to 16384 take 191.5 us in place of 190.2.
-constexpr float kTopWeight = 8.0f, kLag = 7.0f;
+// log2 of the largest weight when M is set, and of the most that one may be until M moves.  With 11 and 15 more of the quiet weights
+// count, and 64 sequences ragged up to 16384 take 191.5 us in place of 190.2.  What a weight may be is judged by the difference to M,
+// which is exact, while M +- a few is not where float32's steps are wider than these; 7, less than half a step of 16, is then
+// rounded away from or up to 8, and a weight's power never passes 15.
+constexpr float kTopWeight = 7.0f, kMostWeight = 15.0f;
 
-// Scores to weights, l, and P^T; `rows` of the page count.  M follows the maximum only when that is ahead by more than 2^7:
+// Scores to weights, l, and P^T; `rows` of the page count.  M follows the maximum only when that is ahead by more than 2^8:
 // P stays at or below 2^15 and most pages need no maximum over the keys and rescale nothing.
 // With FINE, for f16 outputs, whose own rounding is no larger than that of a weight to f16, also what that rounding left.
 template <int D, bool FINE>
@@ -196,13 +198,13 @@ __device__ __forceinline__ void page_weights(UnitState<D>& u, float (&s)[4], flo
         if (g + 8 >= rows) x[2] = x[3] = -INFINITY;
     }
     const float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
-    if (__any_sync(0xffffffffu, t0 > u.m[0] + (kTopWeight + kLag) || t1 > u.m[1] + (kTopWeight + kLag))) {
+    if (__any_sync(0xffffffffu, t0 - u.m[0] > kMostWeight || t1 - u.m[1] > kMostWeight)) {
         float top[2] = {t0, t1};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-            const float next = top[i] > u.m[i] + (kTopWeight + kLag) ? top[i] - kTopWeight : u.m[i];      // heads do not follow their neighbours
+            const float next = top[i] - u.m[i] > kMostWeight ? top[i] - kTopWeight : u.m[i];      // heads do not follow their neighbours
             const float r = next == u.m[i] ? 1.0f : paged_ex2(u.m[i] - next);
             u.m[i] = next;
             u.l[i] *= r;

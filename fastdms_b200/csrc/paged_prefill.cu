@@ -189,8 +189,9 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[8]
 constexpr float kMostWeight = 61440.0f;         // a sum of weights below this keeps each inside f16
 // log2 of what the sum of 32 weights is brought to, or up to a half below, when M is set.  Higher keeps more of the weights that f16
 // cannot hold and leaves less room until M has to move again: 2048 tokens over 16384 rows take 568 us with 7 and 571 with 8, 7 ragged
-// prompts 352 and 352 (head_dim 64), 392 and 394 (128).
-constexpr float kSetWeight = 8.0f;
+// prompts 352 and 352 (head_dim 64), 392 and 394 (128).  Less than 8, so that where float32's steps at M are 16 the largest weight
+// ends up at 1 and not at 2^16.
+constexpr float kSetWeight = 7.0f;
 
 // Exponents of 32 scores: x = s * factor * ks + log2 vs - ref, keys behind `seen` masked.
 __device__ __forceinline__ void exponents(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, float ref, bool cut, int seen,

@@ -132,8 +132,8 @@ def attention_tight(q, k, v, vs, last, scale, f16, terms=None):
     scales of the keys' blocks; `terms`: products of a score that are not zero.
 
     A weight is an f16 value, or for f16 outputs two of them: 2^-11 or 2^-22 of it, or 2^-25 where f16 has no finer steps (three
-    times: the value, the rest, a change of M).  The weights 2^(x + log2 vs - M) of a row sum to 2^7 at least (prefill; 2^8 in
-    decode), so that 3 * 2^-25 is 3 * 2^-32 of the sum of w_j vs_j at most; a key's term is that times v_j / vs_j."""
+    times: the value, the rest, a change of M).  The weights 2^(x + log2 vs - M) of a row sum to 2^6 at least (prefill; 2^7 in
+    decode), so that 3 * 2^-25 is 3 * 2^-31 of the sum of w_j vs_j at most; a key's term is that times v_j / vs_j."""
     n, d = q.shape
     out, lse = np.zeros((n, d)), np.full(n, -np.inf)
     tol, ltol = np.zeros((n, d)), np.zeros(n)
@@ -150,6 +150,6 @@ def attention_tight(q, k, v, vs, last, scale, f16, terms=None):
         mag = float((np.abs(k[:m]) @ np.abs(q[i])).max()) * abs(scale)
         ds = mag * ((d if terms is None else terms) + 4) * 2.0 ** -23 + (np.abs(s).max() * 1.45 + 64) * 2.0 ** -23
         tol[i] = (np.abs(v[:m]).T @ w) * ((2.0 ** -22 if f16 else 2.0 ** -11) + 2 * ds + m * 2.0 ** -24)
-        tol[i] += 3 * 2.0 ** -32 * (w * vs[:m]).sum() * (np.abs(v[:m]) / vs[:m, None]).sum(0)
+        tol[i] += 3 * 2.0 ** -31 * (w * vs[:m]).sum() * (np.abs(v[:m]) / vs[:m, None]).sum(0)
         ltol[i] = ds + m * 2.0 ** -24 + (abs(lse[i]) + 64) * 2.0 ** -23
     return out, lse, tol, ltol

@@ -336,6 +336,37 @@ def test_queries_at_the_ends_of_bfloat16(dev, power, wide):
         check_rows(n64(got)[0], None, want, "bf16")
 
 
+@pytest.mark.parametrize("form,seqs", [("decode", 600), ("prefill", 1)])
+def test_scores_whose_steps_are_coarse(dev, form, seqs):
+    """Scores of 2^24 to 2^29 times log2(e): what lies between two neighbouring float32 numbers there is the room that the weights
+    have, so that M and the bound of a weight are rounded themselves.  No weight may leave f16 for it."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
+    d, rows, heads = 64, 300, 24
+    k, v = np.zeros((rows, d)), np.ones((rows, d))
+    k[:, 0] = k[:, 2] = 1.0
+    k[200, 1], v[200] = 1.0, 2.0                                             # ahead of the keys before it by a few such steps
+    kc, vc, ks, vs, table = one_sequence(dev, k, v)
+    for dt in ("bf16", "f16"):
+        q = torch.zeros((1, heads, d), dtype=torch.float64)
+        for h in range(heads):
+            q[0, h, 0] = 2.0 ** (24 + h % 6)
+            q[0, h, 1] = 2.0 ** (1 + h // 6) * (1 + (h % 2) / 2)
+            q[0, h, 2] = 2.0 ** (1 + h % 5)
+        scale = float(np.log(2.0))
+        if dt == "f16":                                                      # the same scores from queries that f16 holds
+            q, scale = q * 2.0 ** -15, scale * 2.0 ** 15
+        q = q.to(DT[dt])
+        assert (q[0, :, 0] > 0).all() and torch.isfinite(q.float()).all()
+        args = (q.to(dev).expand(seqs, heads, d).contiguous(), kc, vc, ks, vs, table.expand(seqs, table.shape[1]), i32([rows] * seqs, dev))
+        lse = torch.empty((seqs, heads), device=dev)
+        if form == "decode":
+            got = paged_decode_attention(*args, scale, lse_out=lse)
+        else:
+            got = paged_prefill_attention(*args, i32([0, 1], dev), scale, lse_out=lse.t())
+        assert torch.isfinite(got.float()).all() and torch.isfinite(lse).all()
+        assert (got >= 1.0).all() and (got <= 2.0).all()
+
+
 # ---- caches --------------------------------------------------------------------------------------------------------
 
 def test_a_cache_without_blocks(dev):
