@@ -192,6 +192,10 @@ constexpr float kMostWeight = 61440.0f;         // a sum of weights below this k
 // prompts 352 and 352 (head_dim 64), 392 and 394 (128).  Less than 8, so that where float32's steps at M are 16 the largest weight
 // ends up at 1 and not at 2^16.
 constexpr float kSetWeight = 7.0f;
+// From here on whole numbers are not all float32 numbers, and M would differ from s * factor * ks, which a multiply-add takes
+// exactly, by a rounding that no weight survives.  Such a row gets M = inf, under which all its weights are 0, and is computed by itself
+// in the end.
+constexpr float kCoarse = 0x1p24f;
 
 // Exponents of 32 scores: x = s * factor * ks + log2 vs - ref, keys behind `seen` masked.
 __device__ __forceinline__ void exponents(const uint32_t (&s)[32], float factor, const float4& p0, const float4& p1, float ref, bool cut, int seen,
@@ -332,6 +336,61 @@ __device__ __forceinline__ void issue_values(uint32_t base, uint32_t tmem, int t
             mma_ts(tmem + L::kO + D * ti, tmem + (L::kBufs * ti + buf) * kHalf + 32 + 8 * i, v + (i * 2048 >> 4), instruction(D, true), true);
     tc_commit(&sh.pv_done[ti][buf]);
     if (again) tc_commit(&sh.v_empty[st]);
+}
+
+// One row by a warp, its weights in float32: the first `keys` cached rows from row `from` of the sequence on.  `q`: the row's f16
+// elements in shared memory, of row r of its tile; a lane has a key, then D / 32 channels.
+template <int D>
+__device__ __forceinline__ void whole_row(const PagedCache& c, const uint8_t* q, int r, float factor, int seq, int head, int from, int keys,
+                                          float (&acc)[D / 32], float& m, float& l) {
+    const int lane = threadIdx.x & 31;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+    for (int base = 0; base < keys; base += 32) {
+        const int at = from + base + lane, in_block = at & ((1 << c.shift) - 1);
+        int blk = base + lane < keys ? c.tables[seq * c.table_stride + (at >> c.shift)] : -1;
+        if (blk >= c.num_blocks) blk = -1;
+        float x = -INFINITY, inv = 1.0f;
+        if (blk >= 0) {
+            const uint8_t* k = c.k + blk * c.k_sb + head * c.k_sh + in_block * c.k_sr;
+            const float vs = paged_v_scale(c.v_scale[(int64_t)blk * c.heads + head]);
+            float dot = 0.0f;
+#pragma unroll 1
+            for (int i = 0; i < D / 8; ++i) {
+                const uint4 w = *(const uint4*)(q + (i >> 3) * kSlab + (((i & 7) ^ (r & 7)) << 4));
+                const uint2 b = *(const uint2*)(k + 8 * i);
+                const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const __half2 h = *(const __half2*)&y[e >> 1];
+                    dot = fmaf(e & 1 ? __high2float(h) : __low2float(h), e4m3_to_float((uint8_t)((e < 4 ? b.x : b.y) >> (8 * (e & 3)))), dot);
+                }
+            }
+            x = fmaf(dot, factor * c.k_scale[(int64_t)blk * c.heads + head], paged_lg2(vs));
+            inv = __frcp_rn(vs);
+        }
+        float top = x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.0f : next, scale = paged_ex2(m - ref), p = paged_ex2(x - ref);
+        m = next;
+        l = fmaf(l, scale, p * inv);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] *= scale;
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) {
+            const int b = __shfl_sync(0xffffffffu, blk, j);
+            const float w = __shfl_sync(0xffffffffu, p, j);
+            if (b < 0) continue;
+            const uint8_t* v = c.v + b * c.v_sb + head * c.v_sh + ((from + base + j) & ((1 << c.shift) - 1)) * c.v_sr + lane * (D / 32);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, e4m3_to_float(v[i]), acc[i]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 }
 
 template <int D, bool BF16>
@@ -480,7 +539,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                         const float top = largest(s_at + 32 * c, factor, page + 2 * c, seen - 32 * c);
                         if (!known) to = ceilf(top);
                     }
-                    const float next = moves ? fmaxf(m, to - kSetWeight) : m;
+                    float next = moves ? fmaxf(m, to - kSetWeight) : m;
+                    if (fabsf(next) >= kCoarse && next != -INFINITY) next = INFINITY;
                     const float r = next == m ? 1.0f : paged_ex2(m - next);
                     m = next;
                     l *= r;
@@ -517,6 +577,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
             if (halves > 0 && ok) ok = warp_wait(&sh.pv_done[ti][(halves - 1) % L::kBufs], ((halves - 1) / L::kBufs) & 1, give_up);
             tc_fence_after();
             const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
+            const bool again = live && m == INFINITY, write = live && !again;
             uint16_t* out = a.out + tok * a.o_st + (int64_t)hq * a.o_sh;
             float* mine = a.parts + (((int64_t)blockIdx.z * a.tokens + tok) * (a.c.heads * a.group) + hq) * (D + 4);
 #pragma unroll
@@ -528,10 +589,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     tmem_load(o_at + 16 * c, o);
                     tc_wait_ld(o);
                 }
-                if (live && a.splits > 1) {
+                if (write && a.splits > 1) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) *(uint4*)(mine + 16 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                } else if (live) {
+                } else if (write) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 8) {
                         uint32_t y[4];
@@ -542,8 +603,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) paged_prefill_kernel(PrefillAr
                     }
                 }
             }
-            if (live && a.splits > 1) *(float2*)(mine + D) = make_float2(m, l);
-            else if (live && a.lse) a.lse[(int64_t)hq * a.lse_sh + tok * a.lse_st] = kPagedLn2 * (m + paged_lg2(l));
+            if (write && a.splits > 1) *(float2*)(mine + D) = make_float2(m, l);
+            else if (write && a.lse) a.lse[(int64_t)hq * a.lse_sh + tok * a.lse_st] = kPagedLn2 * (m + paged_lg2(l));
+            for (unsigned todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
+                const int src = __ffs(todo) - 1, row = (r & ~31) + src;
+                const int keys = (int)min(max(__shfl_sync(0xffffffffu, last, src) + 1, (int64_t)0), here);
+                float acc[D / 32], rm, rl;
+                whole_row<D>(a.c, tile + L::kQ + ti * L::kTile + row * 128, row, __shfl_sync(0xffffffffu, factor, src), seq, head, from, keys, acc, rm, rl);
+                const int64_t row_tok = __shfl_sync(0xffffffffu, tok, src);
+                const int row_hq = __shfl_sync(0xffffffffu, hq, src);
+                if (a.splits > 1) {
+                    float* part = a.parts + (((int64_t)blockIdx.z * a.tokens + row_tok) * (a.c.heads * a.group) + row_hq) * (D + 4);
+#pragma unroll
+                    for (int i = 0; i < D / 32; i += 2) *(float2*)(part + lane * (D / 32) + i) = make_float2(acc[i], acc[i + 1]);
+                    if (lane == 0) *(float2*)(part + D) = make_float2(rm, rl);
+                } else {
+                    const float by = rl > 0.0f || rl != rl ? __frcp_rn(rl) : 0.0f;
+                    uint16_t* to = a.out + row_tok * a.o_st + (int64_t)row_hq * a.o_sh + lane * (D / 32);
+#pragma unroll
+                    for (int i = 0; i < D / 32; i += 2) *(uint32_t*)(to + i) = pack_pair<BF16>(acc[i] * by, acc[i + 1] * by);
+                    if (lane == 0 && a.lse) a.lse[(int64_t)row_hq * a.lse_sh + row_tok * a.lse_st] = kPagedLn2 * (rm + paged_lg2(rl));
+                }
+            }
+            __syncwarp();
             // NaN codes of V in steps that not every row sees whole were left out of the products: into the rows that see them
             const int lo = *(volatile int*)&sh.nan_lo, hi = *(volatile int*)&sh.nan_hi;
             if (live && lo <= hi)

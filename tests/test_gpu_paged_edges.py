@@ -367,6 +367,46 @@ def test_scores_whose_steps_are_coarse(dev, form, seqs):
         assert (got >= 1.0).all() and (got <= 2.0).all()
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("d,dt,power", [(64, "bf16", 28), (128, "bf16", 40), (64, "bf16", 100), (128, "f16", 13)])
+def test_scores_beyond_float32s_whole_numbers(dev, d, dt, power, wide):
+    """Scores so loud that one key takes all: its row of V comes out, from decode and from prefill, of tokens that see it and of
+    tokens that do not; rows of ordinary queries between them give the bits that they give alone."""
+    from fastdms_b200.layers.paged_attention import paged_decode_attention, paged_prefill_attention
+    rng = np.random.default_rng(power)
+    heads, group, bs, rows, n = 1, 8, 16, 700, 40
+    (kc, vc, ks, vs, table), (codes, scale, tab) = build_case(rng, [rows], heads, bs, d, dev, loud=False)
+    if wide:
+        table = wide_table(table, bs)
+    x = rng.standard_normal((n, group, d))
+    calm = torch.from_numpy(x).to(DT[dt])
+    x[:, ::2] *= 2.0 ** power
+    q = torch.from_numpy(x).to(DT[dt])
+    mul = 2.0 ** 15 if dt == "f16" else 1.0
+    k, v = (O.rows_of(codes[c], scale[c], tab[0], rows, 0, bs) for c in range(2))
+    args = (kc, vc, ks, vs, table, i32([rows], dev))
+    lse = torch.empty((group, n), device=dev)
+    pre = n64(paged_prefill_attention(q.to(dev), *args, i32([0, n], dev), mul, lse_out=lse))
+    dec = n64(paged_decode_attention(q[-1:].to(dev), *args, mul))
+    if mul == 1.0:
+        ref = n64(paged_prefill_attention(calm.to(dev), *args, i32([0, n], dev), mul))
+        assert np.array_equal(pre[:, 1::2], ref[:, 1::2])
+    half, checked = torch.finfo(DT[dt]).eps / 2, 0
+    for i in range(n):
+        for h in range(0, group, 2):
+            s = k[:rows - n + i + 1] @ n64(q)[i, h] * mul
+            top = np.sort(s)[-2:]
+            mag = (np.abs(k) @ np.abs(n64(q)[i, h])).max() * mul
+            if top[1] - top[0] <= 64 + mag * (d + 8) * 2.0 ** -22:          # nearer than the scores' own roundings
+                continue
+            want = v[s.argmax()]
+            checked += 1
+            for got in (pre[i, h], dec[0, h])[:2 if i == n - 1 else 1]:
+                assert (np.abs(got - want) <= half * np.abs(want)).all()
+            assert abs(float(lse[h, i]) - top[1]) <= mag * (d + 8) * 2.0 ** -22
+    assert checked > n
+
+
 # ---- caches --------------------------------------------------------------------------------------------------------
 
 def test_a_cache_without_blocks(dev):
