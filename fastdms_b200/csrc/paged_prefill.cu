@@ -14,9 +14,9 @@
 // their product.  Two tiles per CTA halve the conversions.  Every wait is bounded; when one runs out the CTA raises
 // FDMS_DEV_WAIT_TIMEOUT, lets what it issued complete, gives its tensor memory back and returns.
 //
-// Measured (32 q heads on 8 KV heads, a B200): 2048 tokens over 16384 rows at head_dim 128 take 571 us in bf16 (902 TFLOP/s) and 795 in
-// f16, whose weights take a second product; 7 ragged prompts of up to 3001 tokens at head_dim 64 353 and 440 us.  No unit bounds
-// it: of the SMs' active time the tensor pipe works 48 %, the unit of the exponential 49 %, and an instruction issues in 46 % of the
+// Measured (32 q heads on 8 KV heads, a B200): 2048 tokens over 16384 rows at head_dim 128 take 579 us in bf16 (890 TFLOP/s) and 741 in
+// f16, whose weights take a second product; 7 ragged prompts of up to 3001 tokens at head_dim 64 355 and 431 us.  No unit bounds
+// it: of the SMs' active time the tensor pipe works 48 %, the unit of the exponential 48 %, and an instruction issues in 45 % of the
 // cycles.  A step of 128 keys takes about 2.4 us at both head sizes, where its exponentials need 1.1: each softmax warp goes through
 // load, weights, store and arrival in turn, and the two of a scheduler do not fill each other's waits.  256 equal CTAs on 148 SMs
 // run in two waves and leave 14 % of them idle.
